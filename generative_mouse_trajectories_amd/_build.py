@@ -12,7 +12,9 @@ CSRC = os.path.join(PKG, 'csrc')
 OBJ = os.path.join(CSRC, 'build')
 LIB = os.path.join(PKG, 'libgmt_hip.so')
 HIPCC = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
-BASE_FLAGS = ['--offload-arch=gfx950', '-O3', '-fPIC', '-std=c++17', '-Wall', '-Wno-unused-function']
+BASE_FLAGS = ['--offload-arch=gfx950', '-O3', '-fPIC', '-std=c++17', '-Wall', '-Wno-unused-function',
+              # no packed fp32 arithmetic: some of its forms have given wrong results on this hardware
+              '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 # per-file extra flags: the f64 telemetry kernel must not fuse a*b+c (bit parity with MT.rs)
 EXTRA = {'telemetry.hip': ['-ffp-contract=off'],
          # the per-trajectory loss arithmetic follows the CPU reference operation by operation (no fused multiply-add)
