@@ -10,7 +10,7 @@ import torch
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, 'libgmt_hip.so')
-ABI_VERSION = 9
+ABI_VERSION = 10
 _lib = None
 
 ERRORS = {-1: 'bad argument (null pointer / shape / alignment)', -2: 'unsupported configuration',
@@ -84,6 +84,21 @@ class HeadBwdArgs(ctypes.Structure):
         + [(n, c_i) for n in ('Bp', 'H', 'a2_pitch')] + [('slope', c_f), ('dropout_p', c_f), ('seed', ctypes.c_uint)]
 
 
+class ConvArgs(ctypes.Structure):
+    _fields_ = [(n, c_p) for n in ('x', 'x_scale', 'w', 'bias', 'state', 'lengths', 'y', 'state_out', 'dy', 'dstate_out', 'dx',
+                                   'dparam', 'dstate', 'workspace')] \
+        + [(n, c_ll) for n in ('workspace_floats', 'x_t', 'x_b', 'dy_t', 'dy_b')] \
+        + [(n, c_i) for n in ('L', 'B', 'C', 'K', 'bf16', 'silu')]
+
+
+class ScanArgs(ctypes.Structure):
+    _fields_ = [(n, c_p) for n in ('x', 'dt', 'z', 'x_scale', 'dt_scale', 'z_scale', 'Bm', 'Cm', 'A', 'D', 'dt_bias', 'state', 'lengths',
+                                   'y', 'state_out', 'ck', 'dy', 'dstate_out', 'dx', 'ddt', 'dz', 'dB', 'dC', 'dparam', 'dstate',
+                                   'workspace')] \
+        + [(n, c_ll) for n in ('workspace_floats', 'x_t', 'x_b', 'dt_t', 'dt_b', 'z_t', 'z_b', 'B_t', 'B_b', 'B_g', 'C_t', 'C_b',
+                               'C_g', 'dy_t', 'dy_b')] + [(n, c_i) for n in ('L', 'B', 'C', 'N', 'G', 'bf16')]
+
+
 SN_MAX_LAYERS = 8
 
 _SIGS = {
@@ -141,6 +156,18 @@ _SIGS = {
     'gmt_bf16_gen_rollout_fwd': [c_p, c_p],
     'gmt_bf16_gen_rollout_bwd': [c_p, c_p],
     'gmt_gen_rollout_bwd': [c_p, c_p],
+    'gmt_causal_conv_fwd': [c_p, c_p],
+    'gmt_causal_conv_bwd_workspace_floats': [c_p, c_p],
+    'gmt_causal_conv_bwd': [c_p, c_p],
+    'gmt_causal_conv_step': [c_p, c_p, c_p],
+    'gmt_selective_scan_workspace': [c_p, c_p, c_p, c_p],
+    'gmt_selective_scan_fwd': [c_p, c_p],
+    'gmt_selective_scan_bwd': [c_p, c_p],
+    'gmt_selective_scan_step': [c_p, c_p, c_p],
+    'gmt_ckpt8_pack': [c_p, c_ll, c_ll, c_p, c_p, c_ll, c_i, c_i, c_i, c_p],
+    'gmt_ckpt8_unpack': [c_p, c_p, c_p, c_ll, c_i, c_i, c_p],
+    'gmt_ckpt8_wgrad_workspace_floats': [c_ll, c_i, c_i, c_p],
+    'gmt_ckpt8_wgrad': [c_p, c_ll, c_p, c_p, c_p, c_ll, c_i, c_i, c_i, c_i, c_p, c_ll, c_p],
 }
 
 

@@ -1,0 +1,358 @@
+// 8-bit activation checkpoints, and the weight gradient that reads them.
+//
+// A row is cut into blocks of 32 channels.  A block is stored as int8 codes q and one exponent byte s = e + 127 and stands for
+// q 2^e:  e = the smallest exponent in -118 .. 121 with max|x| <= 127 * 2^e, q = x 2^-e rounded to nearest even (|q| <= 127).  The
+// scale is a power of two, so that packing rounds once, a code's value is exact in fp32 and in bf16 (7 bits), and its error
+// is at most 2^(e-1), that is max|x| / 127.  The exponent's range keeps 2^-e, and every value that a block of normal numbers stands
+// for, a normal number.  A block that holds an infinity or a NaN stands for NaN throughout: s = 255, q = 0.
+//
+// Weight gradient: dW[n][i] = sum_r dY[r][n] Xhat[r][i], db[n] = sum_r dY[r][n].  Xhat is exact in bf16; an fp32 dY is exactly
+// the sum of three bf16 numbers (its 24 mantissa bits cut into 8 + 8 + 8), so three bf16 MFMAs give the products without a
+// rounding, accumulated in fp32, at 16 / 3 the rate of the fp32 matrix instruction.  A bf16 dY is one.
+#include "ssm_common.h"
+#include "bf16_maps.h"
+
+namespace {
+
+using namespace gmt_ssm;
+
+constexpr int BLK = 32;
+
+template <class T, int V> __device__ __forceinline__ void load_vec(const typename T::raw* p, float (&o)[V])
+{
+    if constexpr (V == 1) o[0] = to_f(*p);
+    else {
+        typedef typename T::raw vec __attribute__((ext_vector_type(V)));
+        const vec v = *reinterpret_cast<const vec*>(p);
+#pragma unroll
+        for (int i = 0; i < V; ++i) o[i] = to_f((typename T::raw)v[i]);
+    }
+}
+
+// 32 / V lanes share a block: V = 16 bytes of elements where the layout allows, else 1
+template <class T, int V>
+__global__ __launch_bounds__(256)
+void pack_kernel(const typename T::raw* __restrict__ x, long long x_t, long long x_b, signed char* __restrict__ codes,
+                 unsigned char* __restrict__ scale, long long rows, int B, int C, int nb)
+{
+    constexpr int LPB = BLK / V;
+    const long long total = rows * nb * LPB, step = (long long)gridDim.x * 256;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += step) {
+        const long long blk = i / LPB, row = blk / nb;
+        const int part = (int)(i % LPB), c = (int)(blk % nb) * BLK + part * V;
+        const bool in = c < C;                          // (C % V == 0)
+        float v[V] = {};
+        if (in) load_vec<T, V>(x + row / B * x_t + row % B * x_b + c, v);
+        unsigned m = 0;                                 // largest magnitude by its bits: NaN > infinity > numbers
+#pragma unroll
+        for (int k = 0; k < V; ++k) m = max(m, __float_as_uint(v[k]) & 0x7fffffffu);
+#pragma unroll
+        for (int o = 1; o < LPB; o <<= 1) m = max(m, (unsigned)__shfl_xor((int)m, o, 64));
+        int e = (int)(m >> 23) - 133 + ((m & 0x7fffffu) > 0x7e0000u);
+        e = min(max(e, -118), 121);
+        const bool bad = m >= 0x7f800000u;
+        const float inv = __uint_as_float((unsigned)(127 - e) << 23);
+        if (in) {
+            signed char q[V];
+#pragma unroll
+            for (int k = 0; k < V; ++k) q[k] = bad ? 0 : (signed char)(int)fminf(fmaxf(rintf(v[k] * inv), -127.f), 127.f);
+            if constexpr (V == 1) codes[row * C + c] = q[0];
+            else {
+                typedef signed char vec __attribute__((ext_vector_type(V)));
+                vec o;
+#pragma unroll
+                for (int k = 0; k < V; ++k) o[k] = q[k];
+                *reinterpret_cast<vec*>(codes + row * C + c) = o;
+            }
+            if (part == 0) scale[blk] = bad ? 255 : (unsigned char)(e + 127);
+        }
+    }
+}
+
+template <class T, int V>
+__global__ __launch_bounds__(256)
+void unpack_kernel(const signed char* __restrict__ codes, const unsigned char* __restrict__ scale, typename T::raw* __restrict__ out,
+                   long long rows, int C, int nb)
+{
+    const int cv = C / V;
+    const long long total = rows * cv, step = (long long)gridDim.x * 256;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += step) {
+        const long long row = i / cv;
+        const int c = (int)(i % cv) * V;
+        const unsigned char s = scale[row * nb + c / BLK];
+        if constexpr (V == 1) out[i] = from_f<T>(to_f(Q8::raw{codes[i], s}));
+        else {
+            typedef signed char qvec __attribute__((ext_vector_type(V)));
+            typedef typename T::raw vec __attribute__((ext_vector_type(V)));
+            const qvec q = *reinterpret_cast<const qvec*>(codes + i * V);
+            vec o;
+#pragma unroll
+            for (int k = 0; k < V; ++k) o[k] = from_f<T>(to_f(Q8::raw{(signed char)q[k], s}));
+            *reinterpret_cast<vec*>(out + i * V) = o;
+        }
+    }
+}
+
+// ---- weight gradient.  A workgroup owns a 128 (n) x 128 (i) tile for one slab of rows, 4 waves of 64 x 64 (2 x 2 accumulators of
+// 32 x 32).  Both operands have the contraction index as their ROW: stages of 32 rows go global -> registers -> LDS as bf16
+// [32][128] images (dY as PL of them), requested one stage ahead, and the fragments (8 consecutive rows of one column a lane)
+// come out of ds_read_b64_tr_b16.  Chunk c (16 bytes) of row r sits at c ^ ((r & 3) << 2): the four rows that half a wave reads
+// together fall on different banks.  Slabs are summed in a fixed order.
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int WG_K = 32, WG_T = 128, WG_IMG = WG_K * WG_T * 2;     // rows a stage, tile width, bytes an image
+
+__device__ __forceinline__ int img_addr(int row, int col) { return row * 256 + (((col >> 3) ^ ((row & 3) << 2)) << 4) + (col & 7) * 2; }
+
+__device__ __forceinline__ bf16x8 tr_frag(const char* img, int col0, int s, int lane)
+{
+    s16x4 h[2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        int row, col;
+        gmt_bf16_maps::wg_tr_lane(lane, col0, s, half, row, col);
+        h[half] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)(img + img_addr(row, col)));
+    }
+    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// the high halves of two floats as a pair of bf16 (cut, not rounded)
+__device__ __forceinline__ unsigned hi_pair(float a, float b) { return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u); }
+
+// T: type of dY; YV: dY is read 4 elements at a time (16 or 8 bytes); XV: codes 16 at a time
+template <class T, bool YV, bool XV>
+__global__ __launch_bounds__(256, 2)
+void wgrad8_kernel(const typename T::raw* __restrict__ dY, long long ldy, const signed char* __restrict__ codes,
+                   const unsigned char* __restrict__ scale, float* __restrict__ out, long long R, int N, int I, int ks, long long rows_per_slab,
+                   int want_db)
+{
+    constexpr int PL = __is_same(T, F32) ? 3 : 1;
+    __shared__ __align__(16) char lds[2][(PL + 1) * WG_IMG];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wp = wave >> 1, wq = wave & 1;
+    const int n_t = (N + WG_T - 1) / WG_T, i_t = (I + WG_T - 1) / WG_T, tiles = n_t * i_t;
+    // block = xcd + 8 (tile + tiles * group), slab = 8 group + xcd: the tiles of one slab share an XCD's L2
+    const int rest = blockIdx.x >> 3, tile = rest % tiles, slab = rest / tiles * 8 + (blockIdx.x & 7);
+    if (slab >= ks) return;
+    const int n0 = tile % n_t * WG_T, i0 = tile / n_t * WG_T;
+    const long long r0 = slab * rows_per_slab, r1 = min(r0 + rows_per_slab, R);
+    const int nb = (I + BLK - 1) / BLK;
+
+    const int yc = (tid & 31) * 4, yr = tid >> 5;       // dY: 4 columns, rows yr + 8 j
+    const int xc = (tid & 7) * 16, xr = tid >> 3;       // codes: 16 columns of one row (half a block)
+    struct Stage { float y[4][4]; signed char q[16]; unsigned char s; };
+    float colsum[4] = {};
+    auto request = [&](Stage& st, long long r) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const long long rr = r + yr + 8 * j;
+            const bool in = rr < r1;
+            const typename T::raw* p = dY + rr * ldy + n0 + yc;
+            if constexpr (YV) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) st.y[j][k] = 0.f;
+                if (in && n0 + yc < N) load_vec<T, 4>(p, st.y[j]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) st.y[j][k] = in && n0 + yc + k < N ? to_f(p[k]) : 0.f;
+            }
+        }
+        const long long rr = r + xr;
+        const bool in = rr < r1 && i0 + xc < I;
+        st.s = 127;
+        if (in) st.s = scale[rr * nb + (i0 + xc) / BLK];
+        const signed char* p = codes + rr * I + i0 + xc;
+        typedef signed char qvec __attribute__((ext_vector_type(16)));
+        if constexpr (XV) {
+            qvec v = {};
+            if (in) v = *reinterpret_cast<const qvec*>(p);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) st.q[k] = v[k];
+        } else {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) st.q[k] = in && i0 + xc + k < I ? p[k] : (signed char)0;
+        }
+    };
+    auto put = [&](const Stage& st, char* img) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int row = yr + 8 * j;
+            float v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) { v[k] = st.y[j][k]; colsum[k] += v[k]; }
+#pragma unroll
+            for (int pl = 0; pl < PL; ++pl) {
+                uint2 w = make_uint2(hi_pair(v[0], v[1]), hi_pair(v[2], v[3]));
+                *reinterpret_cast<uint2*>(img + pl * WG_IMG + img_addr(row, yc)) = w;
+                if (pl + 1 < PL) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) v[k] -= __uint_as_float(__float_as_uint(v[k]) & 0xffff0000u);
+                }
+            }
+        }
+        const float sc = __uint_as_float((unsigned)st.s << 23);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            unsigned w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w[k] = hi_pair((float)st.q[8 * h + 2 * k] * sc, (float)st.q[8 * h + 2 * k + 1] * sc);
+            *reinterpret_cast<uint4*>(img + PL * WG_IMG + img_addr(xr, xc + 8 * h)) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    };
+    f32x16 acc[2][2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+
+    Stage st;
+    const int nk = r1 > r0 ? (int)((r1 - r0 + WG_K - 1) / WG_K) : 0;
+    if (nk > 0) { request(st, r0); put(st, lds[0]); }
+    __syncthreads();
+    for (int t = 0; t < nk; ++t) {
+        if (t + 1 < nk) request(st, r0 + (long long)(t + 1) * WG_K);
+        const char* img = lds[t & 1];
+#pragma unroll
+        for (int s = 0; s < WG_K / 16; ++s) {
+            bf16x8 q[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) q[j] = tr_frag(img + PL * WG_IMG, wq * 64 + j * 32, s, lane);
+#pragma unroll
+            for (int pl = 0; pl < PL; ++pl) {
+                bf16x8 p[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) p[i] = tr_frag(img + pl * WG_IMG, wp * 64 + i * 32, s, lane);
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(p[i], q[j], acc[i][j], 0, 0, 0);
+            }
+        }
+        if (t + 1 < nk) put(st, lds[(t + 1) & 1]);
+        __syncthreads();                                // stage t + 1 is written; everybody is done with stage t
+    }
+    const int lo = lane & 31, hi = lane >> 5;
+    float* slab_out = out + (long long)slab * ((long long)N * I + N);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int col = i0 + wq * 64 + j * 32 + lo;
+        if (col < I) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int n = n0 + wp * 64 + i * 32 + (r & 3) + 8 * (r >> 2) + 4 * hi;
+                    if (n < N) slab_out[(long long)n * I + col] = acc[i][j][r];
+                }
+        }
+    }
+    if (want_db && i0 == 0) {                           // (uniform) column sums: 8 row groups of 32 threads x 4 columns
+        float (*sum)[WG_T] = reinterpret_cast<float (*)[WG_T]>(lds[0]);
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sum[yr][yc + k] = colsum[k];
+        __syncthreads();
+        if (tid < WG_T && n0 + tid < N) {
+            float v = 0.f;
+#pragma unroll
+            for (int r = 0; r < 8; ++r) v += sum[r][tid];
+            slab_out[(long long)N * I + n0 + tid] = v;
+        }
+    }
+}
+
+// Slabs: two workgroups a CU in all, slabs of four stages or more
+void wgrad8_split(long long R, int N, int I, int& ks, long long& rows)
+{
+    const long long tiles = (long long)((N + WG_T - 1) / WG_T) * ((I + WG_T - 1) / WG_T);
+    long long k = (512 + tiles - 1) / tiles;
+    const long long most = (R + 4 * WG_K - 1) / (4 * WG_K);
+    if (k > most) k = most;
+    if (k < 1) k = 1;
+    rows = ((R + k - 1) / k + WG_K - 1) / WG_K * WG_K;
+    ks = (int)((R + rows - 1) / rows);
+}
+
+template <class T> int launch_wgrad8(const void* dY, long long ldy, const signed char* codes, const unsigned char* scale, float* slab, long long R,
+                                     int N, int I, int ks, long long rows, int want_db, hipStream_t stream)
+{
+    const bool yv = N % 4 == 0 && ldy % 4 == 0 && ((uintptr_t)dY % (4 * sizeof(typename T::raw))) == 0;
+    const bool xv = I % 16 == 0 && ((uintptr_t)codes & 15) == 0;
+    const long long tiles = (long long)((N + WG_T - 1) / WG_T) * ((I + WG_T - 1) / WG_T), grid = 8 * tiles * ((ks + 7) / 8);
+    if (grid >= (1LL << 24)) return GMT_ERR_UNSUPPORTED;
+#define GMT_WG(YV, XV)                                                                                                         \
+    hipLaunchKernelGGL((wgrad8_kernel<T, YV, XV>), dim3((unsigned)grid), dim3(256), 0, stream, (const typename T::raw*)dY, ldy, codes, \
+                       scale, slab, R, N, I, ks, rows, want_db)
+    if (yv) { if (xv) GMT_WG(true, true); else GMT_WG(true, false); }
+    else { if (xv) GMT_WG(false, true); else GMT_WG(false, false); }
+#undef GMT_WG
+    GMT_LAUNCH_CHECK();
+    return GMT_OK;
+}
+
+}  // namespace
+
+extern "C" int gmt_ckpt8_pack(const void* x, long long x_t, long long x_b, signed char* codes, unsigned char* scale, long long T, int B,
+                              int C, int bf16, hipStream_t stream)
+{
+    GMT_CHECK_ARG(x && codes && scale && T > 0 && B > 0 && C > 0);
+    const int esz = bf16 ? 2 : 4, V = 16 / esz, nb = (C + BLK - 1) / BLK;
+    const bool vec = C % V == 0 && x_t % V == 0 && x_b % V == 0 && ((uintptr_t)x & 15) == 0 && ((uintptr_t)codes % V) == 0;
+    const long long rows = T * B;
+    const int grid = gmt_grid_1d(rows * nb * (vec ? BLK / V : BLK), 256, 256 * 16);
+    if (bf16) {
+        if (vec) hipLaunchKernelGGL((pack_kernel<B16, 8>), dim3(grid), dim3(256), 0, stream, (const unsigned short*)x, x_t, x_b, codes, scale, rows, B, C, nb);
+        else hipLaunchKernelGGL((pack_kernel<B16, 1>), dim3(grid), dim3(256), 0, stream, (const unsigned short*)x, x_t, x_b, codes, scale, rows, B, C, nb);
+    } else {
+        if (vec) hipLaunchKernelGGL((pack_kernel<F32, 4>), dim3(grid), dim3(256), 0, stream, (const float*)x, x_t, x_b, codes, scale, rows, B, C, nb);
+        else hipLaunchKernelGGL((pack_kernel<F32, 1>), dim3(grid), dim3(256), 0, stream, (const float*)x, x_t, x_b, codes, scale, rows, B, C, nb);
+    }
+    GMT_LAUNCH_CHECK();
+    return GMT_OK;
+}
+
+extern "C" int gmt_ckpt8_unpack(const signed char* codes, const unsigned char* scale, void* out, long long rows, int C, int bf16, hipStream_t stream)
+{
+    GMT_CHECK_ARG(out && codes && scale && rows > 0 && C > 0);
+    const int V = bf16 ? 8 : 4, nb = (C + BLK - 1) / BLK;
+    const bool vec = C % V == 0 && ((uintptr_t)out & 15) == 0 && ((uintptr_t)codes % V) == 0;
+    const int grid = gmt_grid_1d(rows * (vec ? C / V : C), 256, 256 * 16);
+    if (bf16) {
+        if (vec) hipLaunchKernelGGL((unpack_kernel<B16, 8>), dim3(grid), dim3(256), 0, stream, codes, scale, (unsigned short*)out, rows, C, nb);
+        else hipLaunchKernelGGL((unpack_kernel<B16, 1>), dim3(grid), dim3(256), 0, stream, codes, scale, (unsigned short*)out, rows, C, nb);
+    } else {
+        if (vec) hipLaunchKernelGGL((unpack_kernel<F32, 4>), dim3(grid), dim3(256), 0, stream, codes, scale, (float*)out, rows, C, nb);
+        else hipLaunchKernelGGL((unpack_kernel<F32, 1>), dim3(grid), dim3(256), 0, stream, codes, scale, (float*)out, rows, C, nb);
+    }
+    GMT_LAUNCH_CHECK();
+    return GMT_OK;
+}
+
+extern "C" int gmt_ckpt8_wgrad_workspace_floats(long long R, int N, int I, long long* floats_out)
+{
+    GMT_CHECK_ARG(R > 0 && N > 0 && I > 0 && floats_out);
+    int ks; long long rows;
+    wgrad8_split(R, N, I, ks, rows);
+    *floats_out = ks > 1 ? ks * ((long long)N * I + N) : 0;
+    return GMT_OK;
+}
+
+extern "C" int gmt_ckpt8_wgrad(const void* dY, long long ldy, const signed char* codes, const unsigned char* scale, float* dW_db, long long R,
+                               int N, int I, int bf16, int want_db, float* workspace, long long workspace_floats, hipStream_t stream)
+{
+    GMT_CHECK_ARG(dY && codes && scale && dW_db && R > 0 && N > 0 && I > 0 && ldy >= N);
+    int ks; long long rows;
+    wgrad8_split(R, N, I, ks, rows);
+    const long long n = (long long)N * I + (want_db ? N : 0), pitch = (long long)N * I + N;
+    if (ks > 1 && (!workspace || workspace_floats < ks * pitch)) return GMT_ERR_WORKSPACE;
+    float* slab = ks > 1 ? workspace : dW_db;
+    const int rc = bf16 ? launch_wgrad8<B16>(dY, ldy, codes, scale, slab, R, N, I, ks, rows, want_db, stream)
+                        : launch_wgrad8<F32>(dY, ldy, codes, scale, slab, R, N, I, ks, rows, want_db, stream);
+    if (rc || ks == 1) return rc;
+    return launch_slab_reduce(workspace, dW_db, n, pitch, ks, stream);
+}

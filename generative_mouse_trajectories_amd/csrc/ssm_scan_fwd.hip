@@ -1,0 +1,273 @@
+// Selective scan, forward (ssm_scan.h has the formulas and the layout), its single-step form, and the segment chain that the
+// backward pass shares.
+#include "ssm_scan.h"
+
+namespace {
+
+using namespace gmt_ssm;
+
+// what a launch writes: y; y and the kept states; the kept states alone; a segment's (h_loc, S)
+enum Mode { OUT = 0, TRAIN = 1, STATES = 2, LOCAL = 3 };
+
+template <class T, class M, int NP, int MODE, bool GATED>
+__global__ __launch_bounds__(256)
+void scan_fwd_kernel(ScanArgs<T, M> a)
+{
+    constexpr bool Y = MODE == OUT || MODE == TRAIN, KEEP = MODE == TRAIN || MODE == STATES;
+    __shared__ __align__(16) float sB[2][CH * NP], sC[Y ? 2 : 1][Y ? CH * NP : 1];
+    const int cb = blockIdx.x % a.p.cblk, rest = blockIdx.x / a.p.cblk;
+    const int g = rest % a.G, rest2 = rest / a.G;
+    const int b = rest2 % a.B, seg = rest2 / a.B;
+    const int cg = a.C / a.G, ci = cb * a.p.width + threadIdx.x;
+    const bool on = ci < cg, wave_on = ci - (int)(threadIdx.x & 63) < cg;
+    const int c = g * cg + (on ? ci : cg - 1);          // lanes beyond the group repeat its last channel
+    const int len = length_of(a.lengths, b, a.L);
+    const int t0 = seg * a.p.seglen, t1 = min(t0 + a.p.seglen, a.L), te = min(t1, len);
+
+    float A2[NP], h[NP];
+    load_states<NP>(a.A + (long long)c * a.N, a.N, A2);
+#pragma unroll
+    for (int n = 0; n < NP; ++n) { A2[n] *= LOG2E; h[n] = 0.f; }
+    const long long row = (long long)b * a.C + c;
+    if (MODE != LOCAL) {
+        if (a.p.nseg > 1) load_kept<NP>(a.seg_h, seg, a.B, b, a.C, c, h);
+        else if (a.state) load_states<NP>(a.state + row * a.N, a.N, h);
+    }
+    const float bias = a.dt_bias ? a.dt_bias[c] : 0.f, Dc = Y && a.D ? a.D[c] : 0.f;
+    const typename M::raw* Bp = a.Bm + b * a.B_b + g * a.B_g;
+    const typename M::raw* Cp = a.Cm + b * a.C_b + g * a.C_g;
+
+    typename T::raw xr[CH], dr[CH], zr[CH];
+    MapTile<M, NP> mB, mC;
+    auto request = [&](int tc) {
+#pragma unroll
+        for (int s = 0; s < CH; ++s) {
+            const int t = min(tc + s, te - 1);          // (behind the end: the last step again, masked below)
+            xr[s] = load_elem<T, M, 0>(a, t, b, c);
+            dr[s] = load_elem<T, M, 1>(a, t, b, c);
+            if (GATED) zr[s] = load_elem<T, M, 2>(a, t, b, c);
+        }
+        mB.request(Bp, a.B_t, tc, te, a.N);
+        if (Y) mC.request(Cp, a.C_t, tc, te, a.N);
+    };
+    float S = 0.f;
+    if (te > t0) request(t0);
+    int buf = 0;
+    for (int tc = t0; tc < te; tc += CH, buf ^= 1) {
+        typename T::raw xc[CH], dc[CH], zc[CH];
+#pragma unroll
+        for (int s = 0; s < CH; ++s) { xc[s] = xr[s]; dc[s] = dr[s]; zc[s] = zr[s]; }
+        mB.put(sB[buf]);
+        if (Y) mC.put(sC[Y ? buf : 0]);
+        // one barrier a chunk: a buffer is written again two chunks later, behind the next barrier, which its readers have passed
+        __syncthreads();
+        if (tc + CH < te) request(tc + CH);
+        if (KEEP && tc > 0 && wave_on) store_kept<NP>(a.ck, tc / CH - 1, a.B, b, a.C, c, h);
+        if (MODE == STATES && tc + CH >= te) break;     // nothing is kept behind the last chunk
+        if (wave_on) {
+#pragma unroll
+            for (int s = 0; s < CH; ++s) {
+                const int t = tc + s;
+                const bool live = t < te;               // behind the row's end: a step of 0, which changes nothing
+                const float xv = live ? to_f(xc[s]) : 0.f;
+                float sig, st = softplus(to_f(dc[s]) + bias, sig);
+                st = live ? st : 0.f;
+                pin(st);
+                const float sx = st * xv;
+                if (MODE == LOCAL) S += st;
+                float y0 = 0.f, y1 = 0.f;
+                const float* Bt = sB[buf] + s * NP;
+                const float* Ct = sC[Y ? buf : 0] + (Y ? s * NP : 0);
+#pragma unroll
+                for (int n = 0; n < NP; ++n) {
+                    const float e = __builtin_amdgcn_exp2f(st * A2[n]);
+                    h[n] = fmaf(e, h[n], sx * Bt[n]);
+                    if (Y) { if (n & 1) y1 = fmaf(h[n], Ct[n], y1); else y0 = fmaf(h[n], Ct[n], y0); }
+                }
+                if (Y) {
+                    float o = fmaf(Dc, xv, y0 + y1);
+                    if (GATED) { const float zv = to_f(zc[s]); o *= zv * sigmoid(zv); }
+                    if (t < t1) a.y[((long long)t * a.B + b) * a.C + c] = from_f<M>(live ? o : 0.f);
+                }
+                step_fence();
+            }
+        }
+    }
+    if (!on) return;
+    if (MODE == LOCAL) {
+        store_kept<NP>(a.seg_h, seg, a.B, b, a.C, c, h);
+        a.seg_s[(long long)(seg * a.B + b) * a.C + c] = S;
+        return;
+    }
+    // the segment in which the row ends (the first one for an empty row) holds its final state
+    if (Y && a.state_out && ((len > t0 && len <= t1) || (len == 0 && seg == 0))) store_states<NP>(a.state_out + row * a.N, a.N, h);
+    if (Y)
+        for (int t = t0 + (max(te - t0, 0) + CH - 1) / CH * CH; t < t1; ++t) a.y[((long long)t * a.B + b) * a.C + c] = from_f<M>(0.f);
+}
+
+// seg_h: (h_loc of every segment) -> (its incoming state), in place.  A thread is one state of one channel and row.
+__global__ __launch_bounds__(256)
+void scan_chain_kernel(float* __restrict__ seg_h, const float* __restrict__ seg_s, const float* __restrict__ A, const float* __restrict__ first,
+                       int nseg, int np, int B, int C, int N, int reverse)
+{
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x, n_all = (long long)B * np * C;
+    if (i >= n_all) return;
+    const int c = (int)(i % C), n = (int)(i / C % np);
+    const long long b = i / C / np;
+    if (n >= N) return;                                 // (padding: zeros in every segment)
+    const float A2 = A[(long long)c * N + n] * LOG2E;
+    float h = first ? first[(b * C + c) * N + n] : 0.f;
+    for (int k = 0; k < nseg; ++k) {
+        const int s = reverse ? nseg - 1 - k : k;
+        const long long at = s * n_all + i;
+        const float loc = seg_h[at], S = seg_s[((long long)s * B + b) * C + c];
+        seg_h[at] = h;
+        h = fmaf(__builtin_amdgcn_exp2f(A2 * S), h, loc);
+    }
+}
+
+// One step of every row: state [B][C][N] -> state_out (may be the same buffer).  LPC lanes hold a channel, V = 4 or 1 states
+// each: whole lines of the state, which is all of the traffic, and a sum over LPC neighbouring lanes.
+template <class M, int V, int LPC>
+__global__ __launch_bounds__(256)
+void scan_step_kernel(const typename M::raw* __restrict__ x, long long x_b, const typename M::raw* __restrict__ dt, long long dt_b,
+                      const typename M::raw* __restrict__ z, long long z_b, const typename M::raw* __restrict__ Bm, long long B_b,
+                      long long B_g, const typename M::raw* __restrict__ Cm, long long C_b, long long C_g, const float* __restrict__ A,
+                      const float* __restrict__ D, const float* __restrict__ dt_bias, const float* state, float* state_out,
+                      const unsigned char* __restrict__ active, typename M::raw* __restrict__ y, int B, int C, int N, int G)
+{
+    const int part = threadIdx.x % LPC, n0 = part * V;
+    const long long n_ch = (long long)B * C, step = (long long)gridDim.x * (256 / LPC);
+    const int cg = C / G;
+    for (long long i = (long long)blockIdx.x * (256 / LPC) + threadIdx.x / LPC; i < n_ch; i += step) {
+        const int b = (int)(i / C), c = (int)(i % C), g = c / cg;
+        const bool act = !active || active[b], has = n0 < N;
+        float hv[V] = {};
+        if (has) {
+            if constexpr (V == 4) *reinterpret_cast<float4*>(hv) = *reinterpret_cast<const float4*>(state + i * N + n0);
+            else hv[0] = state[i * N + n0];
+        }
+        float yv = 0.f;
+        if (act) {                                      // (an inactive row's state stays as it is)
+            const float xv = to_f(x[b * x_b + c]);
+            float sig;
+            const float st = softplus(to_f(dt[b * dt_b + c]) + (dt_bias ? dt_bias[c] : 0.f), sig);
+            const float sx = st * xv;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                if (has) {
+                    const int n = n0 + v;
+                    hv[v] = fmaf(__builtin_amdgcn_exp2f(st * (A[(long long)c * N + n] * LOG2E)), hv[v], sx * to_f(Bm[b * B_b + g * B_g + n]));
+                    yv = fmaf(hv[v], to_f(Cm[b * C_b + g * C_g + n]), yv);
+                }
+            }
+#pragma unroll
+            for (int o = 1; o < LPC; o <<= 1) yv += __shfl_xor(yv, o, 64);
+            yv = fmaf(D ? D[c] : 0.f, xv, yv);
+            if (z) { const float zv = to_f(z[b * z_b + c]); yv *= zv * sigmoid(zv); }
+        }
+        if (has && (act || state_out != state)) {
+            if constexpr (V == 4) *reinterpret_cast<float4*>(state_out + i * N + n0) = *reinterpret_cast<float4*>(hv);
+            else state_out[i * N + n0] = hv[0];
+        }
+        if (part == 0) y[i] = from_f<M>(yv);
+    }
+}
+
+template <class T, class M, int NP, int MODE> int launch(const ScanArgs<T, M>& a, hipStream_t stream)
+{
+    const dim3 grid((unsigned)((long long)a.p.cblk * a.G * a.B * a.p.nseg));
+    if constexpr (MODE == OUT || MODE == TRAIN) {
+        if (a.zq) hipLaunchKernelGGL((scan_fwd_kernel<T, M, NP, MODE, true>), grid, dim3(a.p.width), 0, stream, a);
+        else hipLaunchKernelGGL((scan_fwd_kernel<T, M, NP, MODE, false>), grid, dim3(a.p.width), 0, stream, a);
+    } else {
+        hipLaunchKernelGGL((scan_fwd_kernel<T, M, NP, MODE, false>), grid, dim3(a.p.width), 0, stream, a);
+    }
+    GMT_LAUNCH_CHECK();
+    return GMT_OK;
+}
+template <class T, class M, int MODE> int by_np(const ScanArgs<T, M>& a, hipStream_t stream)
+{
+    return a.p.np == 8 ? launch<T, M, 8, MODE>(a, stream) : a.p.np == 16 ? launch<T, M, 16, MODE>(a, stream) : launch<T, M, 32, MODE>(a, stream);
+}
+
+// segments (if any), then the pass itself
+template <class T, class M, int MODE> int run(const gmt_scan_args* args, hipStream_t stream)
+{
+    ScanArgs<T, M> a = scan_args<T, M>(args);
+    if (a.p.nseg > 1) {
+        const long long nh = (long long)a.p.nseg * a.B * a.p.np * a.C, ns = (long long)a.p.nseg * a.B * a.C;
+        if (!args->workspace || args->workspace_floats < nh + ns) return GMT_ERR_WORKSPACE;
+        a.seg_h = args->workspace;
+        a.seg_s = args->workspace + nh;
+        if (int rc = by_np<T, M, LOCAL>(a, stream)) return rc;
+        if (int rc = scan_chain(a.seg_h, a.seg_s, a.A, a.state, a.p.nseg, a.p.np, a.B, a.C, a.N, 0, stream)) return rc;
+    }
+    return by_np<T, M, MODE>(a, stream);
+}
+
+template <class M, int V, int LPC> int launch_step(const gmt_scan_args* a, const unsigned char* active, hipStream_t stream)
+{
+    using R = typename M::raw;
+    const long long per = 256 / LPC, need = ((long long)a->B * a->C + per - 1) / per;
+    const unsigned grid = (unsigned)(need < 256 * 32 ? need : 256 * 32);
+    hipLaunchKernelGGL((scan_step_kernel<M, V, LPC>), dim3(grid), dim3(256), 0, stream, (const R*)a->x, a->x_b, (const R*)a->dt, a->dt_b,
+                       (const R*)a->z, a->z_b, (const R*)a->Bm, a->B_b, a->B_g, (const R*)a->Cm, a->C_b, a->C_g, a->A, a->D, a->dt_bias,
+                       a->state, a->state_out, active, (R*)a->y, a->B, a->C, a->N, a->G);
+    GMT_LAUNCH_CHECK();
+    return GMT_OK;
+}
+template <class M> int step(const gmt_scan_args* a, const unsigned char* active, hipStream_t stream)
+{
+    const int N = a->N;
+    if (N % 4 == 0 && (((uintptr_t)a->state | (uintptr_t)a->state_out) & 15) == 0)
+        return N <= 4 ? launch_step<M, 4, 1>(a, active, stream) : N <= 8 ? launch_step<M, 4, 2>(a, active, stream)
+             : N <= 16 ? launch_step<M, 4, 4>(a, active, stream) : launch_step<M, 4, 8>(a, active, stream);
+    return N <= 4 ? launch_step<M, 1, 4>(a, active, stream) : N <= 8 ? launch_step<M, 1, 8>(a, active, stream)
+         : N <= 16 ? launch_step<M, 1, 16>(a, active, stream) : launch_step<M, 1, 32>(a, active, stream);
+}
+
+}  // namespace
+
+namespace gmt_ssm {
+int scan_chain(float* seg_h, const float* seg_s, const float* A, const float* first, int nseg, int np, int B, int C, int N,
+               int reverse, hipStream_t stream)
+{
+    const long long n = (long long)B * np * C;
+    hipLaunchKernelGGL(scan_chain_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, seg_h, seg_s, A, first, nseg, np, B, C,
+                       N, reverse);
+    GMT_LAUNCH_CHECK();
+    return GMT_OK;
+}
+// the states before every chunk, from 8-bit checkpoints (backward pass)
+int scan_states_q8(const gmt_scan_args* a, hipStream_t stream)
+{
+    return a->bf16 ? run<Q8, B16, STATES>(a, stream) : run<Q8, F32, STATES>(a, stream);
+}
+}  // namespace gmt_ssm
+
+extern "C" int gmt_selective_scan_workspace(const gmt_scan_args* a, long long* ck_floats, long long* fwd_floats, long long* bwd_floats)
+{
+    if (int rc = scan_check(a)) return rc;
+    GMT_CHECK_ARG(ck_floats && fwd_floats && bwd_floats);
+    const ScanPlan p = scan_plan(a->L, a->B, a->C, a->N, a->G);
+    *ck_floats = (long long)p.nck * a->B * p.np * a->C;
+    *fwd_floats = p.nseg > 1 ? (long long)p.nseg * a->B * a->C * (p.np + 1) : 0;
+    *bwd_floats = scan_bwd_floats(a);
+    return GMT_OK;
+}
+
+extern "C" int gmt_selective_scan_fwd(const gmt_scan_args* a, hipStream_t stream)
+{
+    if (int rc = scan_check(a)) return rc;
+    GMT_CHECK_ARG(a->y && !a->x_scale);
+    if (a->ck) return a->bf16 ? run<B16, B16, TRAIN>(a, stream) : run<F32, F32, TRAIN>(a, stream);
+    return a->bf16 ? run<B16, B16, OUT>(a, stream) : run<F32, F32, OUT>(a, stream);
+}
+
+extern "C" int gmt_selective_scan_step(const gmt_scan_args* a, const unsigned char* active, hipStream_t stream)
+{
+    if (int rc = scan_check(a)) return rc;
+    GMT_CHECK_ARG(a->y && a->state && a->state_out && a->L == 1 && !a->x_scale);
+    return a->bf16 ? step<B16>(a, active, stream) : step<F32>(a, active, stream);
+}

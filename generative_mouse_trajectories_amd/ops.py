@@ -298,7 +298,36 @@ class LinearFn(torch.autograd.Function):
         return dx, dW, db
 
 
-def linear(x: torch.Tensor, w: torch.Tensor, b: Optional[torch.Tensor]) -> torch.Tensor:
+class LinearCkpt8Fn(torch.autograd.Function):
+    """LinearFn whose input is kept for the backward pass in 8 bits (ops_ckpt8): the weight gradient is taken at the values that
+    the checkpoint stands for, by the kernel that reads it.  First-order gradients only."""
+
+    @staticmethod
+    def forward(ctx, x, w, b):
+        from . import ops_ckpt8
+        p = ops_ckpt8.pack(x)
+        ctx.save_for_backward(p.codes, p.exponents, w)
+        ctx.dtype, ctx.has_b = x.dtype, b is not None
+        return F.linear(x, w, b)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        from . import ops_ckpt8
+        codes, exps, w = ctx.saved_tensors
+        dx = dW = db = None
+        if ctx.needs_input_grad[0]:
+            dx = (dy.reshape(-1, dy.shape[-1]) @ w).view(codes.shape)
+        if ctx.needs_input_grad[1] or (ctx.has_b and ctx.needs_input_grad[2]):
+            dW, db = ops_ckpt8.wgrad(dy, ops_ckpt8.Ckpt8(codes, exps, ctx.dtype), want_db=ctx.has_b)
+            dW, db = dW.to(w.dtype), None if db is None else db.to(w.dtype)
+        return dx, dW, db
+
+
+def linear(x: torch.Tensor, w: torch.Tensor, b: Optional[torch.Tensor], ckpt8: bool = False) -> torch.Tensor:
+    """ckpt8: x is kept for the backward pass in 8 bits (LinearCkpt8Fn)."""
+    if ckpt8 and torch.is_grad_enabled() and (w.requires_grad or (b is not None and b.requires_grad)):
+        return LinearCkpt8Fn.apply(x, w, b)
     return LinearFn.apply(x, w, b)
 
 

@@ -1,0 +1,114 @@
+"""8-bit activation checkpoints (csrc/ckpt8.hip): an activation kept for the backward pass as int8 codes and one exponent per
+32 channels, a quarter of its fp32 bytes, and the weight gradient that reads it.
+
+A block of 32 neighbouring channels of one row stands for q 2^e with |q| <= 127 and the smallest e in -118 .. 121 that reaches
+its largest magnitude: an element is off by at most 2^(e-1).  A block that holds an infinity or a NaN stands for NaN.  `ops.linear`,
+`ops_ssm.causal_conv` and `ops_ssm.selective_scan` take `ckpt8=True`: their gradients are then those at the values that the
+checkpoints stand for (the outputs are computed from the inputs themselves).
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import NamedTuple, Optional, Tuple
+
+import torch
+
+from . import _lib as L_
+
+BLOCK = 32
+DTYPES = (torch.float32, torch.bfloat16)
+
+
+class Ckpt8(NamedTuple):
+    """codes int8 [..., C], exponents uint8 [..., ceil(C / 32)] (255: the block stands for NaN), dtype of what was packed."""
+    codes: torch.Tensor
+    exponents: torch.Tensor
+    dtype: torch.dtype
+
+
+def on_device(*tensors) -> torch.device:
+    """The one GPU that all of them are on."""
+    L_.require_cuda(*tensors)
+    devs = {t.device for t in tensors if t is not None}
+    if len(devs) != 1:
+        raise L_.GmtError(f'tensors on different devices: {sorted(str(d) for d in devs)}')
+    return devs.pop()
+
+
+def time_major(t: torch.Tensor) -> torch.Tensor:
+    """`t` itself when its last axis is contiguous (rows may have any pitch), else a contiguous copy."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def pack(x: torch.Tensor) -> Ckpt8:
+    """x [..., C] fp32 or bf16 -> its 8-bit checkpoint."""
+    dev = on_device(x)
+    if x.dtype not in DTYPES:
+        raise L_.GmtError(f'ckpt8 packs float32 and bfloat16, not {x.dtype}')
+    if x.dim() < 1 or x.numel() == 0:
+        raise L_.GmtError(f'ckpt8: nothing to pack in a tensor of shape {tuple(x.shape)}')
+    x = time_major(x.detach())
+    C = x.shape[-1]
+    if x.dim() == 3:
+        T, B, st, sb = x.shape[0], x.shape[1], x.stride(0), x.stride(1)
+    else:
+        x = x if x.dim() <= 2 else x.contiguous()
+        T, B, st, sb = x.numel() // C, 1, (x.stride(0) if x.dim() == 2 else C), C
+    with torch.cuda.device(dev):
+        codes = torch.empty(x.shape, device=dev, dtype=torch.int8)
+        exps = torch.empty(*x.shape[:-1], (C + BLOCK - 1) // BLOCK, device=dev, dtype=torch.uint8)
+        L_.call('gmt_ckpt8_pack', x.data_ptr(), st, sb, codes.data_ptr(), exps.data_ptr(), T, B, C, int(x.dtype == torch.bfloat16),
+                L_.stream(), nbytes=float(x.numel() * (x.element_size() + 1)))
+    return Ckpt8(codes, exps, x.dtype)
+
+
+def check(p: Ckpt8) -> torch.device:
+    dev = on_device(p.codes, p.exponents)
+    C = p.codes.shape[-1]
+    if (p.codes.dtype != torch.int8 or p.exponents.dtype != torch.uint8 or p.codes.numel() == 0 or not p.codes.is_contiguous()
+            or not p.exponents.is_contiguous() or tuple(p.exponents.shape) != (*p.codes.shape[:-1], (C + BLOCK - 1) // BLOCK)):
+        raise L_.GmtError('not an 8-bit checkpoint: contiguous int8 codes [..., C] and uint8 exponents [..., ceil(C / 32)] expected')
+    return dev
+
+
+def unpack(p: Ckpt8, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """The values that a checkpoint stands for, as `dtype` (default: what was packed; both types hold them exactly)."""
+    dev = check(p)
+    dtype = p.dtype if dtype is None else dtype
+    if dtype not in DTYPES:
+        raise L_.GmtError(f'ckpt8 unpacks to float32 and bfloat16, not {dtype}')
+    C = p.codes.shape[-1]
+    with torch.cuda.device(dev):
+        out = torch.empty(p.codes.shape, device=dev, dtype=dtype)
+        L_.call('gmt_ckpt8_unpack', p.codes.data_ptr(), p.exponents.data_ptr(), out.data_ptr(), out.numel() // C, C,
+                int(dtype == torch.bfloat16), L_.stream(), nbytes=float(out.numel() * (out.element_size() + 1)))
+    return out
+
+
+def wgrad(dY: torch.Tensor, p: Ckpt8, want_db: bool = False) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """dW = dY^T X over the rows, X [..., I] given as its checkpoint and dY [..., N] (fp32 or bf16) with as many rows: fp32 [N, I];
+    with want_db also db = dY.sum over the rows.  The products are exact, the sums fp32 (csrc/ckpt8.hip); `ops.wgrad` is the same
+    for an fp32 X."""
+    dev = check(p)
+    if on_device(dY) != dev:
+        raise L_.GmtError('wgrad: dY and the checkpoint are on different devices')
+    if dY.dtype not in DTYPES:
+        raise L_.GmtError(f'wgrad: dY must be float32 or bfloat16, not {dY.dtype}')
+    N, I = dY.shape[-1], p.codes.shape[-1]
+    R = p.codes.numel() // I
+    if N == 0 or dY.numel() // N != R:
+        raise L_.GmtError(f'wgrad: dY {tuple(dY.shape)} and the checkpoint {tuple(p.codes.shape)} have different rows')
+    dY = time_major(dY.detach())
+    if dY.dim() != 2:
+        dY = dY.reshape(R, N)
+    if R > 1 and dY.stride(0) < N:                       # (an expanded gradient: its rows share memory)
+        dY = dY.contiguous()
+    with torch.cuda.device(dev):
+        need = ctypes.c_longlong(0)
+        L_.call('gmt_ckpt8_wgrad_workspace_floats', R, N, I, ctypes.addressof(need), label='skip')
+        ws = torch.empty(need.value, device=dev, dtype=torch.float32)
+        out = torch.empty(N * I + N, device=dev, dtype=torch.float32)
+        L_.call('gmt_ckpt8_wgrad', dY.data_ptr(), max(dY.stride(0), N), p.codes.data_ptr(), p.exponents.data_ptr(), out.data_ptr(), R,
+                N, I, int(dY.dtype == torch.bfloat16), int(want_db), L_.ptr(ws), need.value, L_.stream(),
+                label=f'wgrad8_N{N}_I{I}', flops=2.0 * R * N * I)
+    return out[:N * I].view(N, I), (out[N * I:] if want_db else None)

@@ -41,7 +41,7 @@ typedef struct ihipStream_t* hipStream_t;
 #define GMT_ERR_WORKSPACE (-4)    /* caller's workspace is too small                     */
 
 /* ABI version of this header; gmt_version() of the loaded library must match. */
-#define GMT_ABI_VERSION 9
+#define GMT_ABI_VERSION 10
 int gmt_version(void);
 
 /* ---- kinematic features, "mode A" ---------------------------------------------------
@@ -617,6 +617,75 @@ typedef struct gmt_bf16_gen_bwd_args {
     float dropout_p; unsigned int seed;   /* as in the forward launch */
 } gmt_bf16_gen_bwd_args;
 int gmt_bf16_gen_rollout_bwd(const gmt_bf16_gen_bwd_args* args, hipStream_t stream);
+
+/* ---- selective state-space operators (no counterpart in the reference: recurrent layers beside the LSTM ones) --------------
+ * Time-major sequences whose last axis is contiguous and whose step and row pitches (in elements) are free: element (t, b, c) at
+ * p[t * p_t + b * p_b + c].  bf16 = 0: x, dt, z, B, C, y and their gradients are fp32, 1: bf16.  Parameters, states of the scan
+ * and every sum are fp32.  lengths [B] int32 on the device, or NULL (every row has L steps); values are clamped to 0 .. L.  Steps
+ * at or behind a row's length are never read as numbers; y and the gradients are zero there.
+ * x_scale (dt_scale, z_scale): exponents of 8-bit checkpoints (gmt_ckpt8_pack); x (dt, z) are then their codes, contiguous. */
+
+/* Short causal convolution, one filter of K = 2 .. 4 taps per channel:  past = [state; x],
+ * pre[t] = bias + sum_k w[k] past[t + k],  y[t] = silu(pre[t]) (silu = 0: pre[t]).
+ * state / state_out / dstate / dstate_out [K-1][B][C], like x: the inputs before the first step / before the next call's.
+ * _bwd: dy, dstate_out (or NULL) -> dx, dparam = dw [K][C] then dbias [C], dstate (or NULL); x may be a checkpoint.
+ * _step: one step, x [B][C] -> y [B][C], state -> state_out (may be the same buffer); rows with active[b] == 0 keep their state
+ * and give zeros (active NULL: every row). */
+typedef struct gmt_conv_args {
+    const void* x; const unsigned char* x_scale; const float* w; /* [C][K] */ const float* bias; /* [C] or NULL */
+    const void* state;            /* or NULL: zeros */
+    const int* lengths;
+    void* y; void* state_out;     /* y contiguous; state_out may be NULL (fwd) */
+    const void* dy; const void* dstate_out; void* dx; float* dparam; void* dstate;
+    float* workspace; long long workspace_floats;    /* _bwd: gmt_causal_conv_bwd_workspace_floats */
+    long long x_t, x_b, dy_t, dy_b;
+    int L, B, C, K, bf16, silu;
+} gmt_conv_args;
+int gmt_causal_conv_fwd(const gmt_conv_args* args, hipStream_t stream);
+int gmt_causal_conv_bwd_workspace_floats(const gmt_conv_args* args, long long* floats_out);
+int gmt_causal_conv_bwd(const gmt_conv_args* args, hipStream_t stream);
+int gmt_causal_conv_step(const gmt_conv_args* args, const unsigned char* active, hipStream_t stream);
+
+/* Selective scan: N <= 32 states per channel, G groups of C / G neighbouring channels that share B and C [L][B][G][N]:
+ *   step = softplus(dt + dt_bias),  h[t] = exp(step A) h[t-1] + step x B,
+ *   y = (sum_n C h + D x) silu(z)   (z NULL: no gate; D, dt_bias NULL: zeros).
+ * state / state_out / dstate / dstate_out [B][C][N] fp32, NULL: zeros / not wanted.  ck: the states before every eighth step
+ * (gmt_selective_scan_workspace gives the sizes; NULL in a forward call that no backward call follows).
+ * _bwd: from the same inputs, ck of the forward call, dy and dstate_out (or NULL) -> dx, ddt, dz, dB, dC (contiguous), dparam =
+ * dA [C][N], dD [C], ddt_bias [C], dstate (or NULL).  With 8-bit checkpoints ck is scratch of the same size and every gradient is
+ * taken at the values that the checkpoints stand for.
+ * _step: one step (L = 1) of every row, state -> state_out (may be the same buffer), `active` as above. */
+typedef struct gmt_scan_args {
+    const void* x; const void* dt; const void* z;
+    const unsigned char* x_scale; const unsigned char* dt_scale; const unsigned char* z_scale;
+    const void* Bm; const void* Cm;
+    const float* A; /* [C][N] */ const float* D; const float* dt_bias; const float* state; const int* lengths;
+    void* y; float* state_out; float* ck;
+    const void* dy; const float* dstate_out;
+    void* dx; void* ddt; void* dz; void* dB; void* dC; float* dparam; float* dstate;
+    float* workspace; long long workspace_floats;
+    long long x_t, x_b, dt_t, dt_b, z_t, z_b, B_t, B_b, B_g, C_t, C_b, C_g, dy_t, dy_b;
+    int L, B, C, N, G, bf16;
+} gmt_scan_args;
+int gmt_selective_scan_workspace(const gmt_scan_args* args, long long* ck_floats, long long* fwd_floats, long long* bwd_floats);
+int gmt_selective_scan_fwd(const gmt_scan_args* args, hipStream_t stream);
+int gmt_selective_scan_bwd(const gmt_scan_args* args, hipStream_t stream);
+int gmt_selective_scan_step(const gmt_scan_args* args, const unsigned char* active, hipStream_t stream);
+
+/* ---- 8-bit activation checkpoints ----------------------------------------------------------------------------------------
+ * Blocks of 32 channels of a row as int8 codes q and one exponent byte s, standing for q 2^(s - 127): the smallest scale in
+ * 2^-118 .. 2^121 with |q| <= 127, q rounded to nearest even.  A block that holds an infinity or a NaN stands for NaN throughout
+ * (s = 255, q = 0).  x [T][B][C] with free pitches (fp32, or bf16) -> codes [T][B][C], scale [T][B][ceil(C / 32)].
+ * _unpack: rows of C channels -> out [rows][C].
+ * _wgrad: dW[n][i] = sum_r dY[r][n] Xhat[r][i] (fp32 [N][I]) and, if wanted, db[n] = sum_r dY[r][n] behind it (dW_db holds
+ * N * I + N floats either way); dY [R][ldy] fp32 or bf16, Xhat [R][I] the checkpoint.  Products exact, sums fp32. */
+int gmt_ckpt8_pack(const void* x, long long x_t, long long x_b, signed char* codes, unsigned char* scale, long long T, int B,
+                   int C, int bf16, hipStream_t stream);
+int gmt_ckpt8_unpack(const signed char* codes, const unsigned char* scale, void* out, long long rows, int C, int bf16,
+                     hipStream_t stream);
+int gmt_ckpt8_wgrad_workspace_floats(long long R, int N, int I, long long* floats_out);
+int gmt_ckpt8_wgrad(const void* dY, long long ldy, const signed char* codes, const unsigned char* scale, float* dW_db, long long R,
+                    int N, int I, int bf16, int want_db, float* workspace, long long workspace_floats, hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,130 @@
+"""What the selective state-space operators and the 8-bit checkpoints refuse: every check runs on the host before a launch (CPU)."""
+import pytest
+import torch
+
+from generative_mouse_trajectories_amd import _lib, ops, ops_ckpt8, ops_ssm
+from generative_mouse_trajectories_amd._lib import GmtError
+
+
+@pytest.fixture
+def no_launch(monkeypatch):
+    """CPU tensors past the device check; reaching a launch fails the test."""
+    def launch(name, *a, **k):
+        raise AssertionError(f'{name} was launched')
+    monkeypatch.setattr(_lib, 'call', launch)
+    monkeypatch.setattr(_lib, 'require_cuda', lambda *t: None)
+
+
+def seq(L=4, B=3, C=8, dtype=torch.float32):
+    return torch.zeros(L, B, C, dtype=dtype)
+
+
+def scan_call(**over):
+    L, B, C, N = 4, 3, 8, 5
+    a = dict(x=seq(), dt=seq(), A=torch.zeros(C, N), B=torch.zeros(L, B, N), C=torch.zeros(L, B, N))
+    a.update(over)
+    return ops_ssm.selective_scan(**a)
+
+
+def step_call(**over):
+    B, C, N = 3, 8, 5
+    a = dict(x=torch.zeros(B, C), dt=torch.zeros(B, C), A=torch.zeros(C, N), B=torch.zeros(B, N), C=torch.zeros(B, N), state=torch.zeros(B, C, N))
+    a.update(over)
+    return ops_ssm.selective_scan_step(**a)
+
+
+def test_cpu_tensors():
+    for call in (scan_call, step_call, lambda: ops_ssm.causal_conv(seq(), torch.zeros(8, 4)), lambda: ops_ckpt8.pack(seq()),
+                 lambda: ops_ssm.causal_conv_step(torch.zeros(3, 8), torch.zeros(3, 3, 8), torch.zeros(8, 4))):
+        with pytest.raises(GmtError, match='GPU only'):
+            call()
+
+
+@pytest.mark.parametrize('over', [
+    dict(x=torch.zeros(4, 3)), dict(x=seq(0)), dict(x=seq(B=0)), dict(x=seq(dtype=torch.float16)), dict(x=seq(dtype=torch.float64)),
+    dict(x=seq(dtype=torch.bfloat16)), dict(dt=seq(5)), dict(dt=seq(dtype=torch.bfloat16)), dict(A=torch.zeros(7, 5)), dict(A=torch.zeros(8, 0)),
+    dict(A=torch.zeros(8, 33), B=torch.zeros(4, 3, 33), C=torch.zeros(4, 3, 33)), dict(A=torch.zeros(8, 5, dtype=torch.bfloat16)),
+    dict(B=torch.zeros(4, 3, 6)), dict(B=torch.zeros(4, 3, 3, 5)), dict(B=torch.zeros(4, 3, 2, 5)), dict(C=torch.zeros(4, 2, 5)),
+    dict(C=torch.zeros(4, 3, 5, dtype=torch.bfloat16)), dict(C=torch.zeros(3, 5)), dict(D=torch.zeros(7)), dict(D=torch.zeros(8, dtype=torch.float64)),
+    dict(z=seq(C=9)), dict(dt_bias=torch.zeros(1)), dict(state=torch.zeros(3, 5, 8)), dict(state=torch.zeros(3, 8, 5, dtype=torch.bfloat16)),
+    dict(lengths=torch.zeros(3)), dict(lengths=torch.zeros(4, dtype=torch.int32)), dict(lengths=torch.zeros(3, 1, dtype=torch.int32))])
+def test_scan(no_launch, over):
+    with pytest.raises(GmtError):
+        scan_call(**over)
+
+
+@pytest.mark.parametrize('over', [
+    dict(x=seq()), dict(dt=torch.zeros(3, 9)), dict(B=torch.zeros(3, 4)), dict(B=torch.zeros(3, 3, 5)), dict(state=torch.zeros(3, 8, 4)),
+    dict(state=torch.zeros(3, 5, 8).transpose(1, 2)), dict(state=torch.zeros(3, 8, 5, dtype=torch.bfloat16)),
+    dict(state_out=torch.zeros(3, 8, 5)[:2]), dict(active=torch.zeros(3)), dict(active=torch.zeros(2, dtype=torch.bool)),
+    dict(x=torch.zeros(3, 8, requires_grad=True))])
+def test_scan_step(no_launch, over):
+    with pytest.raises(GmtError):
+        step_call(**over)
+
+
+def test_overlapping_state_buffers(no_launch):
+    pool = torch.zeros(4 * 8 * 5)
+    with pytest.raises(GmtError, match='overlaps'):
+        step_call(state=pool[:120].view(3, 8, 5), state_out=pool[40:].view(3, 8, 5))
+    pool = torch.zeros(4 * 24)
+    with pytest.raises(GmtError, match='overlaps'):
+        ops_ssm.causal_conv_step(torch.zeros(3, 8), pool[:72].view(3, 3, 8), torch.zeros(8, 4), state_out=pool[24:].view(3, 3, 8))
+
+
+@pytest.mark.parametrize('over', [
+    dict(x=torch.zeros(4, 8)), dict(x=seq(0)), dict(x=seq(dtype=torch.float16)), dict(weight=torch.zeros(8, 1)), dict(weight=torch.zeros(8, 5)),
+    dict(weight=torch.zeros(7, 4)), dict(weight=torch.zeros(8, 4, dtype=torch.bfloat16)), dict(bias=torch.zeros(7)),
+    dict(state=torch.zeros(4, 3, 8)), dict(state=torch.zeros(3, 3, 8, dtype=torch.bfloat16)), dict(lengths=torch.zeros(2, dtype=torch.int32))])
+def test_conv(no_launch, over):
+    a = dict(x=seq(), weight=torch.zeros(8, 4))
+    a.update(over)
+    with pytest.raises(GmtError):
+        ops_ssm.causal_conv(**a)
+
+
+def test_ckpt8(no_launch):
+    for bad in (torch.zeros(3, 4, dtype=torch.float16), torch.zeros(0, 4), torch.zeros(())):
+        with pytest.raises(GmtError):
+            ops_ckpt8.pack(bad)
+    good = ops_ckpt8.Ckpt8(torch.zeros(6, 40, dtype=torch.int8), torch.zeros(6, 2, dtype=torch.uint8), torch.float32)
+    with pytest.raises(GmtError):
+        ops_ckpt8.unpack(good, torch.float16)
+    for p in (good._replace(codes=good.codes.t()), good._replace(exponents=good.exponents[:, :1]), good._replace(codes=good.codes.to(torch.uint8)),
+              good._replace(exponents=good.exponents.to(torch.int8))):
+        with pytest.raises(GmtError):
+            ops_ckpt8.unpack(p)
+    for dy in (torch.zeros(5, 8), torch.zeros(6, 8, dtype=torch.float16), torch.zeros(6, 0)):
+        with pytest.raises(GmtError):
+            ops_ckpt8.wgrad(dy, good)
+
+
+def test_library_entry_points_check_their_arguments():
+    """The C entries return codes for what they cannot run; no launch happens."""
+    import ctypes
+    L = _lib.lib()
+    assert L.gmt_causal_conv_fwd(None, None) == -1 and L.gmt_selective_scan_fwd(None, None) == -1
+    a = _lib.ConvArgs(x=16, w=16, L=1, B=1, C=4, K=5, y=16)
+    assert L.gmt_causal_conv_fwd(ctypes.addressof(a), None) == -2
+    a = _lib.ConvArgs(x=16, w=16, L=64, B=2, C=4, K=4, dy=16, dx=16, dparam=16, workspace=16, workspace_floats=1)
+    need = ctypes.c_longlong(0)
+    assert L.gmt_causal_conv_bwd_workspace_floats(ctypes.addressof(a), ctypes.addressof(need)) == 0 and need.value > 1
+    assert L.gmt_causal_conv_bwd(ctypes.addressof(a), None) == -4
+    s = _lib.ScanArgs(x=16, dt=16, A=16, Bm=16, Cm=16, y=16, L=4, B=2, C=6, N=33, G=1)
+    assert L.gmt_selective_scan_fwd(ctypes.addressof(s), None) == -2
+    s.N, s.G = 16, 4
+    assert L.gmt_selective_scan_fwd(ctypes.addressof(s), None) == -1
+    s.G, s.L, s.x_scale = 1, 300, 16
+    assert L.gmt_selective_scan_fwd(ctypes.addressof(s), None) == -1
+    s.x_scale = None
+    sizes = [ctypes.c_longlong(-1) for _ in range(3)]
+    assert L.gmt_selective_scan_workspace(ctypes.addressof(s), *(ctypes.addressof(v) for v in sizes)) == 0
+    assert all(v.value > 0 for v in sizes)
+    assert L.gmt_selective_scan_fwd(ctypes.addressof(s), None) == -4      # cut into segments: needs its workspace
+    s.dy = s.dx = s.ddt = s.dB = s.dC = s.dparam = s.workspace = 16
+    assert L.gmt_selective_scan_bwd(ctypes.addressof(s), None) == -1      # no kept states
+    s.ck = 16
+    assert L.gmt_selective_scan_bwd(ctypes.addressof(s), None) == -4
+    assert L.gmt_ckpt8_pack(None, 1, 1, None, None, 1, 1, 1, 0, None) == -1
+    assert L.gmt_ckpt8_wgrad(16, 128, 16, 16, 16, 1 << 20, 128, 128, 0, 0, None, 0, None) == -4
+    assert L.gmt_ckpt8_wgrad(16, 4, 16, 16, 16, 1, 8, 8, 0, 0, None, 0, None) == -1
