@@ -4,9 +4,12 @@
 //     h[t][n] = exp(step[t] A[n]) h[t-1][n] + step[t] x[t] B[t][n]                                N states per channel
 //     y[t]    = (sum_n C[t][n] h[t][n] + D x[t]) silu(z[t])
 //
-// B and C are shared by the channels of a group.  Time-major [L][B][..]; a LANE is a channel and keeps its N states in
-// registers, a wave is 64 channels of one row, a workgroup up to 4 waves of one group, which share B[t] and C[t] through LDS.
-// Time runs in chunks of CH steps: the chunk's elements are requested one chunk ahead, its B and C sit in LDS as fp32.
+// B and C are shared by the channels of a group.  Time-major [L][B][..].  PARTS = 1 or 2 lanes hold a channel with N / PARTS
+// states each in registers; a workgroup is up to 8 waves of one row and one group, which share B[t] and C[t] through LDS as fp32.
+// Time runs in chunks of CH steps, requested one chunk ahead, in three phases: what depends on (t, channel) alone - softplus,
+// gate - for all steps at once, divided between a channel's lanes; the recurrence, step by step; the outputs, divided again.
+// The recurrence is 5 instructions a state and step, one of them an exponential at half rate: VALU issue bounds these kernels
+// (N = 16: 5.3 cycles of a SIMD per state, against 0.2 bytes), not HBM.
 //
 // Few rows (long prompts) do not fill 1024 SIMDs: time is then cut into segments.  A segment maps its incoming state
 // linearly, h_out = exp(A S) h_in + h_loc, S = the sum of its steps - one float per channel holds the whole decay.  Pass 1 finds
@@ -20,17 +23,20 @@ namespace gmt_ssm {
 
 constexpr int CH = 8;                    // steps per chunk = steps between kept states
 
-struct ScanPlan { int np, waves, width, cblk, nseg, seglen, nck; };   // cblk: workgroups across a group's channels
+struct ScanPlan { int np, parts, waves, width, chans, cblk, nseg, seglen, nck; };   // chans: channels a workgroup; cblk: workgroups a group
 
-// Padded state count, workgroup width and time segments
-static inline ScanPlan scan_plan(int L, int B, int C, int N, int G)
+// Padded state count, lanes per channel, workgroup width (at most max_waves waves) and time segments
+static inline ScanPlan scan_plan(int L, int B, int C, int N, int G, int parts, int max_waves)
 {
     ScanPlan p;
     p.np = N <= 8 ? 8 : N <= 16 ? 16 : 32;
-    const int cg = C / G;
-    p.waves = cg <= 64 ? 1 : cg <= 128 ? 2 : 4;
+    p.parts = parts;
+    const int cg = C / G, per = 64 / parts;
+    p.waves = 1;
+    while (p.waves < max_waves && p.waves * per < cg) p.waves *= 2;
     p.width = 64 * p.waves;
-    p.cblk = (cg + p.width - 1) / p.width;
+    p.chans = p.waves * per;
+    p.cblk = (cg + p.chans - 1) / p.chans;
     const long long waves = (long long)B * G * p.cblk * p.waves;
     long long nseg = 1;
     if (waves <= 512) {
@@ -44,6 +50,13 @@ static inline ScanPlan scan_plan(int L, int B, int C, int N, int G)
     p.nck = (L - 1) / CH;                // states kept before steps CH, 2 CH, ...
     return p;
 }
+// One lane per channel costs the fewest instructions; two lanes fill the machine with half of the rows
+static inline ScanPlan fwd_plan(int L, int B, int C, int N, int G)
+{
+    const ScanPlan p = scan_plan(L, B, C, N, G, 1, 4);
+    return (long long)B * G * p.cblk * p.waves >= 4096 ? p : scan_plan(L, B, C, N, G, 2, 4);
+}
+static inline ScanPlan bwd_plan(int L, int B, int C, int N, int G) { return scan_plan(L, B, C, N, G, 2, 8); }
 
 static inline int scan_check(const gmt_scan_args* a)
 {
@@ -51,15 +64,17 @@ static inline int scan_check(const gmt_scan_args* a)
     GMT_CHECK_ARG(a->C % a->G == 0);
     GMT_CHECK_ARG((a->x_scale != nullptr) == (a->dt_scale != nullptr) && (a->z == nullptr || (a->x_scale != nullptr) == (a->z_scale != nullptr)));
     if (a->N > 32) return GMT_ERR_UNSUPPORTED;
-    const ScanPlan p = scan_plan(a->L, a->B, a->C, a->N, a->G);
-    if ((long long)p.cblk * a->G * a->B * p.nseg >= (1LL << 24)) return GMT_ERR_UNSUPPORTED;
+    // lane offsets are 32 bits: a step's pitch plus a channel, in elements
+    const long long lim = 1LL << 29;
+    if (a->C >= lim || a->x_t >= lim || a->dt_t >= lim || a->z_t >= lim || a->dy_t >= lim || (long long)a->B * a->C >= lim) return GMT_ERR_UNSUPPORTED;
+    for (const ScanPlan& p : {fwd_plan(a->L, a->B, a->C, a->N, a->G), bwd_plan(a->L, a->B, a->C, a->N, a->G)})
+        if ((long long)p.cblk * a->G * a->B * p.nseg >= (1LL << 22)) return GMT_ERR_UNSUPPORTED;
     return GMT_OK;
 }
 
 // pointers and pitches of one launch by value; T / M: element types of x, dt, z / of everything else
 template <class T, class M> struct ScanArgs {
-    const typename T::raw* x; const typename T::raw* dt; const typename T::raw* z;
-    const void *xq, *dtq, *zq; const unsigned char *xs, *dts, *zs;        // 8-bit checkpoints: codes, exponents
+    const void *x, *dt, *z; const unsigned char *xs, *dts, *zs;           // elements, or codes and exponents of 8-bit checkpoints
     const typename M::raw* Bm; const typename M::raw* Cm;
     const float *A, *D, *dt_bias, *state; const int* lengths;
     typename M::raw* y; float* state_out; float* ck; float* seg_h; float* seg_s;
@@ -70,11 +85,10 @@ template <class T, class M> struct ScanArgs {
     ScanPlan p;
 };
 
-template <class T, class M> ScanArgs<T, M> scan_args(const gmt_scan_args* a)
+template <class T, class M> ScanArgs<T, M> scan_args(const gmt_scan_args* a, const ScanPlan& p)
 {
     ScanArgs<T, M> s;
-    s.x = (const typename T::raw*)a->x; s.dt = (const typename T::raw*)a->dt; s.z = (const typename T::raw*)a->z;
-    s.xq = a->x; s.dtq = a->dt; s.zq = a->z; s.xs = a->x_scale; s.dts = a->dt_scale; s.zs = a->z_scale;
+    s.x = a->x; s.dt = a->dt; s.z = a->z; s.xs = a->x_scale; s.dts = a->dt_scale; s.zs = a->z_scale;
     s.Bm = (const typename M::raw*)a->Bm; s.Cm = (const typename M::raw*)a->Cm;
     s.A = a->A; s.D = a->D; s.dt_bias = a->dt_bias; s.state = a->state; s.lengths = a->lengths;
     s.y = (typename M::raw*)a->y; s.state_out = a->state_out; s.ck = a->ck; s.seg_h = s.seg_s = nullptr;
@@ -82,72 +96,119 @@ template <class T, class M> ScanArgs<T, M> scan_args(const gmt_scan_args* a)
     s.dx = (typename M::raw*)a->dx; s.ddt = (typename M::raw*)a->ddt; s.dz = (typename M::raw*)a->dz;
     s.dB = (typename M::raw*)a->dB; s.dC = (typename M::raw*)a->dC; s.dstate = a->dstate; s.part = s.bc_part = nullptr;
     s.x_t = a->x_t; s.x_b = a->x_b; s.dt_t = a->dt_t; s.dt_b = a->dt_b; s.z_t = a->z_t; s.z_b = a->z_b;
+    if (a->x_scale) { s.x_t = s.dt_t = s.z_t = (long long)a->B * a->C; s.x_b = s.dt_b = s.z_b = a->C; }
     s.B_t = a->B_t; s.B_b = a->B_b; s.B_g = a->B_g; s.C_t = a->C_t; s.C_b = a->C_b; s.C_g = a->C_g;
     s.dy_t = a->dy_t; s.dy_b = a->dy_b;
     s.L = a->L; s.B = a->B; s.C = a->C; s.N = a->N; s.G = a->G; s.P = 0;
-    s.p = scan_plan(a->L, a->B, a->C, a->N, a->G);
+    s.p = p;
     return s;
 }
 
 // Between unrolled steps: B and C of the next step are read from LDS when it comes to them, not 8 steps ahead into registers.
 __device__ __forceinline__ void step_fence() { asm volatile("" ::: "memory"); __builtin_amdgcn_sched_barrier(0); }
-
-// ... and what a step computes from v stays behind this point.
+// ... and v is computed before this point, what follows from it behind it (a sum is not put off with its terms in registers).
 __device__ __forceinline__ void pin(float& v) { asm volatile("" : "+v"(v)); }
 
-// which = 0: x, 1: dt, 2: z at (t, b, c)
-template <class T, class M, int WHICH> __device__ __forceinline__ typename T::raw load_elem(const ScanArgs<T, M>& a, int t, int b, int c)
-{
-    if constexpr (__is_same(T, Q8)) {
-        const long long row = (long long)t * a.B + b;
-        const void* q = WHICH == 0 ? a.xq : WHICH == 1 ? a.dtq : a.zq;
-        const unsigned char* s = WHICH == 0 ? a.xs : WHICH == 1 ? a.dts : a.zs;
-        Q8::raw r;
-        r.q = ((const signed char*)q)[row * a.C + c];
-        r.s = s[row * ((a.C + 31) / 32) + c / 32];
-        return r;
-    } else {
-        return WHICH == 0 ? a.x[t * a.x_t + b * a.x_b + c] : WHICH == 1 ? a.dt[t * a.dt_t + b * a.dt_b + c] : a.z[t * a.z_t + b * a.z_b + c];
+template <int CTRL> __device__ __forceinline__ float dpp(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+constexpr int DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E, DPP_XOR7 = 0x141, DPP_XOR8 = 0x128;     // quad_perm, row_half_mirror, row_ror:8
+
+// ---- lanes of a channel.  With two, bit 3 of the lane says which: the other one is 8 lanes on within a row of 16, one DPP away.
+template <int PARTS> struct Lanes {
+    static constexpr int OWN = CH / PARTS;              // a lane's own steps of a chunk: j * PARTS + part
+    int part; unsigned chan;                            // chan: channel within the workgroup
+    __device__ __forceinline__ Lanes() {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        part = PARTS == 1 ? 0 : lane >> 3 & 1;
+        chan = wave * (64 / PARTS) + (PARTS == 1 ? lane : (lane & 7) | (lane >> 4) << 3);
     }
+    // own[j] of the lane that owns step s, on all lanes of the channel
+    __device__ __forceinline__ float of_step(const float (&own)[OWN], int s) const {
+        if constexpr (PARTS == 1) return own[s];
+        else {
+            const float o = dpp<DPP_XOR8>(own[s / 2]);
+            return part == (s & 1) ? own[s / 2] : o;
+        }
+    }
+    __device__ __forceinline__ float sum(float v) const { return PARTS == 1 ? v : v + dpp<DPP_XOR8>(v); }
+    __device__ __forceinline__ void keep(float (&own)[OWN], int s, float v) const {
+        if constexpr (PARTS == 1) own[s] = v; else own[s / 2] = part == (s & 1) ? v : own[s / 2];
+    }
+};
+
+// A lane's own elements of one sequence for one chunk.  full: all CH steps exist (uniform); else steps behind the end repeat the
+// last one and are masked by the caller.
+template <class T, int PARTS> struct Own {
+    static constexpr int OWN = CH / PARTS;
+    typename T::raw v[OWN];
+    __device__ __forceinline__ void request(const void* p, const unsigned char* scale, long long pt, int tc, int te, bool full, int part, unsigned c,
+                                            long long row_pitch, int b, int n_sc) {
+        // p: at (0, b, 0).  A step pair's base is uniform, the lane's part of the offset 32 bits.
+        if constexpr (__is_same(T, Q8)) {
+            const signed char* q = (const signed char*)p;
+#pragma unroll
+            for (int j = 0; j < OWN; ++j) {
+                if (full) {
+                    const long long t = tc + j * PARTS;
+                    v[j].q = (q + t * pt)[(unsigned)(part * pt) + c];
+                    v[j].s = (scale + (t * row_pitch + b) * n_sc)[(unsigned)(part * row_pitch * n_sc) + c / 32];
+                } else {
+                    const long long t = min(tc + j * PARTS + part, te - 1);
+                    v[j].q = q[t * pt + c];
+                    v[j].s = scale[(t * row_pitch + b) * n_sc + c / 32];
+                }
+            }
+        } else {
+            const typename T::raw* q = (const typename T::raw*)p;
+#pragma unroll
+            for (int j = 0; j < OWN; ++j) {
+                if (full) v[j] = (q + (long long)(tc + j * PARTS) * pt)[(unsigned)(part * pt) + c];
+                else v[j] = q[(long long)min(tc + j * PARTS + part, te - 1) * pt + c];
+            }
+        }
+    }
+};
+template <class T> __device__ __forceinline__ const void* row_of(const void* p, long long offset) {
+    if constexpr (__is_same(T, Q8)) return (const signed char*)p + offset; else return (const typename T::raw*)p + offset;
 }
 
-// N floats of a channel's row (state buffers [B][C][N], A [C][N]) <-> NP registers, zero-padded
-template <int NP> __device__ __forceinline__ void load_states(const float* p, int N, float (&h)[NP])
+// NS floats of a channel's row, states n0 .. n0 + NS - 1 (state buffers [B][C][N], A [C][N]) <-> registers, zero-padded
+template <int NS> __device__ __forceinline__ void load_states(const float* p, int n0, int N, float (&h)[NS])
 {
-    if (N == NP && ((uintptr_t)p & 15) == 0) {
+    if ((N & 3) == 0 && n0 + NS <= N && ((uintptr_t)p & 15) == 0) {
 #pragma unroll
-        for (int n = 0; n < NP; n += 4) {
-            const float4 v = *reinterpret_cast<const float4*>(p + n);
+        for (int n = 0; n < NS; n += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(p + n0 + n);
             h[n] = v.x; h[n + 1] = v.y; h[n + 2] = v.z; h[n + 3] = v.w;
         }
     } else {
 #pragma unroll
-        for (int n = 0; n < NP; ++n) h[n] = n < N ? p[n] : 0.f;
+        for (int n = 0; n < NS; ++n) h[n] = n0 + n < N ? p[n0 + n] : 0.f;
     }
 }
-template <int NP> __device__ __forceinline__ void store_states(float* p, int N, const float (&h)[NP])
+template <int NS> __device__ __forceinline__ void store_states(float* p, int n0, int N, const float (&h)[NS])
 {
-    if (N == NP && ((uintptr_t)p & 15) == 0) {
+    if ((N & 3) == 0 && n0 + NS <= N && ((uintptr_t)p & 15) == 0) {
 #pragma unroll
-        for (int n = 0; n < NP; n += 4) *reinterpret_cast<float4*>(p + n) = make_float4(h[n], h[n + 1], h[n + 2], h[n + 3]);
+        for (int n = 0; n < NS; n += 4) *reinterpret_cast<float4*>(p + n0 + n) = make_float4(h[n], h[n + 1], h[n + 2], h[n + 3]);
     } else {
 #pragma unroll
-        for (int n = 0; n < NP; ++n) if (n < N) p[n] = h[n];
+        for (int n = 0; n < NS; ++n) if (n0 + n < N) p[n0 + n] = h[n];
     }
 }
-
 // The kept states and the segments' states: [..][B][NP][C], N padded to NP with zeros.
-template <int NP> __device__ __forceinline__ void load_kept(const float* p, long long slot, int B, int b, int C, int c, float (&h)[NP])
+template <int NP, int NS> __device__ __forceinline__ void load_kept(const float* p, long long slot, int B, int b, int C, unsigned c, int n0, float (&h)[NS])
 {
-    const float* k = p + (slot * B + b) * NP * C + c;
+    const float* k = p + (slot * B + b) * NP * C + c + (long long)n0 * C;
 #pragma unroll
-    for (int n = 0; n < NP; ++n) h[n] = k[(long long)n * C];
+    for (int n = 0; n < NS; ++n) h[n] = k[(long long)n * C];
 }
-template <int NP> __device__ __forceinline__ void store_kept(float* p, long long slot, int B, int b, int C, int c, const float (&h)[NP])
+template <int NP, int NS> __device__ __forceinline__ void store_kept(float* p, long long slot, int B, int b, int C, unsigned c, int n0, const float (&h)[NS])
 {
-    float* k = p + (slot * B + b) * NP * C + c;
+    float* k = p + (slot * B + b) * NP * C + c + (long long)n0 * C;
 #pragma unroll
-    for (int n = 0; n < NP; ++n) k[(long long)n * C] = h[n];
+    for (int n = 0; n < NS; ++n) k[(long long)n * C] = h[n];
 }
 
 // The chunk's B (or C) as fp32 [CH][NP] in LDS, by all threads of the workgroup: request() one chunk ahead, put() behind the wait.

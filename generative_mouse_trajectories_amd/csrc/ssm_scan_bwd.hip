@@ -8,8 +8,8 @@
 // operator at the values the checkpoints stand for).
 //
 // dB and dC are sums over lanes: 2 N values a step.  They leave by halving exchanges - a lane hands half of its values to its
-// partner and keeps the partner's other half, v_permlane32/16_swap then DPP - 70 instructions for 32 values where 32 separate
-// wave sums take 192.  The waves of a workgroup meet in LDS, workgroups of one group through slabs: no float atomics, results
+// partner and keeps the partner's other half, v_permlane32/16_swap then DPP - 34 instructions for 16 values over 32 lanes where 16
+// separate sums take 80.  The waves of a workgroup meet in LDS, workgroups of one group through slabs: no float atomics, results
 // do not depend on the order of execution.
 #include "ssm_scan.h"
 
@@ -17,10 +17,7 @@ namespace {
 
 using namespace gmt_ssm;
 
-template <int CTRL> __device__ __forceinline__ float dpp(float v) {
-    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
-}
-constexpr int DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E, DPP_XOR7 = 0x141, DPP_XOR8 = 0x128;     // quad_perm, row_half_mirror, row_ror:8
+constexpr int PARTS = 2;                                // lanes per channel (ssm_scan.h): bit 3 of the lane
 
 // (a, b) -> lanes with bit 5 (16 lanes: bit 4) clear: a summed over that bit, set: b
 __device__ __forceinline__ float half32(float a, float b) {
@@ -35,116 +32,133 @@ template <int CTRL> __device__ __forceinline__ float half_dpp(float a, float b, 
     const float keep = upper ? b : a, send = upper ? a : b;
     return keep + dpp<CTRL>(send);
 }
-// v[0 .. NV) summed over the wave: lane l returns value index_of(l)
-template <int NV> __device__ __forceinline__ float wave_sums(float (&v)[NV], int lane)
+// v[0 .. NV) summed over the 32 lanes of one part: lane l returns value index_of(l)
+template <int NV> __device__ __forceinline__ float part_sums(float (&v)[NV], int lane)
 {
-    static_assert(NV == 16 || NV == 32, "values per lane");
+    static_assert(NV == 8 || NV == 16 || NV == 32, "values per lane");
 #pragma unroll
     for (int i = 0; i < NV / 2; ++i) v[i] = half32(v[i], v[i + NV / 2]);
 #pragma unroll
     for (int i = 0; i < NV / 4; ++i) v[i] = half16(v[i], v[i + NV / 4]);
-    const bool b3 = lane & 8, b2 = lane & 4, b1 = lane & 2;
+    const bool b2 = lane & 4, b1 = lane & 2, b0 = lane & 1;
 #pragma unroll
-    for (int i = 0; i < NV / 8; ++i) v[i] = half_dpp<DPP_XOR8>(v[i], v[i + NV / 8], b3);
+    for (int i = 0; i < NV / 8; ++i) v[i] = half_dpp<DPP_XOR7>(v[i], v[i + NV / 8], b2);
+    if constexpr (NV >= 16) {
 #pragma unroll
-    for (int i = 0; i < NV / 16; ++i) v[i] = half_dpp<DPP_XOR7>(v[i], v[i + NV / 16], b2);
-    float s = v[0];
-    if constexpr (NV == 32) s = half_dpp<DPP_XOR2>(v[0], v[1], b1);
-    else s += dpp<DPP_XOR2>(s);
-    return s + dpp<DPP_XOR1>(s);
+        for (int i = 0; i < NV / 16; ++i) v[i] = half_dpp<DPP_XOR2>(v[i], v[i + NV / 16], b1);
+    } else v[0] += dpp<DPP_XOR2>(v[0]);
+    return NV == 32 ? half_dpp<DPP_XOR1>(v[0], v[1], b0) : v[0] + dpp<DPP_XOR1>(v[0]);
 }
-template <int NV> __device__ __forceinline__ int index_of(int lane) { return NV == 32 ? lane >> 1 : lane >> 2; }
+template <int NV> __device__ __forceinline__ int index_of(int lane) {        // bits 5, 4, 2, 1, 0 of the lane, the first log2(NV) of them
+    const int i = lane >> 4 << 3 | (lane & 7);
+    return NV == 32 ? i : NV == 16 ? i >> 1 : i >> 2;
+}
 
 // a segment's adjoint: (adjoint of its incoming state for a zero adjoint behind it, S)
 template <class T, class M, int NP, bool GATED>
-__global__ __launch_bounds__(256)
+__global__ __launch_bounds__(512)
 void scan_bwd_local_kernel(ScanArgs<T, M> a)
 {
+    constexpr int NS = NP / PARTS, OWN = CH / PARTS;
     __shared__ __align__(16) float sC[2][CH * NP];
     const int cb = blockIdx.x % a.p.cblk, rest = blockIdx.x / a.p.cblk;
     const int gr = rest % a.G, rest2 = rest / a.G;
     const int b = rest2 % a.B, seg = rest2 / a.B;
-    const int cg = a.C / a.G, ci = cb * a.p.width + threadIdx.x;
+    const Lanes<PARTS> ln;
+    const int cg = a.C / a.G, ci = cb * a.p.chans + ln.chan, n0 = ln.part * NS;
     const bool on = ci < cg;
-    const int c = gr * cg + (on ? ci : cg - 1);
+    const unsigned c = gr * cg + (on ? ci : cg - 1);
     const int len = length_of(a.lengths, b, a.L);
     const int t0 = seg * a.p.seglen, t1 = min(t0 + a.p.seglen, a.L), te = min(t1, len);
-    float A2[NP], g[NP];
-    load_states<NP>(a.A + (long long)c * a.N, a.N, A2);
+    float A2[NS], g[NS];
+    load_states<NS>(a.A + (long long)c * a.N, n0, a.N, A2);
 #pragma unroll
-    for (int n = 0; n < NP; ++n) { A2[n] *= LOG2E; g[n] = 0.f; }
+    for (int n = 0; n < NS; ++n) { A2[n] *= LOG2E; g[n] = 0.f; }
     const float bias = a.dt_bias ? a.dt_bias[c] : 0.f;
     const typename M::raw* Cp = a.Cm + b * a.C_b + gr * a.C_g;
+    const void *dp = row_of<T>(a.dt, b * a.dt_b), *zp = row_of<T>(a.z, b * a.z_b);
+    const int n_sc = (a.C + 31) / 32;
     float S = 0.f;
-    int buf = 0;
-    for (int k = te > t0 ? (te - t0 + CH - 1) / CH - 1 : -1; k >= 0; --k, buf ^= 1) {
-        const int tc = t0 + k * CH;
-        typename T::raw dr[CH], zr[CH];
-        typename M::raw yr[CH];
-        MapTile<M, NP> mC;
-#pragma unroll
-        for (int s = 0; s < CH; ++s) {
-            const int t = min(tc + s, te - 1);
-            dr[s] = load_elem<T, M, 1>(a, t, b, c);
-            if (GATED) zr[s] = load_elem<T, M, 2>(a, t, b, c);
-            yr[s] = a.dy[t * a.dy_t + b * a.dy_b + c];
-        }
+    Own<T, PARTS> dr, zr;
+    Own<M, PARTS> yr;
+    MapTile<M, NP> mC;
+    auto request = [&](int tc) {
+        const bool full = tc + CH <= te;
+        dr.request(dp, a.dts, a.dt_t, tc, te, full, ln.part, c, a.B, b, n_sc);
+        if (GATED) zr.request(zp, a.zs, a.z_t, tc, te, full, ln.part, c, a.B, b, n_sc);
+        yr.request(a.dy + b * a.dy_b, nullptr, a.dy_t, tc, te, full, ln.part, c, a.B, b, n_sc);
         mC.request(Cp, a.C_t, tc, te, a.N);
+    };
+    int buf = 0, k = te > t0 ? (te - t0 + CH - 1) / CH - 1 : -1;
+    if (k >= 0) request(t0 + k * CH);
+    for (; k >= 0; --k, buf ^= 1) {
+        const int tc = t0 + k * CH;
+        float st[OWN], d[OWN];
+#pragma unroll
+        for (int j = 0; j < OWN; ++j) {
+            const bool live = tc + j * PARTS + ln.part < te;
+            float sig;
+            st[j] = softplus(to_f(dr.v[j]) + bias, sig);
+            st[j] = live ? st[j] : 0.f;
+            d[j] = live ? to_f(yr.v[j]) : 0.f;
+            if (GATED) { const float zv = live ? to_f(zr.v[j]) : 0.f; d[j] *= zv * sigmoid(zv); }
+            S += st[j];
+        }
         mC.put(sC[buf]);
         __syncthreads();
+        if (k > 0) request(tc - CH);
 #pragma unroll
         for (int s = CH - 1; s >= 0; --s) {
-            const bool live = tc + s < te;
-            float sig, st = softplus(to_f(dr[s]) + bias, sig);
-            st = live ? st : 0.f;
-            pin(st);
-            float d = live ? to_f(yr[s]) : 0.f;
-            if (GATED) { const float zv = live ? to_f(zr[s]) : 0.f; d *= zv * sigmoid(zv); }
-            S += st;
+            float sts = ln.of_step(st, s);
+            const float ds = ln.of_step(d, s);
+            pin(sts);
 #pragma unroll
-            for (int n = 0; n < NP; ++n) g[n] = __builtin_amdgcn_exp2f(st * A2[n]) * fmaf(d, sC[buf][s * NP + n], g[n]);
+            for (int n = 0; n < NS; ++n) g[n] = __builtin_amdgcn_exp2f(sts * A2[n]) * fmaf(ds, sC[buf][s * NP + n0 + n], g[n]);
             step_fence();
         }
     }
+    S = ln.sum(S);
     if (!on) return;
-    store_kept<NP>(a.seg_h, seg, a.B, b, a.C, c, g);
-    a.seg_s[(long long)(seg * a.B + b) * a.C + c] = S;
+    store_kept<NP, NS>(a.seg_h, seg, a.B, b, a.C, c, n0, g);
+    if (ln.part == 0) a.seg_s[(long long)(seg * a.B + b) * a.C + c] = S;
 }
 
 template <class T, class M, int NP, bool GATED>
-__global__ __launch_bounds__(256, 1)
+__global__ __launch_bounds__(512, 2)
 void scan_bwd_kernel(ScanArgs<T, M> a)
 {
-    constexpr int NV = NP == 8 ? 16 : 32;               // values per wave_sums call: dB and dC together, or one after the other
+    constexpr int NS = NP / PARTS, OWN = CH / PARTS;
+    constexpr bool KEEP_E = NP <= 16;                   // the exponentials of a chunk stay in registers (N = 32: computed twice)
     __shared__ __align__(16) float sB[2][CH * NP], sC[2][CH * NP];
-    __shared__ float red[2][4][CH][2 * NP];
+    __shared__ float red[2][8][CH][2 * NP];             // [wave][step][part][dB, dC of the part's states]
     const int cb = blockIdx.x % a.p.cblk, rest = blockIdx.x / a.p.cblk;
     const int gr = rest % a.G, slab = rest / a.G;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int cg = a.C / a.G, ci = cb * a.p.width + threadIdx.x;
-    const bool on = ci < cg, wave_on = ci - lane < cg;
-    const int c = gr * cg + (on ? ci : cg - 1);         // lanes beyond the group repeat its last channel, outside the sums
-    float A2[NP], dA[NP], dD = 0.f, dbias = 0.f;
-    load_states<NP>(a.A + (long long)c * a.N, a.N, A2);
+    const Lanes<PARTS> ln;
+    const int cg = a.C / a.G, ci = cb * a.p.chans + ln.chan, n0 = ln.part * NS;
+    const bool on = ci < cg, wave_on = cb * a.p.chans + wave * (64 / PARTS) < cg;
+    const unsigned c = gr * cg + (on ? ci : cg - 1);    // lanes beyond the group repeat its last channel with x = dy = 0
+    float A2[NS], dA[NS], dD = 0.f, dbias = 0.f;
+    load_states<NS>(a.A + (long long)c * a.N, n0, a.N, A2);
 #pragma unroll
-    for (int n = 0; n < NP; ++n) { A2[n] *= LOG2E; dA[n] = 0.f; }
+    for (int n = 0; n < NS; ++n) { A2[n] *= LOG2E; dA[n] = 0.f; }
     const float bias = a.dt_bias ? a.dt_bias[c] : 0.f, Dc = a.D ? a.D[c] : 0.f;
     const long long tbg = (long long)a.L * a.B * a.G * a.N;
+    const int n_sc = (a.C + 31) / 32;
 
-    auto put_bc = [&](int t, int b, int j, float v) {   // j < NP: dB, else dC
-        const int n = j % NP;
+    auto put_bc = [&](int t, int b, bool is_c, int n, float v) {
         const long long at = (((long long)t * a.B + b) * a.G + gr) * a.N + n;
-        if (a.p.cblk > 1) a.bc_part[(long long)cb * 2 * tbg + (j < NP ? 0 : tbg) + at] = v;
-        else (j < NP ? a.dB : a.dC)[at] = from_f<M>(v);
+        if (a.p.cblk > 1) a.bc_part[(long long)cb * 2 * tbg + (is_c ? tbg : 0) + at] = v;
+        else (is_c ? a.dC : a.dB)[at] = from_f<M>(v);
     };
     int buf = 0, p_tc = 0, p_te = 0, p_b = 0;           // the chunk whose sums wait in red[buf ^ 1]: steps p_tc .. p_te - 1
     auto flush = [&]() {
         for (int i = threadIdx.x; i < CH * 2 * NP; i += a.p.width) {
-            const int s = i / (2 * NP), j = i % (2 * NP);
-            if (p_tc + s >= p_te || j % NP >= a.N) continue;
+            const int s = i / (2 * NP), j = i % (2 * NP), n = j / (2 * NS) * NS + j % NS;
+            if (p_tc + s >= p_te || n >= a.N) continue;
             float v = 0.f;
             for (int w = 0; w < a.p.waves; ++w) v += red[buf ^ 1][w][s][j];
-            put_bc(p_tc + s, p_b, j, v);
+            put_bc(p_tc + s, p_b, j % (2 * NS) >= NS, n, v);
         }
     };
 
@@ -156,119 +170,129 @@ void scan_bwd_kernel(ScanArgs<T, M> a)
         const long long row = (long long)b * a.C + c;
         const typename M::raw* Bp = a.Bm + b * a.B_b + gr * a.B_g;
         const typename M::raw* Cp = a.Cm + b * a.C_b + gr * a.C_g;
-        float gc[NP];                                   // exp(step[t+1] A) g[t+1]
+        const void *xp = row_of<T>(a.x, b * a.x_b), *dp = row_of<T>(a.dt, b * a.dt_b), *zp = row_of<T>(a.z, b * a.z_b);
+        float gc[NS];                                   // exp(step[t+1] A) g[t+1]
 #pragma unroll
-        for (int n = 0; n < NP; ++n) gc[n] = 0.f;
-        {
-            if (a.p.nseg > 1) load_kept<NP>(a.seg_h, seg, a.B, b, a.C, c, gc);
-            else if (a.dstate_out) load_states<NP>(a.dstate_out + row * a.N, a.N, gc);
+        for (int n = 0; n < NS; ++n) gc[n] = 0.f;
+        if (on) {
+            if (a.p.nseg > 1) load_kept<NP, NS>(a.seg_h, seg, a.B, b, a.C, c, n0, gc);
+            else if (a.dstate_out) load_states<NS>(a.dstate_out + row * a.N, n0, a.N, gc);
         }
-        typename T::raw xr[CH], dr[CH], zr[CH];
-        typename M::raw yr[CH];
+        Own<T, PARTS> xr, dr, zr;
+        Own<M, PARTS> yr;
         MapTile<M, NP> mB, mC;
-        float hk[NP];
+        float hk[NS];
         auto request = [&](int tc) {
-#pragma unroll
-            for (int s = 0; s < CH; ++s) {
-                const int t = min(tc + s, te - 1);
-                xr[s] = load_elem<T, M, 0>(a, t, b, c);
-                dr[s] = load_elem<T, M, 1>(a, t, b, c);
-                if (GATED) zr[s] = load_elem<T, M, 2>(a, t, b, c);
-                yr[s] = a.dy[t * a.dy_t + b * a.dy_b + c];
-            }
+            const bool full = tc + CH <= te;
+            xr.request(xp, a.xs, a.x_t, tc, te, full, ln.part, c, a.B, b, n_sc);
+            dr.request(dp, a.dts, a.dt_t, tc, te, full, ln.part, c, a.B, b, n_sc);
+            if (GATED) zr.request(zp, a.zs, a.z_t, tc, te, full, ln.part, c, a.B, b, n_sc);
+            yr.request(a.dy + b * a.dy_b, nullptr, a.dy_t, tc, te, full, ln.part, c, a.B, b, n_sc);
             mB.request(Bp, a.B_t, tc, te, a.N);
             mC.request(Cp, a.C_t, tc, te, a.N);
-            if (tc > 0) load_kept<NP>(a.ck, tc / CH - 1, a.B, b, a.C, c, hk);
-            else if (a.state) load_states<NP>(a.state + row * a.N, a.N, hk);
+            if (tc > 0) load_kept<NP, NS>(a.ck, tc / CH - 1, a.B, b, a.C, c, n0, hk);
+            else if (a.state) load_states<NS>(a.state + row * a.N, n0, a.N, hk);
             else {
 #pragma unroll
-                for (int n = 0; n < NP; ++n) hk[n] = 0.f;
+                for (int n = 0; n < NS; ++n) hk[n] = 0.f;
             }
         };
         int k = te > t0 ? (te - t0 + CH - 1) / CH - 1 : -1;
         if (k >= 0) request(t0 + k * CH);
         for (; k >= 0; --k) {
             const int tc = t0 + k * CH;
-            typename T::raw xc[CH], dc[CH], zc[CH];
-            typename M::raw yc[CH];
-            float h[CH + 1][NP], st[CH], sig[CH], out[CH];
+            float h[CH + 1][NS], ex[KEEP_E ? CH : 1][NS];
+            float xv[OWN], st[OWN], sig[OWN], d[OWN], dyv[OWN], zv[OWN], out[OWN], gBk[OWN], qAk[OWN];
 #pragma unroll
-            for (int s = 0; s < CH; ++s) { xc[s] = xr[s]; dc[s] = dr[s]; zc[s] = zr[s]; yc[s] = yr[s]; }
+            for (int j = 0; j < OWN; ++j) {
+                const bool live = tc + j * PARTS + ln.part < te;        // behind the row's end: a step of 0 with no adjoint of its own
+                xv[j] = live && on ? to_f(xr.v[j]) : 0.f;
+                const float v = softplus(to_f(dr.v[j]) + bias, sig[j]);
+                st[j] = live ? v : 0.f;
+                sig[j] = live ? sig[j] : 0.f;
+                dyv[j] = d[j] = live && on ? to_f(yr.v[j]) : 0.f;
+                if (GATED) { zv[j] = live ? to_f(zr.v[j]) : 0.f; d[j] *= zv[j] * sigmoid(zv[j]); }
+                out[j] = gBk[j] = qAk[j] = 0.f;
+            }
 #pragma unroll
-            for (int n = 0; n < NP; ++n) h[0][n] = hk[n];
+            for (int n = 0; n < NS; ++n) h[0][n] = hk[n];
             mB.put(sB[buf]);
             mC.put(sC[buf]);
             __syncthreads();
             flush();                                    // the sums of the chunk before, written before the barrier
-            if (k > 0) request(tc - CH);
-            const float *tB = sB[buf], *tC = sC[buf];
             if (wave_on) {
 #pragma unroll
                 for (int s = 0; s < CH; ++s) {
-                    const bool live = tc + s < te;      // behind the row's end: a step of 0 with no adjoint of its own
-                    const float xv = live ? to_f(xc[s]) : 0.f, v = softplus(to_f(dc[s]) + bias, sig[s]);
-                    st[s] = live ? v : 0.f;
-                    sig[s] = live ? sig[s] : 0.f;
-                    pin(st[s]);
-                    const float sx = st[s] * xv;
-                    float o = Dc * xv;
+                    float sts = ln.of_step(st, s);
+                    const float sxs = sts * ln.of_step(xv, s);
+                    pin(sts);
+                    const float *Bt = sB[buf] + s * NP + n0, *Ct = sC[buf] + s * NP + n0;
+                    float o = 0.f;
 #pragma unroll
-                    for (int n = 0; n < NP; ++n) {
-                        const float e = __builtin_amdgcn_exp2f(st[s] * A2[n]);
-                        h[s + 1][n] = fmaf(e, h[s][n], sx * tB[s * NP + n]);
-                        if (GATED) o = fmaf(h[s + 1][n], tC[s * NP + n], o);
+                    for (int n = 0; n < NS; ++n) {
+                        const float e = __builtin_amdgcn_exp2f(sts * A2[n]);
+                        if (KEEP_E) ex[KEEP_E ? s : 0][n] = e;
+                        h[s + 1][n] = fmaf(e, h[s][n], sxs * Bt[n]);
+                        if (GATED) o = fmaf(h[s + 1][n], Ct[n], o);
                     }
-                    out[s] = o;
+                    if (GATED) { o = ln.sum(o); pin(o); ln.keep(out, s, o); }
+                    step_fence();
+                }
+                if (GATED) {
+#pragma unroll
+                    for (int j = 0; j < OWN; ++j) {
+                        const float sz = sigmoid(zv[j]);
+                        if (tc + j * PARTS + ln.part < t1 && on)
+                            (a.dz + ((long long)(tc + j * PARTS) * a.B + b) * a.C)[(unsigned)(ln.part * a.B * a.C) + c] =
+                                from_f<M>(dyv[j] * fmaf(Dc, xv[j], out[j]) * sz * fmaf(zv[j], 1.0f - sz, 1.0f));
+                    }
                     step_fence();
                 }
 #pragma unroll
                 for (int s = CH - 1; s >= 0; --s) {
-                    const int t = tc + s;
-                    const bool live = t < te;
-                    pin(st[s]);                         // the exponentials again, not kept in 128 registers
-                    const float xv = live ? to_f(xc[s]) : 0.f, dyv = live ? to_f(yc[s]) : 0.f, sx = st[s] * xv;
-                    float d = dyv, dz = 0.f;
-                    if (GATED) {
-                        const float zv = live ? to_f(zc[s]) : 0.f, sz = sigmoid(zv);
-                        d = dyv * zv * sz;
-                        dz = dyv * out[s] * sz * fmaf(zv, 1.0f - sz, 1.0f);
-                    }
-                    dD = fmaf(d, xv, dD);
-                    const float sxm = on ? sx : 0.f, dm = on ? d : 0.f;
-                    float gB = 0.f, qA = 0.f, vB[NP], vC[NP];
+                    // the next chunk's elements: by now half of h and ex is free again
+                    if (s == CH / 2 - 1 && k > 0) request(tc - CH);
+                    float sts = ln.of_step(st, s);
+                    const float sxs = sts * ln.of_step(xv, s), ds = ln.of_step(d, s);
+                    pin(sts);
+                    const float *Bt = sB[buf] + s * NP + n0, *Ct = sC[buf] + s * NP + n0;
+                    float gB = 0.f, qA = 0.f, v[2 * NS];
 #pragma unroll
-                    for (int n = 0; n < NP; ++n) {
-                        const float e = __builtin_amdgcn_exp2f(st[s] * A2[n]);
-                        const float gn = fmaf(d, tC[s * NP + n], gc[n]);
-                        vB[n] = gn * sxm;
-                        vC[n] = h[s + 1][n] * dm;
-                        gB = fmaf(gn, tB[s * NP + n], gB);
+                    for (int n = 0; n < NS; ++n) {
+                        const float e = KEEP_E ? ex[KEEP_E ? s : 0][n] : __builtin_amdgcn_exp2f(sts * A2[n]);
+                        const float gn = fmaf(ds, Ct[n], gc[n]);
+                        v[n] = gn * sxs;
+                        v[NS + n] = h[s + 1][n] * ds;
+                        gB = fmaf(gn, Bt[n], gB);
                         gc[n] = gn * e;
                         const float q = gc[n] * h[s][n];
                         qA = fmaf(q, A2[n], qA);
-                        dA[n] = fmaf(q, st[s], dA[n]);
+                        dA[n] = fmaf(q, sts, dA[n]);
                     }
-                    const float dstep = fmaf(gB, xv, qA * LN2) * sig[s];
-                    dbias += dstep;
-                    if (t < t1) {
-                        const long long at = ((long long)t * a.B + b) * a.C + c;
-                        a.dx[at] = from_f<M>(fmaf(gB, st[s], Dc * d));
-                        a.ddt[at] = from_f<M>(dstep);
-                        if (GATED) a.dz[at] = from_f<M>(dz);
-                    }
-                    if constexpr (NP <= 16) {
-                        float v[NV];
+                    gB = ln.sum(gB); qA = ln.sum(qA);
+                    pin(gB); pin(qA);
 #pragma unroll
-                        for (int n = 0; n < NP; ++n) { v[n] = vB[n]; v[NP + n] = vC[n]; }
-                        red[buf][wave][s][index_of<NV>(lane)] = wave_sums<NV>(v, lane);
-                    } else {
-                        red[buf][wave][s][index_of<NV>(lane)] = wave_sums<NV>(vB, lane);
-                        red[buf][wave][s][NP + index_of<NV>(lane)] = wave_sums<NV>(vC, lane);
-                    }
+                    for (int n = 0; n < NS; ++n) pin(dA[n]);
+                    ln.keep(gBk, s, gB);
+                    ln.keep(qAk, s, qA);
+                    red[buf][wave][s][ln.part * 2 * NS + index_of<2 * NS>(lane)] = part_sums<2 * NS>(v, lane);
                     step_fence();
                 }
-            }
-            else {
+#pragma unroll
+                for (int j = 0; j < OWN; ++j) {
+                    const int t = tc + j * PARTS + ln.part;
+                    const float dstep = fmaf(gBk[j], xv[j], qAk[j] * LN2) * sig[j];
+                    dbias += dstep;
+                    dD = fmaf(d[j], xv[j], dD);
+                    if (t < t1 && on) {
+                        const long long base = ((long long)(tc + j * PARTS) * a.B + b) * a.C;
+                        const unsigned at = (unsigned)(ln.part * a.B * a.C) + c;
+                        (a.dx + base)[at] = from_f<M>(fmaf(gBk[j], st[j], Dc * d[j]));
+                        (a.ddt + base)[at] = from_f<M>(dstep);
+                    }
+                }
+            } else {
+                if (k > 0) request(tc - CH);            // (its share of B and C)
 #pragma unroll
                 for (int s = 0; s < CH; ++s)
                     for (int j = lane; j < 2 * NP; j += 64) red[buf][wave][s][j] = 0.f;
@@ -277,8 +301,8 @@ void scan_bwd_kernel(ScanArgs<T, M> a)
             buf ^= 1;
         }
         if (on) {
-            if (a.dstate && seg == 0) store_states<NP>(a.dstate + row * a.N, a.N, gc);
-            for (int t = t0 + (max(te - t0, 0) + CH - 1) / CH * CH; t < t1; ++t) {       // chunks behind the row's end
+            if (a.dstate && seg == 0) store_states<NS>(a.dstate + row * a.N, n0, a.N, gc);
+            for (int t = t0 + (max(te - t0, 0) + CH - 1) / CH * CH + ln.part; t < t1; t += PARTS) {     // chunks behind the row's end
                 const long long at = ((long long)t * a.B + b) * a.C + c;
                 a.dx[at] = from_f<M>(0.f);
                 a.ddt[at] = from_f<M>(0.f);
@@ -287,16 +311,20 @@ void scan_bwd_kernel(ScanArgs<T, M> a)
         }
         const int z0 = max(t0, len);
         for (int i = threadIdx.x; i < (t1 - z0) * 2 * NP; i += a.p.width)
-            if (i % NP < a.N) put_bc(z0 + i / (2 * NP), b, i % (2 * NP), 0.f);
+            if (i % NP < a.N) put_bc(z0 + i / (2 * NP), b, i % (2 * NP) >= NP, i % NP, 0.f);
     }
     __syncthreads();
     flush();
+    dD = ln.sum(dD);
+    dbias = ln.sum(dbias);
     if (!on) return;
     float* part = a.part + (long long)slab * a.C * (a.N + 2);
 #pragma unroll
-    for (int n = 0; n < NP; ++n) if (n < a.N) part[(long long)c * a.N + n] = dA[n];
-    part[(long long)a.C * a.N + c] = dD;
-    part[(long long)a.C * (a.N + 1) + c] = dbias;
+    for (int n = 0; n < NS; ++n) if (n0 + n < a.N) part[(long long)c * a.N + n0 + n] = dA[n];
+    if (ln.part == 0) {
+        part[(long long)a.C * a.N + c] = dD;
+        part[(long long)a.C * (a.N + 1) + c] = dbias;
+    }
 }
 
 // dB and dC of several workgroups across a group's channels: sums in a fixed order
@@ -320,7 +348,7 @@ int slabs(const ScanPlan& p, int B, int G)
 struct BwdSpace { long long part, bc, seg_h, seg_s, total; };
 BwdSpace bwd_space(const gmt_scan_args* a)
 {
-    const ScanPlan p = scan_plan(a->L, a->B, a->C, a->N, a->G);
+    const ScanPlan p = bwd_plan(a->L, a->B, a->C, a->N, a->G);
     BwdSpace s;
     s.part = 0;
     s.bc = s.part + (long long)slabs(p, a->B, a->G) * a->C * (a->N + 2);
@@ -344,12 +372,12 @@ template <class T, class M, int NP, bool GATED> int launch(const ScanArgs<T, M>&
 }
 template <class T, class M, int NP> int by_gate(const ScanArgs<T, M>& a, hipStream_t stream)
 {
-    return a.zq ? launch<T, M, NP, true>(a, stream) : launch<T, M, NP, false>(a, stream);
+    return a.z ? launch<T, M, NP, true>(a, stream) : launch<T, M, NP, false>(a, stream);
 }
 
 template <class T, class M> int run(const gmt_scan_args* args, hipStream_t stream)
 {
-    ScanArgs<T, M> a = scan_args<T, M>(args);
+    ScanArgs<T, M> a = scan_args<T, M>(args, bwd_plan(args->L, args->B, args->C, args->N, args->G));
     const BwdSpace s = bwd_space(args);
     if (args->workspace_floats < s.total) return GMT_ERR_WORKSPACE;
     a.P = slabs(a.p, a.B, a.G);
@@ -377,7 +405,7 @@ extern "C" int gmt_selective_scan_bwd(const gmt_scan_args* a, hipStream_t stream
     if (int rc = scan_check(a)) return rc;
     GMT_CHECK_ARG(a->dy && a->dx && a->ddt && a->dB && a->dC && a->dparam && a->workspace && (!a->z || a->dz));
     GMT_CHECK_ARG(a->ck || a->L <= CH);
-    GMT_CHECK_ARG((long long)a->B * scan_plan(a->L, a->B, a->C, a->N, a->G).nseg < (1LL << 31));
+    GMT_CHECK_ARG((long long)a->B * bwd_plan(a->L, a->B, a->C, a->N, a->G).nseg < (1LL << 31));
     if (a->x_scale) {
         if (a->L > CH) { if (int rc = scan_states_q8(a, stream)) return rc; }
         return a->bf16 ? run<Q8, B16>(a, stream) : run<Q8, F32>(a, stream);

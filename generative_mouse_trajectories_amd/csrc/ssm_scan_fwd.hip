@@ -9,44 +9,45 @@ using namespace gmt_ssm;
 // what a launch writes: y; y and the kept states; the kept states alone; a segment's (h_loc, S)
 enum Mode { OUT = 0, TRAIN = 1, STATES = 2, LOCAL = 3 };
 
-template <class T, class M, int NP, int MODE, bool GATED>
+template <class T, class M, int NP, int PARTS, int MODE, bool GATED>
 __global__ __launch_bounds__(256)
 void scan_fwd_kernel(ScanArgs<T, M> a)
 {
     constexpr bool Y = MODE == OUT || MODE == TRAIN, KEEP = MODE == TRAIN || MODE == STATES;
+    constexpr int NS = NP / PARTS, OWN = CH / PARTS;
     __shared__ __align__(16) float sB[2][CH * NP], sC[Y ? 2 : 1][Y ? CH * NP : 1];
     const int cb = blockIdx.x % a.p.cblk, rest = blockIdx.x / a.p.cblk;
     const int g = rest % a.G, rest2 = rest / a.G;
     const int b = rest2 % a.B, seg = rest2 / a.B;
-    const int cg = a.C / a.G, ci = cb * a.p.width + threadIdx.x;
-    const bool on = ci < cg, wave_on = ci - (int)(threadIdx.x & 63) < cg;
-    const int c = g * cg + (on ? ci : cg - 1);          // lanes beyond the group repeat its last channel
+    const Lanes<PARTS> ln;
+    const int cg = a.C / a.G, ci = cb * a.p.chans + ln.chan, n0 = ln.part * NS;
+    const bool on = ci < cg, wave_on = cb * a.p.chans + (int)(threadIdx.x >> 6) * (64 / PARTS) < cg;
+    const unsigned c = g * cg + (on ? ci : cg - 1);     // lanes beyond the group repeat its last channel
     const int len = length_of(a.lengths, b, a.L);
     const int t0 = seg * a.p.seglen, t1 = min(t0 + a.p.seglen, a.L), te = min(t1, len);
 
-    float A2[NP], h[NP];
-    load_states<NP>(a.A + (long long)c * a.N, a.N, A2);
+    float A2[NS], h[NS];
+    load_states<NS>(a.A + (long long)c * a.N, n0, a.N, A2);
 #pragma unroll
-    for (int n = 0; n < NP; ++n) { A2[n] *= LOG2E; h[n] = 0.f; }
+    for (int n = 0; n < NS; ++n) { A2[n] *= LOG2E; h[n] = 0.f; }
     const long long row = (long long)b * a.C + c;
     if (MODE != LOCAL) {
-        if (a.p.nseg > 1) load_kept<NP>(a.seg_h, seg, a.B, b, a.C, c, h);
-        else if (a.state) load_states<NP>(a.state + row * a.N, a.N, h);
+        if (a.p.nseg > 1) load_kept<NP, NS>(a.seg_h, seg, a.B, b, a.C, c, n0, h);
+        else if (a.state) load_states<NS>(a.state + row * a.N, n0, a.N, h);
     }
     const float bias = a.dt_bias ? a.dt_bias[c] : 0.f, Dc = Y && a.D ? a.D[c] : 0.f;
     const typename M::raw* Bp = a.Bm + b * a.B_b + g * a.B_g;
     const typename M::raw* Cp = a.Cm + b * a.C_b + g * a.C_g;
+    const void *xp = row_of<T>(a.x, b * a.x_b), *dp = row_of<T>(a.dt, b * a.dt_b), *zp = row_of<T>(a.z, b * a.z_b);
+    const int n_sc = (a.C + 31) / 32;
 
-    typename T::raw xr[CH], dr[CH], zr[CH];
+    Own<T, PARTS> xr, dr, zr;
     MapTile<M, NP> mB, mC;
     auto request = [&](int tc) {
-#pragma unroll
-        for (int s = 0; s < CH; ++s) {
-            const int t = min(tc + s, te - 1);          // (behind the end: the last step again, masked below)
-            xr[s] = load_elem<T, M, 0>(a, t, b, c);
-            dr[s] = load_elem<T, M, 1>(a, t, b, c);
-            if (GATED) zr[s] = load_elem<T, M, 2>(a, t, b, c);
-        }
+        const bool full = tc + CH <= te;
+        xr.request(xp, a.xs, a.x_t, tc, te, full, ln.part, c, a.B, b, n_sc);
+        dr.request(dp, a.dts, a.dt_t, tc, te, full, ln.part, c, a.B, b, n_sc);
+        if (GATED) zr.request(zp, a.zs, a.z_t, tc, te, full, ln.part, c, a.B, b, n_sc);
         mB.request(Bp, a.B_t, tc, te, a.N);
         if (Y) mC.request(Cp, a.C_t, tc, te, a.N);
     };
@@ -54,55 +55,65 @@ void scan_fwd_kernel(ScanArgs<T, M> a)
     if (te > t0) request(t0);
     int buf = 0;
     for (int tc = t0; tc < te; tc += CH, buf ^= 1) {
-        typename T::raw xc[CH], dc[CH], zc[CH];
-#pragma unroll
-        for (int s = 0; s < CH; ++s) { xc[s] = xr[s]; dc[s] = dr[s]; zc[s] = zr[s]; }
+        const Own<T, PARTS> xc = xr, dc = dr, zc = zr;
         mB.put(sB[buf]);
         if (Y) mC.put(sC[Y ? buf : 0]);
         // one barrier a chunk: a buffer is written again two chunks later, behind the next barrier, which its readers have passed
         __syncthreads();
         if (tc + CH < te) request(tc + CH);
-        if (KEEP && tc > 0 && wave_on) store_kept<NP>(a.ck, tc / CH - 1, a.B, b, a.C, c, h);
+        if (KEEP && tc > 0 && wave_on) store_kept<NP, NS>(a.ck, tc / CH - 1, a.B, b, a.C, c, n0, h);
         if (MODE == STATES && tc + CH >= te) break;     // nothing is kept behind the last chunk
         if (wave_on) {
+            float xv[OWN], st[OWN];                     // st: the step, then (its step done) the sum over the states
+#pragma unroll
+            for (int j = 0; j < OWN; ++j) {
+                const bool live = tc + j * PARTS + ln.part < te;        // behind the row's end: a step of 0, which changes nothing
+                float sig;
+                xv[j] = live ? to_f(xc.v[j]) : 0.f;
+                st[j] = softplus(to_f(dc.v[j]) + bias, sig);
+                st[j] = live ? st[j] : 0.f;
+                if (MODE == LOCAL) S += st[j];
+            }
 #pragma unroll
             for (int s = 0; s < CH; ++s) {
-                const int t = tc + s;
-                const bool live = t < te;               // behind the row's end: a step of 0, which changes nothing
-                const float xv = live ? to_f(xc[s]) : 0.f;
-                float sig, st = softplus(to_f(dc[s]) + bias, sig);
-                st = live ? st : 0.f;
-                pin(st);
-                const float sx = st * xv;
-                if (MODE == LOCAL) S += st;
+                float sts = ln.of_step(st, s);
+                const float sxs = sts * ln.of_step(xv, s);
+                pin(sts);
                 float y0 = 0.f, y1 = 0.f;
-                const float* Bt = sB[buf] + s * NP;
-                const float* Ct = sC[Y ? buf : 0] + (Y ? s * NP : 0);
+                const float* Bt = sB[buf] + s * NP + n0;
+                const float* Ct = sC[Y ? buf : 0] + (Y ? s * NP + n0 : 0);
 #pragma unroll
-                for (int n = 0; n < NP; ++n) {
-                    const float e = __builtin_amdgcn_exp2f(st * A2[n]);
-                    h[n] = fmaf(e, h[n], sx * Bt[n]);
+                for (int n = 0; n < NS; ++n) {
+                    const float e = __builtin_amdgcn_exp2f(sts * A2[n]);
+                    h[n] = fmaf(e, h[n], sxs * Bt[n]);
                     if (Y) { if (n & 1) y1 = fmaf(h[n], Ct[n], y1); else y0 = fmaf(h[n], Ct[n], y0); }
                 }
-                if (Y) {
-                    float o = fmaf(Dc, xv, y0 + y1);
-                    if (GATED) { const float zv = to_f(zc[s]); o *= zv * sigmoid(zv); }
-                    if (t < t1) a.y[((long long)t * a.B + b) * a.C + c] = from_f<M>(live ? o : 0.f);
-                }
+                if (Y) { float y = ln.sum(y0 + y1); pin(y); ln.keep(st, s, y); }
                 step_fence();
+            }
+            if (Y) {
+#pragma unroll
+                for (int j = 0; j < OWN; ++j) {
+                    const int t = tc + j * PARTS + ln.part;
+                    float o = fmaf(Dc, xv[j], st[j]);
+                    if (GATED) { const float zv = to_f(zc.v[j]); o *= zv * sigmoid(zv); }
+                    typename M::raw* yp = a.y + ((long long)(tc + j * PARTS) * a.B + b) * a.C;
+                    if (t < t1) yp[(unsigned)(ln.part * a.B * a.C) + c] = from_f<M>(t < te ? o : 0.f);
+                }
             }
         }
     }
     if (!on) return;
     if (MODE == LOCAL) {
-        store_kept<NP>(a.seg_h, seg, a.B, b, a.C, c, h);
-        a.seg_s[(long long)(seg * a.B + b) * a.C + c] = S;
+        store_kept<NP, NS>(a.seg_h, seg, a.B, b, a.C, c, n0, h);
+        S = ln.sum(S);
+        if (ln.part == 0) a.seg_s[(long long)(seg * a.B + b) * a.C + c] = S;
         return;
     }
     // the segment in which the row ends (the first one for an empty row) holds its final state
-    if (Y && a.state_out && ((len > t0 && len <= t1) || (len == 0 && seg == 0))) store_states<NP>(a.state_out + row * a.N, a.N, h);
+    if (Y && a.state_out && ((len > t0 && len <= t1) || (len == 0 && seg == 0))) store_states<NS>(a.state_out + row * a.N, n0, a.N, h);
     if (Y)
-        for (int t = t0 + (max(te - t0, 0) + CH - 1) / CH * CH; t < t1; ++t) a.y[((long long)t * a.B + b) * a.C + c] = from_f<M>(0.f);
+        for (int t = t0 + (max(te - t0, 0) + CH - 1) / CH * CH + ln.part; t < t1; t += PARTS) a.y[((long long)t * a.B + b) * a.C + c] = from_f<M>(0.f);
 }
 
 // seg_h: (h_loc of every segment) -> (its incoming state), in place.  A thread is one state of one channel and row.
@@ -174,27 +185,31 @@ void scan_step_kernel(const typename M::raw* __restrict__ x, long long x_b, cons
     }
 }
 
-template <class T, class M, int NP, int MODE> int launch(const ScanArgs<T, M>& a, hipStream_t stream)
+template <class T, class M, int NP, int PARTS, int MODE> int launch(const ScanArgs<T, M>& a, hipStream_t stream)
 {
     const dim3 grid((unsigned)((long long)a.p.cblk * a.G * a.B * a.p.nseg));
     if constexpr (MODE == OUT || MODE == TRAIN) {
-        if (a.zq) hipLaunchKernelGGL((scan_fwd_kernel<T, M, NP, MODE, true>), grid, dim3(a.p.width), 0, stream, a);
-        else hipLaunchKernelGGL((scan_fwd_kernel<T, M, NP, MODE, false>), grid, dim3(a.p.width), 0, stream, a);
+        if (a.z) hipLaunchKernelGGL((scan_fwd_kernel<T, M, NP, PARTS, MODE, true>), grid, dim3(a.p.width), 0, stream, a);
+        else hipLaunchKernelGGL((scan_fwd_kernel<T, M, NP, PARTS, MODE, false>), grid, dim3(a.p.width), 0, stream, a);
     } else {
-        hipLaunchKernelGGL((scan_fwd_kernel<T, M, NP, MODE, false>), grid, dim3(a.p.width), 0, stream, a);
+        hipLaunchKernelGGL((scan_fwd_kernel<T, M, NP, PARTS, MODE, false>), grid, dim3(a.p.width), 0, stream, a);
     }
     GMT_LAUNCH_CHECK();
     return GMT_OK;
 }
+template <class T, class M, int NP, int MODE> int by_parts(const ScanArgs<T, M>& a, hipStream_t stream)
+{
+    return a.p.parts == 1 ? launch<T, M, NP, 1, MODE>(a, stream) : launch<T, M, NP, 2, MODE>(a, stream);
+}
 template <class T, class M, int MODE> int by_np(const ScanArgs<T, M>& a, hipStream_t stream)
 {
-    return a.p.np == 8 ? launch<T, M, 8, MODE>(a, stream) : a.p.np == 16 ? launch<T, M, 16, MODE>(a, stream) : launch<T, M, 32, MODE>(a, stream);
+    return a.p.np == 8 ? by_parts<T, M, 8, MODE>(a, stream) : a.p.np == 16 ? by_parts<T, M, 16, MODE>(a, stream) : by_parts<T, M, 32, MODE>(a, stream);
 }
 
 // segments (if any), then the pass itself
 template <class T, class M, int MODE> int run(const gmt_scan_args* args, hipStream_t stream)
 {
-    ScanArgs<T, M> a = scan_args<T, M>(args);
+    ScanArgs<T, M> a = scan_args<T, M>(args, fwd_plan(args->L, args->B, args->C, args->N, args->G));
     if (a.p.nseg > 1) {
         const long long nh = (long long)a.p.nseg * a.B * a.p.np * a.C, ns = (long long)a.p.nseg * a.B * a.C;
         if (!args->workspace || args->workspace_floats < nh + ns) return GMT_ERR_WORKSPACE;
@@ -250,7 +265,7 @@ extern "C" int gmt_selective_scan_workspace(const gmt_scan_args* a, long long* c
 {
     if (int rc = scan_check(a)) return rc;
     GMT_CHECK_ARG(ck_floats && fwd_floats && bwd_floats);
-    const ScanPlan p = scan_plan(a->L, a->B, a->C, a->N, a->G);
+    const ScanPlan p = fwd_plan(a->L, a->B, a->C, a->N, a->G);
     *ck_floats = (long long)p.nck * a->B * p.np * a->C;
     *fwd_floats = p.nseg > 1 ? (long long)p.nseg * a->B * a->C * (p.np + 1) : 0;
     *bwd_floats = scan_bwd_floats(a);
