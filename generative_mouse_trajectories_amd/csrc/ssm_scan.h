@@ -21,7 +21,8 @@
 
 namespace gmt_ssm {
 
-constexpr int CH = 8;                    // steps per chunk = steps between kept states
+constexpr int BWD_WAVES = 8;              // waves a workgroup of the backward pass, at most
+constexpr int CH = 8;                    // steps per chunk; the state before every chunk is kept for the backward pass
 
 struct ScanPlan { int np, parts, waves, width, chans, cblk, nseg, seglen, nck; };   // chans: channels a workgroup; cblk: workgroups a group
 
@@ -47,7 +48,7 @@ static inline ScanPlan scan_plan(int L, int B, int C, int N, int G, int parts, i
     }
     p.seglen = (int)(((L + nseg - 1) / nseg + CH - 1) / CH * CH);
     p.nseg = (L + p.seglen - 1) / p.seglen;
-    p.nck = (L - 1) / CH;                // states kept before steps CH, 2 CH, ...
+    p.nck = (L + CH - 1) / CH;
     return p;
 }
 // One lane per channel costs the fewest instructions; two lanes fill the machine with half of the rows
@@ -56,7 +57,7 @@ static inline ScanPlan fwd_plan(int L, int B, int C, int N, int G)
     const ScanPlan p = scan_plan(L, B, C, N, G, 1, 4);
     return (long long)B * G * p.cblk * p.waves >= 4096 ? p : scan_plan(L, B, C, N, G, 2, 4);
 }
-static inline ScanPlan bwd_plan(int L, int B, int C, int N, int G) { return scan_plan(L, B, C, N, G, 2, 8); }
+static inline ScanPlan bwd_plan(int L, int B, int C, int N, int G) { return scan_plan(L, B, C, N, G, 2, BWD_WAVES); }
 
 static inline int scan_check(const gmt_scan_args* a)
 {
@@ -64,8 +65,10 @@ static inline int scan_check(const gmt_scan_args* a)
     GMT_CHECK_ARG(a->C % a->G == 0);
     GMT_CHECK_ARG((a->x_scale != nullptr) == (a->dt_scale != nullptr) && (a->z == nullptr || (a->x_scale != nullptr) == (a->z_scale != nullptr)));
     if (a->N > 32) return GMT_ERR_UNSUPPORTED;
-    // lane offsets are 32 bits: a step's pitch plus a channel, in elements
-    const long long lim = 1LL << 29;
+    // byte offsets within a pair of steps (B and C: a chunk) and within a row's kept states are 31 bits
+    const long long lim = 1LL << 28;
+    if ((long long)a->C * 128 >= 1LL << 31 || a->x_t < 0 || a->dt_t < 0 || a->z_t < 0 || a->dy_t < 0 ||
+        a->B_t < 0 || a->C_t < 0 || a->B_t >= lim / 4 || a->C_t >= lim / 4) return GMT_ERR_UNSUPPORTED;
     if (a->C >= lim || a->x_t >= lim || a->dt_t >= lim || a->z_t >= lim || a->dy_t >= lim || (long long)a->B * a->C >= lim) return GMT_ERR_UNSUPPORTED;
     for (const ScanPlan& p : {fwd_plan(a->L, a->B, a->C, a->N, a->G), bwd_plan(a->L, a->B, a->C, a->N, a->G)})
         if ((long long)p.cblk * a->G * a->B * p.nseg >= (1LL << 22)) return GMT_ERR_UNSUPPORTED;
@@ -109,68 +112,96 @@ __device__ __forceinline__ void step_fence() { asm volatile("" ::: "memory"); __
 // ... and v is computed before this point, what follows from it behind it (a sum is not put off with its terms in registers).
 __device__ __forceinline__ void pin(float& v) { asm volatile("" : "+v"(v)); }
 
+// The workgroup's LDS writes before it are seen behind it.  __syncthreads() would also wait for the stores of the chunk before.
+__device__ __forceinline__ void lds_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
 template <int CTRL> __device__ __forceinline__ float dpp(float v) {
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
 }
 constexpr int DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E, DPP_XOR7 = 0x141, DPP_XOR8 = 0x128;     // quad_perm, row_half_mirror, row_ror:8
 
-// ---- lanes of a channel.  With two, bit 3 of the lane says which: the other one is 8 lanes on within a row of 16, one DPP away.
+// (a, b) -> lanes 0 - 31: a summed over bit 5 of the lane, lanes 32 - 63: b
+__device__ __forceinline__ float half32(float a, float b) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// ---- lanes of a channel.  With two parts, the halves of the wave: 32 neighbouring channels each, whole memory sectors, and
+// one v_permlane32_swap spreads the values of two steps or gathers their sums.
 template <int PARTS> struct Lanes {
     static constexpr int OWN = CH / PARTS;              // a lane's own steps of a chunk: j * PARTS + part
     int part; unsigned chan;                            // chan: channel within the workgroup
     __device__ __forceinline__ Lanes() {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        part = PARTS == 1 ? 0 : lane >> 3 & 1;
-        chan = wave * (64 / PARTS) + (PARTS == 1 ? lane : (lane & 7) | (lane >> 4) << 3);
+        part = PARTS == 1 ? 0 : lane >> 5;
+        chan = wave * (64 / PARTS) + (PARTS == 1 ? lane : lane & 31);
     }
-    // own[j] of the lane that owns step s, on all lanes of the channel
-    __device__ __forceinline__ float of_step(const float (&own)[OWN], int s) const {
-        if constexpr (PARTS == 1) return own[s];
+    // a lane's value for its own step -> those of the PARTS neighbouring steps, on every lane of the channel
+    __device__ __forceinline__ void spread(float own, float (&v)[PARTS]) const {
+        if constexpr (PARTS == 1) v[0] = own;
         else {
-            const float o = dpp<DPP_XOR8>(own[s / 2]);
-            return part == (s & 1) ? own[s / 2] : o;
+            const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(own), __float_as_uint(own), false, false);
+            v[0] = __uint_as_float(r[0]);
+            v[1] = __uint_as_float(r[1]);
         }
     }
-    __device__ __forceinline__ float sum(float v) const { return PARTS == 1 ? v : v + dpp<DPP_XOR8>(v); }
-    __device__ __forceinline__ void keep(float (&own)[OWN], int s, float v) const {
-        if constexpr (PARTS == 1) own[s] = v; else own[s / 2] = part == (s & 1) ? v : own[s / 2];
+    // the lanes' terms for PARTS neighbouring steps -> the sum for a lane's own step
+    __device__ __forceinline__ float gather(const float (&v)[PARTS]) const {
+        if constexpr (PARTS == 1) return v[0]; else return half32(v[0], v[1]);
     }
+    __device__ __forceinline__ float sum(float v) const { if constexpr (PARTS == 1) return v; else return half32(v, v); }
 };
 
-// A lane's own elements of one sequence for one chunk.  full: all CH steps exist (uniform); else steps behind the end repeat the
-// last one and are masked by the caller.
+// A pointer that is the same on all lanes, kept in scalar registers: `uniform(p) + 32-bit offset` is then one memory instruction
+// (otherwise the compiler adds the lane's offset first, in 64-bit vector arithmetic, and keeps the results).
+template <class P> __device__ __forceinline__ P* uniform(P* p) { asm("" : "+s"(p)); return p; }
+
+// One sequence of a row, as a lane sees it.  Uniform base of a step plus a 32-bit byte offset of the lane (its part's step and its
+// channel): the scalar-base form of the memory instructions, no 64-bit vector arithmetic.
+template <class T> struct Seq {
+    const char* p; int pt; unsigned off, off0;          // (at step 0), pitch of a step in bytes; off0: of the first part
+    const char* sp; int spt; unsigned soff, soff0;      // exponents of an 8-bit checkpoint
+    __device__ __forceinline__ Seq(const void* base, const unsigned char* scale, long long t, long long b, int row, int part, unsigned c,
+                                   int rows, int channels) {
+        constexpr int E = __is_same(T, Q8) ? 1 : (int)sizeof(typename T::raw);
+        p = (const char*)base + row * b * E;
+        pt = (int)t * E;
+        off0 = c * E;
+        off = (unsigned)(part * pt) + off0;
+        const int n_sc = (channels + 31) / 32;
+        sp = (const char*)scale + (long long)row * n_sc;
+        spt = rows * n_sc;
+        soff0 = c / 32;
+        soff = (unsigned)(part * spt) + soff0;
+    }
+};
+// A lane's own elements for one chunk.  Steps behind the end repeat the last one and are masked by the caller.
 template <class T, int PARTS> struct Own {
     static constexpr int OWN = CH / PARTS;
     typename T::raw v[OWN];
-    __device__ __forceinline__ void request(const void* p, const unsigned char* scale, long long pt, int tc, int te, bool full, int part, unsigned c,
-                                            long long row_pitch, int b, int n_sc) {
-        // p: at (0, b, 0).  A step pair's base is uniform, the lane's part of the offset 32 bits.
-        if constexpr (__is_same(T, Q8)) {
-            const signed char* q = (const signed char*)p;
+    __device__ __forceinline__ void request(const Seq<T>& q, int tc, int te) {
 #pragma unroll
-            for (int j = 0; j < OWN; ++j) {
-                if (full) {
-                    const long long t = tc + j * PARTS;
-                    v[j].q = (q + t * pt)[(unsigned)(part * pt) + c];
-                    v[j].s = (scale + (t * row_pitch + b) * n_sc)[(unsigned)(part * row_pitch * n_sc) + c / 32];
-                } else {
-                    const long long t = min(tc + j * PARTS + part, te - 1);
-                    v[j].q = q[t * pt + c];
-                    v[j].s = scale[(t * row_pitch + b) * n_sc + c / 32];
-                }
-            }
-        } else {
-            const typename T::raw* q = (const typename T::raw*)p;
-#pragma unroll
-            for (int j = 0; j < OWN; ++j) {
-                if (full) v[j] = (q + (long long)(tc + j * PARTS) * pt)[(unsigned)(part * pt) + c];
-                else v[j] = q[(long long)min(tc + j * PARTS + part, te - 1) * pt + c];
-            }
+        for (int j = 0; j < OWN; ++j) {
+            const int t = min(tc + j * PARTS, te - 1);
+            const bool all = t + PARTS <= te;           // (uniform) every part's step exists
+            get(j, uniform(q.p + (long long)t * q.pt), all ? q.off : q.off0, __is_same(T, Q8) ? uniform(q.sp + (long long)t * q.spt) : nullptr,
+                all ? q.soff : q.soff0);
         }
     }
+    __device__ __forceinline__ void get(int j, const char* p, unsigned off, const char* sp, unsigned soff) {
+        if constexpr (__is_same(T, Q8)) {
+            v[j].q = *reinterpret_cast<const signed char*>(p + off);
+            v[j].s = *reinterpret_cast<const unsigned char*>(sp + soff);
+        } else v[j] = *reinterpret_cast<const typename T::raw*>(p + off);
+    }
 };
-template <class T> __device__ __forceinline__ const void* row_of(const void* p, long long offset) {
-    if constexpr (__is_same(T, Q8)) return (const signed char*)p + offset; else return (const typename T::raw*)p + offset;
+// the same for an output [L][B][C]
+template <class M> __device__ __forceinline__ void put_out(typename M::raw* base, long long uniform_elem, unsigned off_bytes, float v) {
+    *reinterpret_cast<typename M::raw*>(uniform(reinterpret_cast<char*>(base + uniform_elem)) + off_bytes) = from_f<M>(v);
 }
 
 // NS floats of a channel's row, states n0 .. n0 + NS - 1 (state buffers [B][C][N], A [C][N]) <-> registers, zero-padded
@@ -197,30 +228,32 @@ template <int NS> __device__ __forceinline__ void store_states(float* p, int n0,
         for (int n = 0; n < NS; ++n) if (n0 + n < N) p[n0 + n] = h[n];
     }
 }
-// The kept states and the segments' states: [..][B][NP][C], N padded to NP with zeros.
-template <int NP, int NS> __device__ __forceinline__ void load_kept(const float* p, long long slot, int B, int b, int C, unsigned c, int n0, float (&h)[NS])
+// The kept states (slot k: before step k CH) and the segments' states: [..][B][NP][C], N padded to NP with zeros.  off: (n0 C + c) * 4
+template <int NP, int NS> __device__ __forceinline__ void load_kept(const float* p, long long slot, int B, int b, int C, unsigned off, float (&h)[NS])
 {
-    const float* k = p + (slot * B + b) * NP * C + c + (long long)n0 * C;
+    const char* k = reinterpret_cast<const char*>(p + (slot * B + b) * NP * C);
 #pragma unroll
-    for (int n = 0; n < NS; ++n) h[n] = k[(long long)n * C];
+    for (int n = 0; n < NS; ++n) h[n] = *reinterpret_cast<const float*>(uniform(k + (long long)n * C * 4) + off);
 }
-template <int NP, int NS> __device__ __forceinline__ void store_kept(float* p, long long slot, int B, int b, int C, unsigned c, int n0, const float (&h)[NS])
+template <int NP, int NS> __device__ __forceinline__ void store_kept(float* p, long long slot, int B, int b, int C, unsigned off, const float (&h)[NS])
 {
-    float* k = p + (slot * B + b) * NP * C + c + (long long)n0 * C;
+    char* k = reinterpret_cast<char*>(p + (slot * B + b) * NP * C);
 #pragma unroll
-    for (int n = 0; n < NS; ++n) k[(long long)n * C] = h[n];
+    for (int n = 0; n < NS; ++n) *reinterpret_cast<float*>(uniform(k + (long long)n * C * 4) + off) = h[n];
 }
 
 // The chunk's B (or C) as fp32 [CH][NP] in LDS, by all threads of the workgroup: request() one chunk ahead, put() behind the wait.
 template <class M, int NP> struct MapTile {
     static constexpr int PER = CH * NP / 64;            // (one wave; wider workgroups need fewer)
     typename M::raw v[PER];
-    __device__ __forceinline__ void request(const typename M::raw* p, long long pt, int t0, int t1, int N) {
+    __device__ __forceinline__ void request(const typename M::raw* p, int pt, int t0, int t1, int N) {
+        const char* q = uniform(reinterpret_cast<const char*>(p + (long long)t0 * pt));
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
             const int i = threadIdx.x + j * blockDim.x, s = i / NP, n = i % NP;
             v[j] = from_f<M>(0.f);
-            if (s < CH && n < N && t0 + s < t1) v[j] = p[(t0 + s) * pt + n];
+            if (s < CH && n < N && t0 + s < t1)
+                v[j] = *reinterpret_cast<const typename M::raw*>(q + (unsigned)((s * pt + n) * (int)sizeof(typename M::raw)));
         }
     }
     __device__ __forceinline__ void put(float* lds) const {

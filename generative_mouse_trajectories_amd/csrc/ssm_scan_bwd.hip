@@ -8,7 +8,7 @@
 // operator at the values the checkpoints stand for).
 //
 // dB and dC are sums over lanes: 2 N values a step.  They leave by halving exchanges - a lane hands half of its values to its
-// partner and keeps the partner's other half, v_permlane32/16_swap then DPP - 34 instructions for 16 values over 32 lanes where 16
+// partner and keeps the partner's other half, v_permlane16_swap then DPP - 38 instructions for 16 values over 32 lanes where 16
 // separate sums take 80.  The waves of a workgroup meet in LDS, workgroups of one group through slabs: no float atomics, results
 // do not depend on the order of execution.
 #include "ssm_scan.h"
@@ -17,13 +17,9 @@ namespace {
 
 using namespace gmt_ssm;
 
-constexpr int PARTS = 2;                                // lanes per channel (ssm_scan.h): bit 3 of the lane
+constexpr int PARTS = 2;                                // lanes per channel (ssm_scan.h): the halves of the wave
 
-// (a, b) -> lanes with bit 5 (16 lanes: bit 4) clear: a summed over that bit, set: b
-__device__ __forceinline__ float half32(float a, float b) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
-    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
+// (a, b) -> lanes with bit 4 clear: a summed over that bit, set: b
 __device__ __forceinline__ float half16(float a, float b) {
     const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
@@ -32,31 +28,30 @@ template <int CTRL> __device__ __forceinline__ float half_dpp(float a, float b, 
     const float keep = upper ? b : a, send = upper ? a : b;
     return keep + dpp<CTRL>(send);
 }
-// v[0 .. NV) summed over the 32 lanes of one part: lane l returns value index_of(l)
+// v[0 .. NV) summed over the 32 lanes of one part: lane l returns value index_of(l).  (row_half_mirror also turns bits 0 and 1
+// round: all lanes that it mixes are summed later on.)
 template <int NV> __device__ __forceinline__ float part_sums(float (&v)[NV], int lane)
 {
     static_assert(NV == 8 || NV == 16 || NV == 32, "values per lane");
+    const bool b3 = lane & 8, b2 = lane & 4, b1 = lane & 2, b0 = lane & 1;
 #pragma unroll
-    for (int i = 0; i < NV / 2; ++i) v[i] = half32(v[i], v[i + NV / 2]);
+    for (int i = 0; i < NV / 2; ++i) v[i] = half16(v[i], v[i + NV / 2]);
 #pragma unroll
-    for (int i = 0; i < NV / 4; ++i) v[i] = half16(v[i], v[i + NV / 4]);
-    const bool b2 = lane & 4, b1 = lane & 2, b0 = lane & 1;
+    for (int i = 0; i < NV / 4; ++i) v[i] = half_dpp<DPP_XOR8>(v[i], v[i + NV / 4], b3);
 #pragma unroll
     for (int i = 0; i < NV / 8; ++i) v[i] = half_dpp<DPP_XOR7>(v[i], v[i + NV / 8], b2);
     if constexpr (NV >= 16) {
 #pragma unroll
         for (int i = 0; i < NV / 16; ++i) v[i] = half_dpp<DPP_XOR2>(v[i], v[i + NV / 16], b1);
     } else v[0] += dpp<DPP_XOR2>(v[0]);
-    return NV == 32 ? half_dpp<DPP_XOR1>(v[0], v[1], b0) : v[0] + dpp<DPP_XOR1>(v[0]);
+    if constexpr (NV == 32) return half_dpp<DPP_XOR1>(v[0], v[1], b0);
+    else return v[0] + dpp<DPP_XOR1>(v[0]);
 }
-template <int NV> __device__ __forceinline__ int index_of(int lane) {        // bits 5, 4, 2, 1, 0 of the lane, the first log2(NV) of them
-    const int i = lane >> 4 << 3 | (lane & 7);
-    return NV == 32 ? i : NV == 16 ? i >> 1 : i >> 2;
-}
+template <int NV> __device__ __forceinline__ int index_of(int lane) { return (lane & 31) >> (NV == 32 ? 0 : NV == 16 ? 1 : 2); }
 
 // a segment's adjoint: (adjoint of its incoming state for a zero adjoint behind it, S)
 template <class T, class M, int NP, bool GATED>
-__global__ __launch_bounds__(512)
+__global__ __launch_bounds__(64 * BWD_WAVES)
 void scan_bwd_local_kernel(ScanArgs<T, M> a)
 {
     constexpr int NS = NP / PARTS, OWN = CH / PARTS;
@@ -76,17 +71,16 @@ void scan_bwd_local_kernel(ScanArgs<T, M> a)
     for (int n = 0; n < NS; ++n) { A2[n] *= LOG2E; g[n] = 0.f; }
     const float bias = a.dt_bias ? a.dt_bias[c] : 0.f;
     const typename M::raw* Cp = a.Cm + b * a.C_b + gr * a.C_g;
-    const void *dp = row_of<T>(a.dt, b * a.dt_b), *zp = row_of<T>(a.z, b * a.z_b);
-    const int n_sc = (a.C + 31) / 32;
+    const Seq<T> dq(a.dt, a.dts, a.dt_t, a.dt_b, b, ln.part, c, a.B, a.C), zq(a.z, a.zs, a.z_t, a.z_b, b, ln.part, c, a.B, a.C);
+    const Seq<M> yq(a.dy, nullptr, a.dy_t, a.dy_b, b, ln.part, c, a.B, a.C);
     float S = 0.f;
     Own<T, PARTS> dr, zr;
     Own<M, PARTS> yr;
     MapTile<M, NP> mC;
     auto request = [&](int tc) {
-        const bool full = tc + CH <= te;
-        dr.request(dp, a.dts, a.dt_t, tc, te, full, ln.part, c, a.B, b, n_sc);
-        if (GATED) zr.request(zp, a.zs, a.z_t, tc, te, full, ln.part, c, a.B, b, n_sc);
-        yr.request(a.dy + b * a.dy_b, nullptr, a.dy_t, tc, te, full, ln.part, c, a.B, b, n_sc);
+        dr.request(dq, tc, te);
+        if (GATED) zr.request(zq, tc, te);
+        yr.request(yq, tc, te);
         mC.request(Cp, a.C_t, tc, te, a.N);
     };
     int buf = 0, k = te > t0 ? (te - t0 + CH - 1) / CH - 1 : -1;
@@ -105,32 +99,36 @@ void scan_bwd_local_kernel(ScanArgs<T, M> a)
             S += st[j];
         }
         mC.put(sC[buf]);
-        __syncthreads();
+        lds_barrier();
         if (k > 0) request(tc - CH);
+        float sts[PARTS], ds[PARTS];
 #pragma unroll
         for (int s = CH - 1; s >= 0; --s) {
-            float sts = ln.of_step(st, s);
-            const float ds = ln.of_step(d, s);
-            pin(sts);
+            const int j = s / PARTS, q = s % PARTS;
+            if (q == PARTS - 1) { ln.spread(st[j], sts); ln.spread(d[j], ds); }
+            pin(sts[q]);
 #pragma unroll
-            for (int n = 0; n < NS; ++n) g[n] = __builtin_amdgcn_exp2f(sts * A2[n]) * fmaf(ds, sC[buf][s * NP + n0 + n], g[n]);
+            for (int n = 0; n < NS; ++n) g[n] = __builtin_amdgcn_exp2f(sts[q] * A2[n]) * fmaf(ds[q], sC[buf][s * NP + n0 + n], g[n]);
             step_fence();
         }
     }
     S = ln.sum(S);
     if (!on) return;
-    store_kept<NP, NS>(a.seg_h, seg, a.B, b, a.C, c, n0, g);
+    store_kept<NP, NS>(a.seg_h, seg, a.B, b, a.C, (unsigned)(n0 * a.C + c) * 4, g);
     if (ln.part == 0) a.seg_s[(long long)(seg * a.B + b) * a.C + c] = S;
 }
 
 template <class T, class M, int NP, bool GATED>
-__global__ __launch_bounds__(512, 2)
+__global__ __launch_bounds__(64 * BWD_WAVES, 2)
 void scan_bwd_kernel(ScanArgs<T, M> a)
 {
     constexpr int NS = NP / PARTS, OWN = CH / PARTS;
-    constexpr bool KEEP_E = NP <= 16;                   // the exponentials of a chunk stay in registers (N = 32: computed twice)
+    // The exponentials of the last KE steps of a chunk stay in registers, those of the others are computed twice: as many as fit
+    // beside the states (N = 16, L=256 B=256 C=512 bf16: 8 kept 499 us, 4 kept 518 us, none 538 us; from 8-bit codes, whose
+    // exponents take registers too, L=129: 506, 390, 399 us).
+    constexpr int KE = NP == 8 ? CH : NP == 32 ? 0 : __is_same(T, Q8) ? CH / 2 : CH;
     __shared__ __align__(16) float sB[2][CH * NP], sC[2][CH * NP];
-    __shared__ float red[2][8][CH][2 * NP];             // [wave][step][part][dB, dC of the part's states]
+    __shared__ float red[2][BWD_WAVES][CH][2 * NP];             // [wave][step][part][dB, dC of the part's states]
     const int cb = blockIdx.x % a.p.cblk, rest = blockIdx.x / a.p.cblk;
     const int gr = rest % a.G, slab = rest / a.G;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -144,7 +142,7 @@ void scan_bwd_kernel(ScanArgs<T, M> a)
     for (int n = 0; n < NS; ++n) { A2[n] *= LOG2E; dA[n] = 0.f; }
     const float bias = a.dt_bias ? a.dt_bias[c] : 0.f, Dc = a.D ? a.D[c] : 0.f;
     const long long tbg = (long long)a.L * a.B * a.G * a.N;
-    const int n_sc = (a.C + 31) / 32;
+    const unsigned koff = (unsigned)(n0 * a.C + c) * 4, ooff = (unsigned)((ln.part * a.B * a.C + c) * sizeof(typename M::raw));
 
     auto put_bc = [&](int t, int b, bool is_c, int n, float v) {
         const long long at = (((long long)t * a.B + b) * a.G + gr) * a.N + n;
@@ -170,12 +168,14 @@ void scan_bwd_kernel(ScanArgs<T, M> a)
         const long long row = (long long)b * a.C + c;
         const typename M::raw* Bp = a.Bm + b * a.B_b + gr * a.B_g;
         const typename M::raw* Cp = a.Cm + b * a.C_b + gr * a.C_g;
-        const void *xp = row_of<T>(a.x, b * a.x_b), *dp = row_of<T>(a.dt, b * a.dt_b), *zp = row_of<T>(a.z, b * a.z_b);
+        const Seq<T> xq(a.x, a.xs, a.x_t, a.x_b, b, ln.part, c, a.B, a.C), dq(a.dt, a.dts, a.dt_t, a.dt_b, b, ln.part, c, a.B, a.C),
+            zq(a.z, a.zs, a.z_t, a.z_b, b, ln.part, c, a.B, a.C);
+        const Seq<M> yq(a.dy, nullptr, a.dy_t, a.dy_b, b, ln.part, c, a.B, a.C);
         float gc[NS];                                   // exp(step[t+1] A) g[t+1]
 #pragma unroll
         for (int n = 0; n < NS; ++n) gc[n] = 0.f;
         if (on) {
-            if (a.p.nseg > 1) load_kept<NP, NS>(a.seg_h, seg, a.B, b, a.C, c, n0, gc);
+            if (a.p.nseg > 1) load_kept<NP, NS>(a.seg_h, seg, a.B, b, a.C, koff, gc);
             else if (a.dstate_out) load_states<NS>(a.dstate_out + row * a.N, n0, a.N, gc);
         }
         Own<T, PARTS> xr, dr, zr;
@@ -183,25 +183,19 @@ void scan_bwd_kernel(ScanArgs<T, M> a)
         MapTile<M, NP> mB, mC;
         float hk[NS];
         auto request = [&](int tc) {
-            const bool full = tc + CH <= te;
-            xr.request(xp, a.xs, a.x_t, tc, te, full, ln.part, c, a.B, b, n_sc);
-            dr.request(dp, a.dts, a.dt_t, tc, te, full, ln.part, c, a.B, b, n_sc);
-            if (GATED) zr.request(zp, a.zs, a.z_t, tc, te, full, ln.part, c, a.B, b, n_sc);
-            yr.request(a.dy + b * a.dy_b, nullptr, a.dy_t, tc, te, full, ln.part, c, a.B, b, n_sc);
+            xr.request(xq, tc, te);
+            dr.request(dq, tc, te);
+            if (GATED) zr.request(zq, tc, te);
+            yr.request(yq, tc, te);
             mB.request(Bp, a.B_t, tc, te, a.N);
             mC.request(Cp, a.C_t, tc, te, a.N);
-            if (tc > 0) load_kept<NP, NS>(a.ck, tc / CH - 1, a.B, b, a.C, c, n0, hk);
-            else if (a.state) load_states<NS>(a.state + row * a.N, n0, a.N, hk);
-            else {
-#pragma unroll
-                for (int n = 0; n < NS; ++n) hk[n] = 0.f;
-            }
+            load_kept<NP, NS>(a.ck, tc / CH, a.B, b, a.C, koff, hk);
         };
         int k = te > t0 ? (te - t0 + CH - 1) / CH - 1 : -1;
         if (k >= 0) request(t0 + k * CH);
         for (; k >= 0; --k) {
             const int tc = t0 + k * CH;
-            float h[CH + 1][NS], ex[KEEP_E ? CH : 1][NS];
+            float h[CH + 1][NS], ex[KE ? KE : 1][NS];
             float xv[OWN], st[OWN], sig[OWN], d[OWN], dyv[OWN], zv[OWN], out[OWN], gBk[OWN], qAk[OWN];
 #pragma unroll
             for (int j = 0; j < OWN; ++j) {
@@ -218,24 +212,29 @@ void scan_bwd_kernel(ScanArgs<T, M> a)
             for (int n = 0; n < NS; ++n) h[0][n] = hk[n];
             mB.put(sB[buf]);
             mC.put(sC[buf]);
-            __syncthreads();
+            lds_barrier();
             flush();                                    // the sums of the chunk before, written before the barrier
             if (wave_on) {
+                float sts[PARTS], xs[PARTS], ds[PARTS], va[PARTS], vb[PARTS];
 #pragma unroll
                 for (int s = 0; s < CH; ++s) {
-                    float sts = ln.of_step(st, s);
-                    const float sxs = sts * ln.of_step(xv, s);
-                    pin(sts);
+                    const int j = s / PARTS, q = s % PARTS;
+                    if (q == 0) { ln.spread(st[j], sts); ln.spread(xv[j], xs); }
+                    pin(sts[q]);
+                    const float sx = sts[q] * xs[q];
                     const float *Bt = sB[buf] + s * NP + n0, *Ct = sC[buf] + s * NP + n0;
-                    float o = 0.f;
+                    va[q] = 0.f;
 #pragma unroll
                     for (int n = 0; n < NS; ++n) {
-                        const float e = __builtin_amdgcn_exp2f(sts * A2[n]);
-                        if (KEEP_E) ex[KEEP_E ? s : 0][n] = e;
-                        h[s + 1][n] = fmaf(e, h[s][n], sxs * Bt[n]);
-                        if (GATED) o = fmaf(h[s + 1][n], Ct[n], o);
+                        const float e = __builtin_amdgcn_exp2f(sts[q] * A2[n]);
+                        if (s >= CH - KE) ex[s >= CH - KE ? s - (CH - KE) : 0][n] = e;
+                        h[s + 1][n] = fmaf(e, h[s][n], sx * Bt[n]);
+                        if (GATED) va[q] = fmaf(h[s + 1][n], Ct[n], va[q]);
                     }
-                    if (GATED) { o = ln.sum(o); pin(o); ln.keep(out, s, o); }
+                    if (GATED) {
+                        pin(va[q]);
+                        if (q == PARTS - 1) out[j] = ln.gather(va);
+                    }
                     step_fence();
                 }
                 if (GATED) {
@@ -243,8 +242,8 @@ void scan_bwd_kernel(ScanArgs<T, M> a)
                     for (int j = 0; j < OWN; ++j) {
                         const float sz = sigmoid(zv[j]);
                         if (tc + j * PARTS + ln.part < t1 && on)
-                            (a.dz + ((long long)(tc + j * PARTS) * a.B + b) * a.C)[(unsigned)(ln.part * a.B * a.C) + c] =
-                                from_f<M>(dyv[j] * fmaf(Dc, xv[j], out[j]) * sz * fmaf(zv[j], 1.0f - sz, 1.0f));
+                            put_out<M>(a.dz, ((long long)(tc + j * PARTS) * a.B + b) * a.C, ooff,
+                                       dyv[j] * fmaf(Dc, xv[j], out[j]) * sz * fmaf(zv[j], 1.0f - sz, 1.0f));
                     }
                     step_fence();
                 }
@@ -252,29 +251,29 @@ void scan_bwd_kernel(ScanArgs<T, M> a)
                 for (int s = CH - 1; s >= 0; --s) {
                     // the next chunk's elements: by now half of h and ex is free again
                     if (s == CH / 2 - 1 && k > 0) request(tc - CH);
-                    float sts = ln.of_step(st, s);
-                    const float sxs = sts * ln.of_step(xv, s), ds = ln.of_step(d, s);
-                    pin(sts);
+                    const int j = s / PARTS, q = s % PARTS;
+                    if (q == PARTS - 1) { ln.spread(st[j], sts); ln.spread(xv[j], xs); ln.spread(d[j], ds); }
+                    pin(sts[q]);
+                    const float sx = sts[q] * xs[q];
                     const float *Bt = sB[buf] + s * NP + n0, *Ct = sC[buf] + s * NP + n0;
-                    float gB = 0.f, qA = 0.f, v[2 * NS];
+                    float v[2 * NS];
+                    va[q] = vb[q] = 0.f;
 #pragma unroll
                     for (int n = 0; n < NS; ++n) {
-                        const float e = KEEP_E ? ex[KEEP_E ? s : 0][n] : __builtin_amdgcn_exp2f(sts * A2[n]);
-                        const float gn = fmaf(ds, Ct[n], gc[n]);
-                        v[n] = gn * sxs;
-                        v[NS + n] = h[s + 1][n] * ds;
-                        gB = fmaf(gn, Bt[n], gB);
+                        const float e = s >= CH - KE ? ex[s >= CH - KE ? s - (CH - KE) : 0][n] : __builtin_amdgcn_exp2f(sts[q] * A2[n]);
+                        const float gn = fmaf(ds[q], Ct[n], gc[n]);
+                        v[n] = gn * sx;
+                        v[NS + n] = h[s + 1][n] * ds[q];
+                        va[q] = fmaf(gn, Bt[n], va[q]);
                         gc[n] = gn * e;
-                        const float q = gc[n] * h[s][n];
-                        qA = fmaf(q, A2[n], qA);
-                        dA[n] = fmaf(q, sts, dA[n]);
+                        const float p = gc[n] * h[s][n];
+                        vb[q] = fmaf(p, A2[n], vb[q]);
+                        dA[n] = fmaf(p, sts[q], dA[n]);
                     }
-                    gB = ln.sum(gB); qA = ln.sum(qA);
-                    pin(gB); pin(qA);
+                    pin(va[q]); pin(vb[q]);
 #pragma unroll
                     for (int n = 0; n < NS; ++n) pin(dA[n]);
-                    ln.keep(gBk, s, gB);
-                    ln.keep(qAk, s, qA);
+                    if (q == 0) { gBk[j] = ln.gather(va); qAk[j] = ln.gather(vb); }
                     red[buf][wave][s][ln.part * 2 * NS + index_of<2 * NS>(lane)] = part_sums<2 * NS>(v, lane);
                     step_fence();
                 }
@@ -286,9 +285,8 @@ void scan_bwd_kernel(ScanArgs<T, M> a)
                     dD = fmaf(d[j], xv[j], dD);
                     if (t < t1 && on) {
                         const long long base = ((long long)(tc + j * PARTS) * a.B + b) * a.C;
-                        const unsigned at = (unsigned)(ln.part * a.B * a.C) + c;
-                        (a.dx + base)[at] = from_f<M>(fmaf(gBk[j], st[j], Dc * d[j]));
-                        (a.ddt + base)[at] = from_f<M>(dstep);
+                        put_out<M>(a.dx, base, ooff, fmaf(gBk[j], st[j], Dc * d[j]));
+                        put_out<M>(a.ddt, base, ooff, dstep);
                     }
                 }
             } else {
@@ -313,7 +311,7 @@ void scan_bwd_kernel(ScanArgs<T, M> a)
         for (int i = threadIdx.x; i < (t1 - z0) * 2 * NP; i += a.p.width)
             if (i % NP < a.N) put_bc(z0 + i / (2 * NP), b, i % (2 * NP) >= NP, i % NP, 0.f);
     }
-    __syncthreads();
+    lds_barrier();
     flush();
     dD = ln.sum(dD);
     dbias = ln.sum(dbias);
@@ -404,10 +402,10 @@ extern "C" int gmt_selective_scan_bwd(const gmt_scan_args* a, hipStream_t stream
 {
     if (int rc = scan_check(a)) return rc;
     GMT_CHECK_ARG(a->dy && a->dx && a->ddt && a->dB && a->dC && a->dparam && a->workspace && (!a->z || a->dz));
-    GMT_CHECK_ARG(a->ck || a->L <= CH);
+    GMT_CHECK_ARG(a->ck);
     GMT_CHECK_ARG((long long)a->B * bwd_plan(a->L, a->B, a->C, a->N, a->G).nseg < (1LL << 31));
     if (a->x_scale) {
-        if (a->L > CH) { if (int rc = scan_states_q8(a, stream)) return rc; }
+        if (int rc = scan_states_q8(a, stream)) return rc;
         return a->bf16 ? run<Q8, B16>(a, stream) : run<Q8, F32>(a, stream);
     }
     return a->bf16 ? run<B16, B16>(a, stream) : run<F32, F32>(a, stream);

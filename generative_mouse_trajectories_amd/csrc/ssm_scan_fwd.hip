@@ -31,23 +31,23 @@ void scan_fwd_kernel(ScanArgs<T, M> a)
 #pragma unroll
     for (int n = 0; n < NS; ++n) { A2[n] *= LOG2E; h[n] = 0.f; }
     const long long row = (long long)b * a.C + c;
+    const unsigned koff = (unsigned)(n0 * a.C + c) * 4, yoff = (unsigned)((ln.part * a.B * a.C + c) * sizeof(typename M::raw));
     if (MODE != LOCAL) {
-        if (a.p.nseg > 1) load_kept<NP, NS>(a.seg_h, seg, a.B, b, a.C, c, n0, h);
+        if (a.p.nseg > 1) load_kept<NP, NS>(a.seg_h, seg, a.B, b, a.C, koff, h);
         else if (a.state) load_states<NS>(a.state + row * a.N, n0, a.N, h);
     }
     const float bias = a.dt_bias ? a.dt_bias[c] : 0.f, Dc = Y && a.D ? a.D[c] : 0.f;
     const typename M::raw* Bp = a.Bm + b * a.B_b + g * a.B_g;
     const typename M::raw* Cp = a.Cm + b * a.C_b + g * a.C_g;
-    const void *xp = row_of<T>(a.x, b * a.x_b), *dp = row_of<T>(a.dt, b * a.dt_b), *zp = row_of<T>(a.z, b * a.z_b);
-    const int n_sc = (a.C + 31) / 32;
+    const Seq<T> xq(a.x, a.xs, a.x_t, a.x_b, b, ln.part, c, a.B, a.C), dq(a.dt, a.dts, a.dt_t, a.dt_b, b, ln.part, c, a.B, a.C),
+        zq(a.z, a.zs, a.z_t, a.z_b, b, ln.part, c, a.B, a.C);
 
     Own<T, PARTS> xr, dr, zr;
     MapTile<M, NP> mB, mC;
     auto request = [&](int tc) {
-        const bool full = tc + CH <= te;
-        xr.request(xp, a.xs, a.x_t, tc, te, full, ln.part, c, a.B, b, n_sc);
-        dr.request(dp, a.dts, a.dt_t, tc, te, full, ln.part, c, a.B, b, n_sc);
-        if (GATED) zr.request(zp, a.zs, a.z_t, tc, te, full, ln.part, c, a.B, b, n_sc);
+        xr.request(xq, tc, te);
+        dr.request(dq, tc, te);
+        if (GATED) zr.request(zq, tc, te);
         mB.request(Bp, a.B_t, tc, te, a.N);
         if (Y) mC.request(Cp, a.C_t, tc, te, a.N);
     };
@@ -59,9 +59,9 @@ void scan_fwd_kernel(ScanArgs<T, M> a)
         mB.put(sB[buf]);
         if (Y) mC.put(sC[Y ? buf : 0]);
         // one barrier a chunk: a buffer is written again two chunks later, behind the next barrier, which its readers have passed
-        __syncthreads();
+        lds_barrier();
         if (tc + CH < te) request(tc + CH);
-        if (KEEP && tc > 0 && wave_on) store_kept<NP, NS>(a.ck, tc / CH - 1, a.B, b, a.C, c, n0, h);
+        if (KEEP && wave_on) store_kept<NP, NS>(a.ck, tc / CH, a.B, b, a.C, koff, h);
         if (MODE == STATES && tc + CH >= te) break;     // nothing is kept behind the last chunk
         if (wave_on) {
             float xv[OWN], st[OWN];                     // st: the step, then (its step done) the sum over the states
@@ -74,21 +74,27 @@ void scan_fwd_kernel(ScanArgs<T, M> a)
                 st[j] = live ? st[j] : 0.f;
                 if (MODE == LOCAL) S += st[j];
             }
+            float sts[PARTS], xs[PARTS], ys[PARTS];
 #pragma unroll
             for (int s = 0; s < CH; ++s) {
-                float sts = ln.of_step(st, s);
-                const float sxs = sts * ln.of_step(xv, s);
-                pin(sts);
+                const int j = s / PARTS, k = s % PARTS;
+                if (k == 0) { ln.spread(st[j], sts); ln.spread(xv[j], xs); }
+                pin(sts[k]);
+                const float sx = sts[k] * xs[k];
                 float y0 = 0.f, y1 = 0.f;
                 const float* Bt = sB[buf] + s * NP + n0;
                 const float* Ct = sC[Y ? buf : 0] + (Y ? s * NP + n0 : 0);
 #pragma unroll
                 for (int n = 0; n < NS; ++n) {
-                    const float e = __builtin_amdgcn_exp2f(sts * A2[n]);
-                    h[n] = fmaf(e, h[n], sxs * Bt[n]);
+                    const float e = __builtin_amdgcn_exp2f(sts[k] * A2[n]);
+                    h[n] = fmaf(e, h[n], sx * Bt[n]);
                     if (Y) { if (n & 1) y1 = fmaf(h[n], Ct[n], y1); else y0 = fmaf(h[n], Ct[n], y0); }
                 }
-                if (Y) { float y = ln.sum(y0 + y1); pin(y); ln.keep(st, s, y); }
+                if (Y) {
+                    ys[k] = y0 + y1;
+                    pin(ys[k]);
+                    if (k == PARTS - 1) st[j] = ln.gather(ys);
+                }
                 step_fence();
             }
             if (Y) {
@@ -97,15 +103,14 @@ void scan_fwd_kernel(ScanArgs<T, M> a)
                     const int t = tc + j * PARTS + ln.part;
                     float o = fmaf(Dc, xv[j], st[j]);
                     if (GATED) { const float zv = to_f(zc.v[j]); o *= zv * sigmoid(zv); }
-                    typename M::raw* yp = a.y + ((long long)(tc + j * PARTS) * a.B + b) * a.C;
-                    if (t < t1) yp[(unsigned)(ln.part * a.B * a.C) + c] = from_f<M>(t < te ? o : 0.f);
+                    if (t < t1) put_out<M>(a.y, ((long long)(tc + j * PARTS) * a.B + b) * a.C, yoff, t < te ? o : 0.f);
                 }
             }
         }
     }
     if (!on) return;
     if (MODE == LOCAL) {
-        store_kept<NP, NS>(a.seg_h, seg, a.B, b, a.C, c, n0, h);
+        store_kept<NP, NS>(a.seg_h, seg, a.B, b, a.C, koff, h);
         S = ln.sum(S);
         if (ln.part == 0) a.seg_s[(long long)(seg * a.B + b) * a.C + c] = S;
         return;
@@ -117,23 +122,33 @@ void scan_fwd_kernel(ScanArgs<T, M> a)
 }
 
 // seg_h: (h_loc of every segment) -> (its incoming state), in place.  A thread is one state of one channel and row.
-__global__ __launch_bounds__(256)
+__global__ __launch_bounds__(64)
 void scan_chain_kernel(float* __restrict__ seg_h, const float* __restrict__ seg_s, const float* __restrict__ A, const float* __restrict__ first,
                        int nseg, int np, int B, int C, int N, int reverse)
 {
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x, n_all = (long long)B * np * C;
+    const long long i = (long long)blockIdx.x * 64 + threadIdx.x, n_all = (long long)B * np * C;
     if (i >= n_all) return;
     const int c = (int)(i % C), n = (int)(i / C % np);
     const long long b = i / C / np;
     if (n >= N) return;                                 // (padding: zeros in every segment)
     const float A2 = A[(long long)c * N + n] * LOG2E;
     float h = first ? first[(b * C + c) * N + n] : 0.f;
-    for (int k = 0; k < nseg; ++k) {
-        const int s = reverse ? nseg - 1 - k : k;
-        const long long at = s * n_all + i;
-        const float loc = seg_h[at], S = seg_s[((long long)s * B + b) * C + c];
-        seg_h[at] = h;
-        h = fmaf(__builtin_amdgcn_exp2f(A2 * S), h, loc);
+    constexpr int AHEAD = 16;                           // segments requested at once: one round trip to memory for 16 links
+    for (int k0 = 0; k0 < nseg; k0 += AHEAD) {
+        float loc[AHEAD], S[AHEAD];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            const int k = min(k0 + j, nseg - 1), s = reverse ? nseg - 1 - k : k;
+            loc[j] = seg_h[s * n_all + i];
+            S[j] = seg_s[((long long)s * B + b) * C + c];
+        }
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            if (k0 + j >= nseg) break;
+            const int s = reverse ? nseg - 1 - (k0 + j) : k0 + j;
+            seg_h[s * n_all + i] = h;
+            h = fmaf(__builtin_amdgcn_exp2f(A2 * S[j]), h, loc[j]);
+        }
     }
 }
 
@@ -249,7 +264,7 @@ int scan_chain(float* seg_h, const float* seg_s, const float* A, const float* fi
                int reverse, hipStream_t stream)
 {
     const long long n = (long long)B * np * C;
-    hipLaunchKernelGGL(scan_chain_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, seg_h, seg_s, A, first, nseg, np, B, C,
+    hipLaunchKernelGGL(scan_chain_kernel, dim3((unsigned)((n + 63) / 64)), dim3(64), 0, stream, seg_h, seg_s, A, first, nseg, np, B, C,
                        N, reverse);
     GMT_LAUNCH_CHECK();
     return GMT_OK;
