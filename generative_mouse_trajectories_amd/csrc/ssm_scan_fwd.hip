@@ -123,7 +123,7 @@ void scan_fwd_kernel(ScanArgs<T, M> a)
 
 // seg_h: (h_loc of every segment) -> (its incoming state), in place.  A thread is one state of one channel and row.
 __global__ __launch_bounds__(64)
-void scan_chain_kernel(float* __restrict__ seg_h, const float* __restrict__ seg_s, const float* __restrict__ A, const float* __restrict__ first,
+void scan_chain_kernel(float* seg_h, const float* __restrict__ seg_s, const float* __restrict__ A, const float* __restrict__ first,
                        int nseg, int np, int B, int C, int N, int reverse)
 {
     const long long i = (long long)blockIdx.x * 64 + threadIdx.x, n_all = (long long)B * np * C;
@@ -133,70 +133,119 @@ void scan_chain_kernel(float* __restrict__ seg_h, const float* __restrict__ seg_
     if (n >= N) return;                                 // (padding: zeros in every segment)
     const float A2 = A[(long long)c * N + n] * LOG2E;
     float h = first ? first[(b * C + c) * N + n] : 0.f;
-    constexpr int AHEAD = 16;                           // segments requested at once: one round trip to memory for 16 links
-    for (int k0 = 0; k0 < nseg; k0 += AHEAD) {
-        float loc[AHEAD], S[AHEAD];
+    // AHEAD links are requested while the AHEAD before them are chained and stored: one round trip to memory for all of them
+    constexpr int AHEAD = 16;
+    float loc[2][AHEAD], S[2][AHEAD];
+    auto request = [&](int k0, float (&l)[AHEAD], float (&sums)[AHEAD]) {
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) {
             const int k = min(k0 + j, nseg - 1), s = reverse ? nseg - 1 - k : k;
-            loc[j] = seg_h[s * n_all + i];
-            S[j] = seg_s[((long long)s * B + b) * C + c];
+            l[j] = seg_h[s * n_all + i];
+            sums[j] = seg_s[((long long)s * B + b) * C + c];
         }
+    };
+    auto chain = [&](int k0, const float (&l)[AHEAD], const float (&sums)[AHEAD]) {
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) {
             if (k0 + j >= nseg) break;
             const int s = reverse ? nseg - 1 - (k0 + j) : k0 + j;
             seg_h[s * n_all + i] = h;
-            h = fmaf(__builtin_amdgcn_exp2f(A2 * S[j]), h, loc[j]);
+            h = fmaf(__builtin_amdgcn_exp2f(A2 * sums[j]), h, l[j]);
         }
+    };
+    request(0, loc[0], S[0]);
+    for (int k0 = 0; k0 < nseg; k0 += 2 * AHEAD) {
+        if (k0 + AHEAD < nseg) request(k0 + AHEAD, loc[1], S[1]);
+        chain(k0, loc[0], S[0]);
+        if (k0 + 2 * AHEAD < nseg) request(k0 + 2 * AHEAD, loc[0], S[0]);
+        chain(k0 + AHEAD, loc[1], S[1]);
     }
 }
 
-// One step of every row: state [B][C][N] -> state_out (may be the same buffer).  LPC lanes hold a channel, V = 4 or 1 states
-// each: whole lines of the state, which is all of the traffic, and a sum over LPC neighbouring lanes.
-template <class M, int V, int LPC>
+// One step of every row: state [B][C][N] -> state_out (may be the same buffer).  The state, read and written once, is all of the
+// traffic: LPC lanes hold a channel, V = 4 or 1 states each, whole lines of it, and a sum over LPC neighbouring lanes.  A workgroup
+// keeps the parameters of its 256 / LPC channels in registers and walks down the rows, ROWS at a time, so that as many
+// lines are in flight from each lane.
+template <class M, int V> __device__ __forceinline__ void load_map(const typename M::raw* p, bool wide, int n0, int N, float (&o)[V])
+{
+    if constexpr (V == 4) {
+        if (wide) {                                     // (uniform) 4 elements at once
+            typedef typename M::raw vec __attribute__((ext_vector_type(4)));
+            const vec v = *reinterpret_cast<const vec*>(p + n0);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[k] = to_f((typename M::raw)v[k]);
+            return;
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < V; ++k) o[k] = to_f(p[n0 + k]);
+}
+
+template <class M, int V, int LPC, int ROWS>
 __global__ __launch_bounds__(256)
 void scan_step_kernel(const typename M::raw* __restrict__ x, long long x_b, const typename M::raw* __restrict__ dt, long long dt_b,
                       const typename M::raw* __restrict__ z, long long z_b, const typename M::raw* __restrict__ Bm, long long B_b,
                       long long B_g, const typename M::raw* __restrict__ Cm, long long C_b, long long C_g, const float* __restrict__ A,
                       const float* __restrict__ D, const float* __restrict__ dt_bias, const float* state, float* state_out,
-                      const unsigned char* __restrict__ active, typename M::raw* __restrict__ y, int B, int C, int N, int G)
+                      const unsigned char* __restrict__ active, typename M::raw* __restrict__ y, int B, int C, int N, int G, int gx, int wide)
 {
-    const int part = threadIdx.x % LPC, n0 = part * V;
-    const long long n_ch = (long long)B * C, step = (long long)gridDim.x * (256 / LPC);
-    const int cg = C / G;
-    for (long long i = (long long)blockIdx.x * (256 / LPC) + threadIdx.x / LPC; i < n_ch; i += step) {
-        const int b = (int)(i / C), c = (int)(i % C), g = c / cg;
-        const bool act = !active || active[b], has = n0 < N;
-        float hv[V] = {};
-        if (has) {
-            if constexpr (V == 4) *reinterpret_cast<float4*>(hv) = *reinterpret_cast<const float4*>(state + i * N + n0);
-            else hv[0] = state[i * N + n0];
-        }
-        float yv = 0.f;
-        if (act) {                                      // (an inactive row's state stays as it is)
-            const float xv = to_f(x[b * x_b + c]);
-            float sig;
-            const float st = softplus(to_f(dt[b * dt_b + c]) + (dt_bias ? dt_bias[c] : 0.f), sig);
-            const float sx = st * xv;
+    constexpr int CHANS = 256 / LPC;
+    const int part = threadIdx.x % LPC, ci = blockIdx.x % gx * CHANS + threadIdx.x / LPC;
+    const bool on = ci < C;
+    const int c = on ? ci : C - 1, g = c / (C / G);
+    // lanes beyond the states or the channels repeat the last ones, add nothing and store nothing
+    const bool has = part * V < N;
+    const int n0 = has ? part * V : N - V;
+    float A2[V];
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                if (has) {
-                    const int n = n0 + v;
-                    hv[v] = fmaf(__builtin_amdgcn_exp2f(st * (A[(long long)c * N + n] * LOG2E)), hv[v], sx * to_f(Bm[b * B_b + g * B_g + n]));
-                    yv = fmaf(hv[v], to_f(Cm[b * C_b + g * C_g + n]), yv);
+    for (int v = 0; v < V; ++v) A2[v] = A[(long long)c * N + n0 + v] * LOG2E;
+    const float bias = dt_bias ? dt_bias[c] : 0.f, Dc = D ? D[c] : 0.f;
+    const long long at0 = (long long)c * N + n0, pitch = (long long)C * N;
+    const int groups = gridDim.x / gx;
+    for (int b0 = blockIdx.x / gx * ROWS; b0 < B; b0 += groups * ROWS) {
+        float h[ROWS][V], Bv[ROWS][V], Cv[ROWS][V];
+        typename M::raw xr[ROWS], dr[ROWS], zr[ROWS];
+        bool act[ROWS];
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            const int b = min(b0 + r, B - 1);
+            const float* sp = state + b * pitch + at0;
+            if constexpr (V == 4) *reinterpret_cast<float4*>(h[r]) = *reinterpret_cast<const float4*>(sp);
+            else h[r][0] = *sp;
+            xr[r] = x[b * x_b + c];
+            dr[r] = dt[b * dt_b + c];
+            zr[r] = z ? z[b * z_b + c] : from_f<M>(0.f);
+            load_map<M, V>(Bm + b * B_b + g * B_g, wide, n0, N, Bv[r]);
+            load_map<M, V>(Cm + b * C_b + g * C_g, wide, n0, N, Cv[r]);
+            act[r] = !active || active[b];
+        }
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            const int b = b0 + r;
+            if (b >= B) break;
+            float yv = 0.f;
+            if (act[r]) {                               // (an inactive row's state stays as it is)
+                const float xv = to_f(xr[r]);
+                float sig;
+                const float st = softplus(to_f(dr[r]) + bias, sig), sx = st * xv;
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    h[r][v] = fmaf(__builtin_amdgcn_exp2f(st * A2[v]), h[r][v], sx * Bv[r][v]);
+                    yv = fmaf(h[r][v], Cv[r][v], yv);
                 }
-            }
+                yv = has ? yv : 0.f;
 #pragma unroll
-            for (int o = 1; o < LPC; o <<= 1) yv += __shfl_xor(yv, o, 64);
-            yv = fmaf(D ? D[c] : 0.f, xv, yv);
-            if (z) { const float zv = to_f(z[b * z_b + c]); yv *= zv * sigmoid(zv); }
+                for (int o = 1; o < LPC; o <<= 1) yv += __shfl_xor(yv, o, 64);
+                yv = fmaf(Dc, xv, yv);
+                if (z) { const float zv = to_f(zr[r]); yv *= zv * sigmoid(zv); }
+            }
+            if (on && has && (act[r] || state_out != state)) {
+                float* sp = state_out + b * pitch + at0;
+                if constexpr (V == 4) *reinterpret_cast<float4*>(sp) = *reinterpret_cast<float4*>(h[r]);
+                else *sp = h[r][0];
+            }
+            if (on && part == 0) y[(long long)b * C + c] = from_f<M>(yv);
         }
-        if (has && (act || state_out != state)) {
-            if constexpr (V == 4) *reinterpret_cast<float4*>(state_out + i * N + n0) = *reinterpret_cast<float4*>(hv);
-            else state_out[i * N + n0] = hv[0];
-        }
-        if (part == 0) y[i] = from_f<M>(yv);
     }
 }
 
@@ -239,11 +288,18 @@ template <class T, class M, int MODE> int run(const gmt_scan_args* args, hipStre
 template <class M, int V, int LPC> int launch_step(const gmt_scan_args* a, const unsigned char* active, hipStream_t stream)
 {
     using R = typename M::raw;
-    const long long per = 256 / LPC, need = ((long long)a->B * a->C + per - 1) / per;
-    const unsigned grid = (unsigned)(need < 256 * 32 ? need : 256 * 32);
-    hipLaunchKernelGGL((scan_step_kernel<M, V, LPC>), dim3(grid), dim3(256), 0, stream, (const R*)a->x, a->x_b, (const R*)a->dt, a->dt_b,
+    const int chans = 256 / LPC, gx = (a->C + chans - 1) / chans;
+    // 4 rows at a time once 8 workgroups a CU are at work, 16 workgroups a CU at most
+    const int rows = (long long)gx * a->B >= 4 * 8 * 256 ? 4 : 1;
+    long long groups = (a->B + rows - 1) / rows;
+    const long long most = (16 * 256 + gx - 1) / gx;
+    if (groups > most) groups = most;
+    const int esz = sizeof(R);
+    const int wide = (((uintptr_t)a->Bm | (uintptr_t)a->Cm) % (4 * esz)) == 0 && ((a->B_b | a->B_g | a->C_b | a->C_g) & 3) == 0;
+    auto k = rows == 4 ? scan_step_kernel<M, V, LPC, 4> : scan_step_kernel<M, V, LPC, 1>;
+    hipLaunchKernelGGL(k, dim3((unsigned)(gx * groups)), dim3(256), 0, stream, (const R*)a->x, a->x_b, (const R*)a->dt, a->dt_b,
                        (const R*)a->z, a->z_b, (const R*)a->Bm, a->B_b, a->B_g, (const R*)a->Cm, a->C_b, a->C_g, a->A, a->D, a->dt_bias,
-                       a->state, a->state_out, active, (R*)a->y, a->B, a->C, a->N, a->G);
+                       a->state, a->state_out, active, (R*)a->y, a->B, a->C, a->N, a->G, gx, wide);
     GMT_LAUNCH_CHECK();
     return GMT_OK;
 }

@@ -8,6 +8,7 @@ checkpoints stand for (the outputs are computed from the inputs themselves).
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from typing import NamedTuple, Optional, Tuple
 
@@ -26,18 +27,31 @@ class Ckpt8(NamedTuple):
     dtype: torch.dtype
 
 
-def on_device(*tensors) -> torch.device:
-    """The one GPU that all of them are on."""
-    L_.require_cuda(*tensors)
-    devs = {t.device for t in tensors if t is not None}
-    if len(devs) != 1:
-        raise L_.GmtError(f'tensors on different devices: {sorted(str(d) for d in devs)}')
-    return devs.pop()
+_HERE = contextlib.nullcontext()
+
+
+def on_device(*tensors) -> int:
+    """Index of the one GPU that all of them (None: left out) are on."""
+    dev = None
+    for t in tensors:
+        if t is not None:
+            d = t.get_device()
+            if d != dev:
+                L_.require_cuda(t)
+                if dev is not None:
+                    raise L_.GmtError(f'tensors on different devices: cuda:{dev} and cuda:{d}')
+                dev = d
+    return dev
+
+
+def on(dev: int):
+    """Context in which `dev` is the current device (nothing to do where it is already: a device switch costs microseconds)."""
+    return _HERE if dev == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
 def time_major(t: torch.Tensor) -> torch.Tensor:
     """`t` itself when its last axis is contiguous (rows may have any pitch), else a contiguous copy."""
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    return t if t.stride()[-1] == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
 def pack(x: torch.Tensor) -> Ckpt8:
@@ -47,26 +61,26 @@ def pack(x: torch.Tensor) -> Ckpt8:
         raise L_.GmtError(f'ckpt8 packs float32 and bfloat16, not {x.dtype}')
     if x.dim() < 1 or x.numel() == 0:
         raise L_.GmtError(f'ckpt8: nothing to pack in a tensor of shape {tuple(x.shape)}')
-    x = time_major(x.detach())
+    x = time_major(x.detach()) if x.requires_grad else time_major(x)
     C = x.shape[-1]
     if x.dim() == 3:
         T, B, st, sb = x.shape[0], x.shape[1], x.stride(0), x.stride(1)
     else:
         x = x if x.dim() <= 2 else x.contiguous()
         T, B, st, sb = x.numel() // C, 1, (x.stride(0) if x.dim() == 2 else C), C
-    with torch.cuda.device(dev):
-        codes = torch.empty(x.shape, device=dev, dtype=torch.int8)
-        exps = torch.empty(*x.shape[:-1], (C + BLOCK - 1) // BLOCK, device=dev, dtype=torch.uint8)
+    with on(dev):
+        codes = x.new_empty(x.shape, dtype=torch.int8)
+        exps = x.new_empty((*x.shape[:-1], (C + BLOCK - 1) // BLOCK), dtype=torch.uint8)
         L_.call('gmt_ckpt8_pack', x.data_ptr(), st, sb, codes.data_ptr(), exps.data_ptr(), T, B, C, int(x.dtype == torch.bfloat16),
                 L_.stream(), nbytes=float(x.numel() * (x.element_size() + 1)))
     return Ckpt8(codes, exps, x.dtype)
 
 
-def check(p: Ckpt8) -> torch.device:
+def check(p: Ckpt8) -> int:
     dev = on_device(p.codes, p.exponents)
     C = p.codes.shape[-1]
     if (p.codes.dtype != torch.int8 or p.exponents.dtype != torch.uint8 or p.codes.numel() == 0 or not p.codes.is_contiguous()
-            or not p.exponents.is_contiguous() or tuple(p.exponents.shape) != (*p.codes.shape[:-1], (C + BLOCK - 1) // BLOCK)):
+            or not p.exponents.is_contiguous() or p.exponents.shape != (*p.codes.shape[:-1], (C + BLOCK - 1) // BLOCK)):
         raise L_.GmtError('not an 8-bit checkpoint: contiguous int8 codes [..., C] and uint8 exponents [..., ceil(C / 32)] expected')
     return dev
 
@@ -78,8 +92,8 @@ def unpack(p: Ckpt8, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     if dtype not in DTYPES:
         raise L_.GmtError(f'ckpt8 unpacks to float32 and bfloat16, not {dtype}')
     C = p.codes.shape[-1]
-    with torch.cuda.device(dev):
-        out = torch.empty(p.codes.shape, device=dev, dtype=dtype)
+    with on(dev):
+        out = p.codes.new_empty(p.codes.shape, dtype=dtype)
         L_.call('gmt_ckpt8_unpack', p.codes.data_ptr(), p.exponents.data_ptr(), out.data_ptr(), out.numel() // C, C,
                 int(dtype == torch.bfloat16), L_.stream(), nbytes=float(out.numel() * (out.element_size() + 1)))
     return out
@@ -98,16 +112,16 @@ def wgrad(dY: torch.Tensor, p: Ckpt8, want_db: bool = False) -> Tuple[torch.Tens
     R = p.codes.numel() // I
     if N == 0 or dY.numel() // N != R:
         raise L_.GmtError(f'wgrad: dY {tuple(dY.shape)} and the checkpoint {tuple(p.codes.shape)} have different rows')
-    dY = time_major(dY.detach())
+    dY = time_major(dY.detach()) if dY.requires_grad else time_major(dY)
     if dY.dim() != 2:
         dY = dY.reshape(R, N)
     if R > 1 and dY.stride(0) < N:                       # (an expanded gradient: its rows share memory)
         dY = dY.contiguous()
-    with torch.cuda.device(dev):
+    with on(dev):
         need = ctypes.c_longlong(0)
         L_.call('gmt_ckpt8_wgrad_workspace_floats', R, N, I, ctypes.addressof(need), label='skip')
-        ws = torch.empty(need.value, device=dev, dtype=torch.float32)
-        out = torch.empty(N * I + N, device=dev, dtype=torch.float32)
+        ws = dY.new_empty(need.value, dtype=torch.float32)
+        out = dY.new_empty(N * I + N, dtype=torch.float32)
         L_.call('gmt_ckpt8_wgrad', dY.data_ptr(), max(dY.stride(0), N), p.codes.data_ptr(), p.exponents.data_ptr(), out.data_ptr(), R,
                 N, I, int(dY.dtype == torch.bfloat16), int(want_db), L_.ptr(ws), need.value, L_.stream(),
                 label=f'wgrad8_N{N}_I{I}', flops=2.0 * R * N * I)

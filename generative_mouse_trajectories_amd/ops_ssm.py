@@ -20,7 +20,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib as L_
 from . import ops_ckpt8
-from .ops_ckpt8 import Ckpt8, on_device, time_major
+from .ops_ckpt8 import Ckpt8, on, on_device, time_major
 
 MAX_STATES = 32
 
@@ -29,9 +29,9 @@ def _fail(msg: str):
     raise L_.GmtError(msg)
 
 
-def _want(t: Optional[torch.Tensor], name: str, shape, dtype) -> None:
-    if t is not None and (tuple(t.shape) != tuple(shape) or t.dtype != dtype):
-        _fail(f'{name}: {dtype} {tuple(shape)} expected, got {t.dtype} {tuple(t.shape)}')
+def _want(t: Optional[torch.Tensor], name: str, shape: tuple, dtype) -> None:
+    if t is not None and (t.shape != shape or t.dtype != dtype):
+        _fail(f'{name}: {dtype} {shape} expected, got {t.dtype} {tuple(t.shape)}')
 
 
 def _seq(x: torch.Tensor, name: str, dims: int) -> None:
@@ -41,96 +41,120 @@ def _seq(x: torch.Tensor, name: str, dims: int) -> None:
         _fail(f'{name}: float32 or bfloat16 expected, got {x.dtype}')
 
 
-def _lengths(lengths: Optional[torch.Tensor], B: int, L: int, dev) -> Optional[torch.Tensor]:
+def _lengths(lengths: Optional[torch.Tensor], B: int, L: int, x: torch.Tensor) -> Optional[torch.Tensor]:
     if lengths is None:
         return None
-    if lengths.dtype not in (torch.int32, torch.int64) or tuple(lengths.shape) != (B,):
+    if lengths.dtype not in (torch.int32, torch.int64) or lengths.shape != (B,):
         _fail(f'lengths: an int32 or int64 tensor of {B} rows expected, got {lengths.dtype} {tuple(lengths.shape)}')
     if lengths.dtype == torch.int64:
         lengths = lengths.clamp(0, L)
-    return lengths.to(device=dev, dtype=torch.int32).contiguous()
+    return lengths.to(device=x.device, dtype=torch.int32).contiguous()
 
 
-def _active(active: Optional[torch.Tensor], B: int, dev) -> Optional[torch.Tensor]:
+def _active(active: Optional[torch.Tensor], B: int, x: torch.Tensor) -> Optional[torch.Tensor]:
     if active is None:
         return None
-    if active.dtype not in (torch.bool, torch.uint8) or tuple(active.shape) != (B,):
+    if active.dtype not in (torch.bool, torch.uint8) or active.shape != (B,):
         _fail(f'active: a bool tensor of {B} rows expected, got {active.dtype} {tuple(active.shape)}')
-    return active.to(dev).contiguous()
+    return active.to(x.device).contiguous()
 
 
-def _step_states(state: torch.Tensor, state_out: Optional[torch.Tensor], name: str, shape, dtype) -> torch.Tensor:
+def _step_states(state: torch.Tensor, state_out: Optional[torch.Tensor], shape: tuple, dtype) -> torch.Tensor:
     """The buffer of the updated state: `state` itself, or one that does not overlap it."""
-    _want(state, name, shape, dtype)
-    out = state if state_out is None else state_out
-    _want(out, f'{name}_out', shape, dtype)
-    if not state.is_contiguous() or not out.is_contiguous():
-        _fail(f'{name}: states of a single step are updated where they are and must be contiguous')
-    if out.data_ptr() != state.data_ptr():
-        n = state.numel() * state.element_size()
-        if abs(out.data_ptr() - state.data_ptr()) < n:
-            _fail(f'{name}_out overlaps {name}')
-    return out
+    _want(state, 'state', shape, dtype)
+    if not state.is_contiguous():
+        _fail('state: the state of a single step is updated where it is and must be contiguous')
+    if state_out is None:
+        return state
+    _want(state_out, 'state_out', shape, dtype)
+    if not state_out.is_contiguous():
+        _fail('state_out: must be contiguous')
+    apart = abs(state_out.data_ptr() - state.data_ptr())
+    if 0 < apart < state.numel() * state.element_size():
+        _fail('state_out overlaps state')
+    return state_out
 
 
 def _no_grad_only(name: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        _fail(f'{name} has no backward pass: call it under torch.no_grad() (for training, {name[:-5]} over whole sequences)')
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            _fail(f'{name} has no backward pass: call it under torch.no_grad() (for training, {name[:-5]} over whole sequences)')
+
+
+def _any_grad(*tensors) -> bool:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+def _whole(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
+def _at(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _space(n: int, like: torch.Tensor) -> Optional[torch.Tensor]:
+    return like.new_empty(n, dtype=torch.float32) if n else None
 
 
 # ----------------------------------------------------------------------------------------
 # short causal convolution
 # ----------------------------------------------------------------------------------------
 def _conv_args(x, weight, bias, state, lengths, silu, **more) -> L_.ConvArgs:
-    p = L_.ptr
-    shape = (x.codes if isinstance(x, Ckpt8) else x).shape
-    a = L_.ConvArgs(w=p(weight), bias=p(bias), state=p(state), lengths=p(lengths), L=shape[0], B=shape[1], C=shape[2],
-                    K=weight.shape[1], silu=int(silu), **more)
     if isinstance(x, Ckpt8):
-        a.x, a.x_scale, a.bf16 = p(x.codes), p(x.exponents), int(x.dtype == torch.bfloat16)
+        shape = x.codes.shape
+        more.update(x=x.codes.data_ptr(), x_scale=x.exponents.data_ptr(), bf16=x.dtype == torch.bfloat16)
     else:
-        a.x, a.x_t, a.x_b, a.bf16 = x.data_ptr(), x.stride(0), x.stride(1), int(x.dtype == torch.bfloat16)
-    return a
+        shape, st = x.shape, x.stride()
+        more.update(x=x.data_ptr(), x_t=st[0], x_b=st[1], bf16=x.dtype == torch.bfloat16)
+    return L_.ConvArgs(w=weight.data_ptr(), bias=_at(bias), state=_at(state), lengths=_at(lengths), L=shape[0], B=shape[1], C=shape[2],
+                       K=weight.shape[1], silu=silu, **more)
+
+
+def _conv_forward(x, weight, bias, state, lengths, silu):
+    y = x.new_empty(x.shape)
+    last = x.new_empty((weight.shape[1] - 1, x.shape[1], x.shape[2]))
+    a = _conv_args(x, weight, bias, state, lengths, silu, y=y.data_ptr(), state_out=last.data_ptr())
+    L_.call('gmt_causal_conv_fwd', ctypes.addressof(a), L_.stream(), nbytes=2.0 * x.numel() * x.element_size())
+    return y, last
 
 
 class CausalConvFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, state, lengths, silu, ckpt8, keep):
-        L, B, C = x.shape
-        K = weight.shape[1]
-        y = torch.empty(L, B, C, device=x.device, dtype=x.dtype)
-        last = torch.empty(K - 1, B, C, device=x.device, dtype=x.dtype)
-        a = _conv_args(x, weight, bias, state, lengths, silu, y=L_.ptr(y), state_out=L_.ptr(last))
-        L_.call('gmt_causal_conv_fwd', ctypes.addressof(a), L_.stream(), nbytes=2.0 * x.numel() * x.element_size())
-        if keep:
-            packed = ops_ckpt8.pack(x) if ckpt8 else None
-            ctx.save_for_backward(*((packed.codes, packed.exponents) if ckpt8 else (x, None)), weight, bias, state, lengths)
-            ctx.silu, ctx.dtype, ctx.ckpt8 = silu, x.dtype, ckpt8
-            ctx.set_materialize_grads(False)
+    def forward(ctx, x, weight, bias, state, lengths, silu, ckpt8):
+        y, last = _conv_forward(x, weight, bias, state, lengths, silu)
+        packed = ops_ckpt8.pack(x) if ckpt8 else None
+        ctx.save_for_backward(*((packed.codes, packed.exponents) if ckpt8 else (x, None)), weight, bias, state, lengths)
+        ctx.silu, ctx.dtype, ctx.ckpt8 = silu, x.dtype, ckpt8
+        ctx.set_materialize_grads(False)
         return y, last
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dlast):
         x, exps, weight, bias, state, lengths = ctx.saved_tensors
+        shape, dtype, K = x.shape, ctx.dtype, weight.shape[1]
         if ctx.ckpt8:
-            x = Ckpt8(x, exps, ctx.dtype)
-        L, B, C = (x.codes if ctx.ckpt8 else x).shape
-        K, dev = weight.shape[1], weight.device
-        with torch.cuda.device(dev):
-            dy = torch.zeros(L, B, C, device=dev, dtype=ctx.dtype) if dy is None else time_major(dy)
-            dlast = None if dlast is None else dlast.contiguous()
-            dx = torch.empty(L, B, C, device=dev, dtype=ctx.dtype)
-            dparam = torch.empty(K + 1, C, device=dev, dtype=torch.float32)
+            x = Ckpt8(x, exps, dtype)
+        with on(weight.get_device()):
+            dy = weight.new_zeros(shape, dtype=dtype) if dy is None else time_major(dy)
+            dlast = _whole(dlast)
+            dx = weight.new_empty(shape, dtype=dtype)
+            dparam = weight.new_empty((K + 1, shape[2]))
             dstate = None if state is None else torch.empty_like(state)
-            a = _conv_args(x, weight, bias, state, lengths, ctx.silu, dy=dy.data_ptr(), dstate_out=L_.ptr(dlast), dx=L_.ptr(dx),
-                           dparam=L_.ptr(dparam), dstate=L_.ptr(dstate), dy_t=dy.stride(0), dy_b=dy.stride(1))
+            st = dy.stride()
+            a = _conv_args(x, weight, bias, state, lengths, ctx.silu, dy=dy.data_ptr(), dstate_out=_at(dlast), dx=dx.data_ptr(),
+                           dparam=dparam.data_ptr(), dstate=_at(dstate), dy_t=st[0], dy_b=st[1])
             need = ctypes.c_longlong(0)
             L_.call('gmt_causal_conv_bwd_workspace_floats', ctypes.addressof(a), ctypes.addressof(need), label='skip')
-            ws = torch.empty(need.value, device=dev, dtype=torch.float32)
-            a.workspace, a.workspace_floats = L_.ptr(ws), need.value
+            ws = _space(need.value, weight)
+            a.workspace, a.workspace_floats = _at(ws), need.value
             L_.call('gmt_causal_conv_bwd', ctypes.addressof(a), L_.stream(), nbytes=3.0 * dx.numel() * dx.element_size())
-        return dx, dparam[:K].t().contiguous(), (None if bias is None else dparam[K]), dstate, None, None, None, None
+        return dx, dparam[:K].t().contiguous(), (None if bias is None else dparam[K]), dstate, None, None, None
 
 
 def _conv_checks(x, weight, bias, dims: int):
@@ -152,11 +176,12 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     C, K = _conv_checks(x, weight, bias, 3)
     L, B = x.shape[:2]
     _want(state, 'state', (K - 1, B, C), x.dtype)
-    keep = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, state))
-    lengths = _lengths(lengths, B, L, dev)
-    with torch.cuda.device(dev):
-        return CausalConvFn.apply(time_major(x), weight.contiguous(), None if bias is None else bias.contiguous(),
-                                  None if state is None else state.contiguous(), lengths, bool(silu), bool(ckpt8), keep)
+    lengths = _lengths(lengths, B, L, x)
+    args = time_major(x), _whole(weight), _whole(bias), _whole(state), lengths, bool(silu)
+    with on(dev):
+        if _any_grad(x, weight, bias, state):
+            return CausalConvFn.apply(*args, bool(ckpt8))
+        return _conv_forward(*args)
 
 
 def causal_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, silu: bool = True,
@@ -166,16 +191,16 @@ def causal_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor,
     dev = on_device(x, state, weight, bias, state_out)
     C, K = _conv_checks(x, weight, bias, 2)
     B = x.shape[0]
-    out = _step_states(state, state_out, 'state', (K - 1, B, C), x.dtype)
-    _no_grad_only('causal_conv_step', x, state, weight, bias, state_out)
-    x, active = time_major(x), _active(active, B, dev)
-    with torch.cuda.device(dev):
-        weight, bias = weight.contiguous(), None if bias is None else bias.contiguous()
-        y = torch.empty(B, C, device=dev, dtype=x.dtype)
-        a = L_.ConvArgs(x=x.data_ptr(), w=L_.ptr(weight), bias=L_.ptr(bias), state=L_.ptr(state), y=L_.ptr(y), state_out=L_.ptr(out),
-                        x_b=x.stride(0), L=1, B=B, C=C, K=K, bf16=int(x.dtype == torch.bfloat16), silu=int(silu))
-        L_.call('gmt_causal_conv_step', ctypes.addressof(a), L_.ptr(active), L_.stream(),
-                nbytes=float(2 * K * x.numel() * x.element_size()))
+    out = _step_states(state, state_out, (K - 1, B, C), x.dtype)
+    if torch.is_grad_enabled():
+        _no_grad_only('causal_conv_step', x, state, weight, bias, state_out)
+    active = _active(active, B, x)
+    x, weight, bias = time_major(x), _whole(weight), _whole(bias)
+    with on(dev):
+        y = x.new_empty((B, C))
+        a = L_.ConvArgs(x=x.data_ptr(), w=weight.data_ptr(), bias=_at(bias), state=state.data_ptr(), y=y.data_ptr(), state_out=out.data_ptr(),
+                        x_b=x.stride()[0], L=1, B=B, C=C, K=K, bf16=x.dtype == torch.bfloat16, silu=bool(silu))
+        L_.call('gmt_causal_conv_step', ctypes.addressof(a), _at(active), L_.stream(), nbytes=2.0 * K * B * C * x.element_size())
     torch.autograd.graph.increment_version(out)
     return y
 
@@ -183,112 +208,114 @@ def causal_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor,
 # ----------------------------------------------------------------------------------------
 # selective scan
 # ----------------------------------------------------------------------------------------
+def _map_pitches(m: torch.Tensor, lead: int):
+    """Pitches of B or C [.., N] or [.., G, N]: (step, row, group), the step's 0 without a step axis."""
+    st = m.stride()
+    return (st[0] if lead == 2 else 0), st[lead - 1], (st[lead] if m.dim() == lead + 2 else 0)
+
+
 def _scan_args(x, dt, z, A, B, C, D, dt_bias, state, lengths, **more) -> L_.ScanArgs:
-    p = L_.ptr
-    q8 = isinstance(x, Ckpt8)
-    shape = (x.codes if q8 else x).shape
-    a = L_.ScanArgs(A=p(A), Bm=B.data_ptr(), Cm=C.data_ptr(), D=p(D), dt_bias=p(dt_bias), state=p(state), lengths=p(lengths),
-                    B_t=B.stride(0), B_b=B.stride(1), B_g=B.stride(2), C_t=C.stride(0), C_b=C.stride(1), C_g=C.stride(2),
-                    L=shape[0], B=shape[1], C=shape[2], N=A.shape[1], G=B.shape[2], bf16=int(B.dtype == torch.bfloat16), **more)
-    for name, t in (('x', x), ('dt', dt), ('z', z)):
-        if t is None:
-            continue
-        if q8:
-            setattr(a, name, p(t.codes))
-            setattr(a, name + '_scale', p(t.exponents))
-        else:
-            setattr(a, name, t.data_ptr())
-            setattr(a, name + '_t', t.stride(0))
-            setattr(a, name + '_b', t.stride(1))
-    return a
+    if isinstance(x, Ckpt8):
+        shape = x.codes.shape
+        more.update(x=x.codes.data_ptr(), x_scale=x.exponents.data_ptr(), dt=dt.codes.data_ptr(), dt_scale=dt.exponents.data_ptr())
+        if z is not None:
+            more.update(z=z.codes.data_ptr(), z_scale=z.exponents.data_ptr())
+    else:
+        shape, xs, ds = x.shape, x.stride(), dt.stride()
+        more.update(x=x.data_ptr(), x_t=xs[0], x_b=xs[1], dt=dt.data_ptr(), dt_t=ds[0], dt_b=ds[1])
+        if z is not None:
+            zs = z.stride()
+            more.update(z=z.data_ptr(), z_t=zs[0], z_b=zs[1])
+    Bp, Cp = _map_pitches(B, 2), _map_pitches(C, 2)
+    return L_.ScanArgs(A=A.data_ptr(), Bm=B.data_ptr(), Cm=C.data_ptr(), D=_at(D), dt_bias=_at(dt_bias), state=_at(state), lengths=_at(lengths),
+                       B_t=Bp[0], B_b=Bp[1], B_g=Bp[2], C_t=Cp[0], C_b=Cp[1], C_g=Cp[2], L=shape[0], B=shape[1], C=shape[2], N=A.shape[1],
+                       G=1 if B.dim() == 3 else B.shape[2], bf16=B.dtype == torch.bfloat16, **more)
 
 
-def _workspace(a) -> Tuple[int, int, int]:
-    n = [ctypes.c_longlong(0) for _ in range(3)]
-    L_.call('gmt_selective_scan_workspace', ctypes.addressof(a), *(ctypes.addressof(v) for v in n), label='skip')
-    return tuple(v.value for v in n)
+def _workspace(a):
+    """Floats of (the kept states, a forward call's workspace, a backward call's)."""
+    n = (ctypes.c_longlong * 3)()
+    at = ctypes.addressof(n)
+    L_.call('gmt_selective_scan_workspace', ctypes.addressof(a), at, at + 8, at + 16, label='skip')
+    return n
+
+
+def _scan_forward(x, dt, A, B, C, D, z, dt_bias, state, lengths, keep):
+    y = x.new_empty(x.shape)
+    last = A.new_empty((x.shape[1], *A.shape))
+    a = _scan_args(x, dt, z, A, B, C, D, dt_bias, state, lengths, y=y.data_ptr(), state_out=last.data_ptr())
+    n_ck, n_fwd, _ = _workspace(a)
+    ck, ws = _space(n_ck if keep else 0, A), _space(n_fwd, A)
+    a.ck, a.workspace, a.workspace_floats = _at(ck), _at(ws), n_fwd
+    L_.call('gmt_selective_scan_fwd', ctypes.addressof(a), L_.stream(), nbytes=float((3 + (z is not None)) * x.numel() * x.element_size()))
+    return y, last, ck
 
 
 class SelectiveScanFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, dt, A, B, C, D, z, dt_bias, state, lengths, ckpt8, keep):
-        L, Bt, Ch = x.shape
-        dev = x.device
-        y = torch.empty(L, Bt, Ch, device=dev, dtype=x.dtype)
-        last = torch.empty(Bt, Ch, A.shape[1], device=dev, dtype=torch.float32)
-        a = _scan_args(x, dt, z, A, B, C, D, dt_bias, state, lengths, y=L_.ptr(y), state_out=L_.ptr(last))
-        n_ck, n_fwd, _ = _workspace(a)
-        # the states before every eighth step; from 8-bit checkpoints the backward pass finds them itself
-        ck = torch.empty(n_ck if keep and not ckpt8 else 0, device=dev, dtype=torch.float32)
-        ws = torch.empty(n_fwd, device=dev, dtype=torch.float32)
-        a.ck, a.workspace, a.workspace_floats = L_.ptr(ck), L_.ptr(ws), n_fwd
-        L_.call('gmt_selective_scan_fwd', ctypes.addressof(a), L_.stream(),
-                nbytes=float((3 + (z is not None)) * x.numel() * x.element_size()))
-        if keep:
-            seqs = []
-            for t in (x, dt, z):
-                p = ops_ckpt8.pack(t) if ckpt8 and t is not None else None
-                seqs += [t, None] if p is None else [p.codes, p.exponents]
-            ctx.save_for_backward(*seqs, A, B, C, D, dt_bias, state, lengths, ck)
-            ctx.dtype, ctx.ckpt8 = x.dtype, ckpt8
-            ctx.set_materialize_grads(False)
+    def forward(ctx, x, dt, A, B, C, D, z, dt_bias, state, lengths, ckpt8):
+        # the state before every eighth step; from 8-bit checkpoints the backward pass finds them itself
+        y, last, ck = _scan_forward(x, dt, A, B, C, D, z, dt_bias, state, lengths, not ckpt8)
+        seqs = []
+        for t in (x, dt, z):
+            p = ops_ckpt8.pack(t) if ckpt8 and t is not None else None
+            seqs += [t, None] if p is None else [p.codes, p.exponents]
+        ctx.save_for_backward(*seqs, A, B, C, D, dt_bias, state, lengths, ck)
+        ctx.dtype, ctx.ckpt8 = x.dtype, ckpt8
+        ctx.set_materialize_grads(False)
         return y, last
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dlast):
         x, xe, dt, dte, z, ze, A, B, C, D, dt_bias, state, lengths, ck = ctx.saved_tensors
-        L, Bt, Ch = x.shape
-        N, dev, dtype = A.shape[1], A.device, ctx.dtype
+        shape, dtype, (Ch, N) = x.shape, ctx.dtype, A.shape
         if ctx.ckpt8:
             x, dt = Ckpt8(x, xe, dtype), Ckpt8(dt, dte, dtype)
             z = None if z is None else Ckpt8(z, ze, dtype)
-        with torch.cuda.device(dev):
-            dy = torch.zeros(L, Bt, Ch, device=dev, dtype=dtype) if dy is None else time_major(dy)
-            dlast = None if dlast is None else dlast.contiguous()
-            dx, ddt, dz = (torch.empty(L, Bt, Ch, device=dev, dtype=dtype) for _ in range(3)) if z is not None else \
-                (torch.empty(L, Bt, Ch, device=dev, dtype=dtype), torch.empty(L, Bt, Ch, device=dev, dtype=dtype), None)
-            dB, dC = (torch.empty(B.shape, device=dev, dtype=dtype) for _ in range(2))
-            dparam = torch.empty(Ch * (N + 2), device=dev, dtype=torch.float32)
+        with on(A.get_device()):
+            dy = A.new_zeros(shape, dtype=dtype) if dy is None else time_major(dy)
+            dlast = _whole(dlast)
+            dx, ddt = A.new_empty(shape, dtype=dtype), A.new_empty(shape, dtype=dtype)
+            dz = None if z is None else A.new_empty(shape, dtype=dtype)
+            dB, dC = B.new_empty(B.shape), C.new_empty(C.shape)
+            dparam = A.new_empty(Ch * (N + 2))
             dstate = None if state is None else torch.empty_like(state)
-            p = L_.ptr
-            a = _scan_args(x, dt, z, A, B, C, D, dt_bias, state, lengths, dy=dy.data_ptr(), dstate_out=p(dlast), dx=p(dx), ddt=p(ddt),
-                           dz=p(dz), dB=p(dB), dC=p(dC), dparam=p(dparam), dstate=p(dstate), dy_t=dy.stride(0), dy_b=dy.stride(1))
+            st = dy.stride()
+            a = _scan_args(x, dt, z, A, B, C, D, dt_bias, state, lengths, dy=dy.data_ptr(), dstate_out=_at(dlast), dx=dx.data_ptr(),
+                           ddt=ddt.data_ptr(), dz=_at(dz), dB=dB.data_ptr(), dC=dC.data_ptr(), dparam=dparam.data_ptr(), dstate=_at(dstate),
+                           dy_t=st[0], dy_b=st[1])
             n_ck, _, n_bwd = _workspace(a)
             if ctx.ckpt8:
-                ck = torch.empty(n_ck, device=dev, dtype=torch.float32)
-            ws = torch.empty(n_bwd, device=dev, dtype=torch.float32)
-            a.ck, a.workspace, a.workspace_floats = p(ck), p(ws), n_bwd
+                ck = _space(n_ck, A)
+            ws = _space(n_bwd, A)
+            a.ck, a.workspace, a.workspace_floats = ck.data_ptr(), _at(ws), n_bwd
             L_.call('gmt_selective_scan_bwd', ctypes.addressof(a), L_.stream(),
                     nbytes=float((5 + 2 * (z is not None)) * dx.numel() * dx.element_size()))
-        dA = dparam[:Ch * N].view(Ch, N)
-        return (dx, ddt, dA, dB, dC, None if D is None else dparam[Ch * N:Ch * (N + 1)], dz,
-                None if dt_bias is None else dparam[Ch * (N + 1):], dstate, None, None, None)
+        return (dx, ddt, dparam[:Ch * N].view(Ch, N), dB, dC, None if D is None else dparam[Ch * N:Ch * (N + 1)], dz,
+                None if dt_bias is None else dparam[Ch * (N + 1):], dstate, None, None)
 
 
-def _scan_checks(x, dt, A, B, C, D, z, dt_bias, state, lead):
-    """Shapes and types of a scan over `lead` = (L, B) or (B,) -> B and C with their group axis."""
-    Ch = x.shape[-1]
+def _scan_checks(x, dt, A, B, C, D, z, dt_bias, lead: tuple):
+    """Shapes and types of a scan over `lead` = (L, B) or (B,)."""
+    shape, dtype = x.shape, x.dtype
+    Ch = shape[-1]
     if A.dim() != 2 or not 1 <= A.shape[1] <= MAX_STATES:
         _fail(f'A: [{Ch}, N] with N = 1 .. {MAX_STATES} states expected, got {tuple(A.shape)}')
     N = A.shape[1]
     _want(A, 'A', (Ch, N), torch.float32)
-    _want(dt, 'dt', x.shape, x.dtype)
-    _want(z, 'z', x.shape, x.dtype)
+    _want(dt, 'dt', shape, dtype)
+    _want(z, 'z', shape, dtype)
     _want(D, 'D', (Ch,), torch.float32)
     _want(dt_bias, 'dt_bias', (Ch,), torch.float32)
-    _want(state, 'state', (lead[-1], Ch, N), torch.float32)
-    maps = []
+    groups = []
     for name, m in (('B', B), ('C', C)):
-        if m.dim() == len(lead) + 1:
-            m = m.unsqueeze(-2)
-        if m.dim() != len(lead) + 2 or m.shape[-2] < 1 or Ch % m.shape[-2]:
-            _fail(f'{name}: {(*lead, N)} or {(*lead, "G", N)} with G dividing {Ch} channels expected, got {tuple(m.shape)}')
-        _want(m, name, (*lead, m.shape[-2], N), x.dtype)
-        maps.append(time_major(m))
-    if maps[0].shape != maps[1].shape:
-        _fail(f'B and C have different groups: {maps[0].shape[-2]} and {maps[1].shape[-2]}')
-    return maps
+        G = m.shape[-2] if m.dim() == len(lead) + 2 else 1
+        if G < 1 or Ch % G or m.shape != ((*lead, N) if m.dim() == len(lead) + 1 else (*lead, G, N)) or m.dtype != dtype:
+            _fail(f'{name}: {dtype} {(*lead, N)} or {(*lead, "G", N)} with G dividing {Ch} channels expected, got {m.dtype} {tuple(m.shape)}')
+        groups.append(G)
+    if groups[0] != groups[1]:
+        _fail(f'B and C have different groups: {groups[0]} and {groups[1]}')
 
 
 def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor, D: Optional[torch.Tensor] = None,
@@ -299,14 +326,16 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     last step).  ckpt8: x, dt and z are kept in 8 bits for the backward pass, which then finds the states again."""
     dev = on_device(x, dt, A, B, C, D, z, dt_bias, state)
     _seq(x, 'x', 3)
-    L, Bt, _ = x.shape
-    Bm, Cm = _scan_checks(x, dt, A, B, C, D, z, dt_bias, state, (L, Bt))
-    keep = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, dt, A, B, C, D, z, dt_bias, state))
-    whole = lambda t: None if t is None else t.contiguous()  # noqa: E731
-    lengths = _lengths(lengths, Bt, L, dev)
-    with torch.cuda.device(dev):
-        return SelectiveScanFn.apply(time_major(x), time_major(dt), whole(A), Bm, Cm, whole(D), None if z is None else time_major(z),
-                                     whole(dt_bias), whole(state), lengths, bool(ckpt8), keep)
+    L, Bt, Ch = x.shape
+    _scan_checks(x, dt, A, B, C, D, z, dt_bias, (L, Bt))
+    _want(state, 'state', (Bt, Ch, A.shape[1]), torch.float32)
+    lengths = _lengths(lengths, Bt, L, x)
+    args = (time_major(x), time_major(dt), _whole(A), time_major(B), time_major(C), _whole(D), None if z is None else time_major(z),
+            _whole(dt_bias), _whole(state), lengths)
+    with on(dev):
+        if _any_grad(x, dt, A, B, C, D, z, dt_bias, state):
+            return SelectiveScanFn.apply(*args, bool(ckpt8))
+        return _scan_forward(*args, False)[:2]
 
 
 def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor, state: torch.Tensor,
@@ -317,17 +346,22 @@ def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: t
     dev = on_device(x, dt, A, B, C, state, D, z, dt_bias, state_out)
     _seq(x, 'x', 2)
     Bt, Ch = x.shape
-    Bm, Cm = _scan_checks(x, dt, A, B, C, D, z, dt_bias, None, (Bt,))
+    _scan_checks(x, dt, A, B, C, D, z, dt_bias, (Bt,))
     N = A.shape[1]
-    out = _step_states(state, state_out, 'state', (Bt, Ch, N), torch.float32)
-    _no_grad_only('selective_scan_step', x, dt, A, B, C, state, D, z, dt_bias, state_out)
-    active = _active(active, Bt, dev)
-    with torch.cuda.device(dev):
-        y = torch.empty(Bt, Ch, device=dev, dtype=x.dtype)
-        up = lambda t: None if t is None else time_major(t).unsqueeze(0)  # noqa: E731
-        whole = lambda t: None if t is None else t.contiguous()  # noqa: E731
-        A, D, dt_bias, x, dt, z = whole(A), whole(D), whole(dt_bias), up(x), up(dt), up(z)
-        a = _scan_args(x, dt, z, A, Bm.unsqueeze(0), Cm.unsqueeze(0), D, dt_bias, state, None, y=L_.ptr(y), state_out=L_.ptr(out))
-        L_.call('gmt_selective_scan_step', ctypes.addressof(a), L_.ptr(active), L_.stream(), nbytes=float(8 * state.numel()))
+    out = _step_states(state, state_out, (Bt, Ch, N), torch.float32)
+    if torch.is_grad_enabled():
+        _no_grad_only('selective_scan_step', x, dt, A, B, C, state, D, z, dt_bias, state_out)
+    active = _active(active, Bt, x)
+    x, dt, B, C = time_major(x), time_major(dt), time_major(B), time_major(C)
+    A, D, dt_bias = _whole(A), _whole(D), _whole(dt_bias)
+    z = None if z is None else time_major(z)
+    Bp, Cp = _map_pitches(B, 1), _map_pitches(C, 1)
+    with on(dev):
+        y = x.new_empty((Bt, Ch))
+        a = L_.ScanArgs(x=x.data_ptr(), dt=dt.data_ptr(), z=_at(z), Bm=B.data_ptr(), Cm=C.data_ptr(), A=A.data_ptr(), D=_at(D),
+                        dt_bias=_at(dt_bias), state=state.data_ptr(), y=y.data_ptr(), state_out=out.data_ptr(), x_b=x.stride()[0],
+                        dt_b=dt.stride()[0], z_b=0 if z is None else z.stride()[0], B_b=Bp[1], B_g=Bp[2], C_b=Cp[1], C_g=Cp[2],
+                        L=1, B=Bt, C=Ch, N=N, G=1 if B.dim() == 2 else B.shape[1], bf16=x.dtype == torch.bfloat16)
+        L_.call('gmt_selective_scan_step', ctypes.addressof(a), _at(active), L_.stream(), nbytes=8.0 * Bt * Ch * N)
     torch.autograd.graph.increment_version(out)
     return y
