@@ -18,77 +18,79 @@ using namespace gmt_ssm;
 
 constexpr int BLK = 32;
 
-template <class T, int V> __device__ __forceinline__ void load_vec(const typename T::raw* p, float (&o)[V])
-{
-    if constexpr (V == 1) o[0] = to_f(*p);
-    else {
-        typedef typename T::raw vec __attribute__((ext_vector_type(V)));
-        const vec v = *reinterpret_cast<const vec*>(p);
-#pragma unroll
-        for (int i = 0; i < V; ++i) o[i] = to_f((typename T::raw)v[i]);
-    }
-}
+// several elements at any address: one memory instruction, which need not be aligned on this hardware
+template <class V, class E> __device__ __forceinline__ V load_any(const E* p) { V v; __builtin_memcpy(&v, p, sizeof(V)); return v; }
+template <class V, class E> __device__ __forceinline__ void store_any(E* p, const V& v) { __builtin_memcpy(p, &v, sizeof(V)); }
 
-// 32 / V lanes share a block: V = 16 bytes of elements where the layout allows, else 1
-template <class T, int V>
+// A lane takes 16 bytes of elements, 32 / V lanes share a block; a row's last lanes take what is left of it one by one.
+// Bound by HBM: 210 MB of bf16 in, 105 MB of codes out, and back (200 x 512 rows of 512 channels): 33 and 26 us.
+template <class T>
 __global__ __launch_bounds__(256)
 void pack_kernel(const typename T::raw* __restrict__ x, long long x_t, long long x_b, signed char* __restrict__ codes,
                  unsigned char* __restrict__ scale, long long rows, int B, int C, int nb)
 {
-    constexpr int LPB = BLK / V;
+    using R = typename T::raw;
+    constexpr int V = 16 / sizeof(R), LPB = BLK / V;
+    typedef R vec __attribute__((ext_vector_type(V)));
+    typedef signed char qvec __attribute__((ext_vector_type(V)));
     const long long total = rows * nb * LPB, step = (long long)gridDim.x * 256;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += step) {
         const long long blk = i / LPB, row = blk / nb;
         const int part = (int)(i % LPB), c = (int)(blk % nb) * BLK + part * V;
-        const bool in = c < C;                          // (C % V == 0)
-        float v[V] = {};
-        if (in) load_vec<T, V>(x + row / B * x_t + row % B * x_b + c, v);
+        const R* p = x + row / B * x_t + row % B * x_b + c;
+        vec v = {};
+        if (c + V <= C) v = load_any<vec>(p);
+        else {
+#pragma unroll
+            for (int k = 0; k < V; ++k) if (c + k < C) v[k] = p[k];
+        }
         unsigned m = 0;                                 // largest magnitude by its bits: NaN > infinity > numbers
 #pragma unroll
-        for (int k = 0; k < V; ++k) m = max(m, __float_as_uint(v[k]) & 0x7fffffffu);
+        for (int k = 0; k < V; ++k) m = max(m, __float_as_uint(to_f((R)v[k])) & 0x7fffffffu);
 #pragma unroll
         for (int o = 1; o < LPB; o <<= 1) m = max(m, (unsigned)__shfl_xor((int)m, o, 64));
         int e = (int)(m >> 23) - 133 + ((m & 0x7fffffu) > 0x7e0000u);
         e = min(max(e, -118), 121);
         const bool bad = m >= 0x7f800000u;
         const float inv = __uint_as_float((unsigned)(127 - e) << 23);
-        if (in) {
-            signed char q[V];
+        qvec q;
 #pragma unroll
-            for (int k = 0; k < V; ++k) q[k] = bad ? 0 : (signed char)(int)fminf(fmaxf(rintf(v[k] * inv), -127.f), 127.f);
-            if constexpr (V == 1) codes[row * C + c] = q[0];
-            else {
-                typedef signed char vec __attribute__((ext_vector_type(V)));
-                vec o;
+        for (int k = 0; k < V; ++k) q[k] = bad ? 0 : (signed char)(int)fminf(fmaxf(rintf(to_f((R)v[k]) * inv), -127.f), 127.f);
+        signed char* o = codes + row * C + c;
+        if (c + V <= C) store_any(o, q);
+        else {
 #pragma unroll
-                for (int k = 0; k < V; ++k) o[k] = q[k];
-                *reinterpret_cast<vec*>(codes + row * C + c) = o;
-            }
-            if (part == 0) scale[blk] = bad ? 255 : (unsigned char)(e + 127);
+            for (int k = 0; k < V; ++k) if (c + k < C) o[k] = q[k];
         }
+        if (part == 0) scale[blk] = bad ? 255 : (unsigned char)(e + 127);
     }
 }
 
-template <class T, int V>
+template <class T>
 __global__ __launch_bounds__(256)
 void unpack_kernel(const signed char* __restrict__ codes, const unsigned char* __restrict__ scale, typename T::raw* __restrict__ out,
                    long long rows, int C, int nb)
 {
-    const int cv = C / V;
+    using R = typename T::raw;
+    constexpr int V = 16 / sizeof(R);
+    typedef R vec __attribute__((ext_vector_type(V)));
+    typedef signed char qvec __attribute__((ext_vector_type(V)));
+    const int cv = (C + V - 1) / V;
     const long long total = rows * cv, step = (long long)gridDim.x * 256;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += step) {
         const long long row = i / cv;
         const int c = (int)(i % cv) * V;
         const unsigned char s = scale[row * nb + c / BLK];
-        if constexpr (V == 1) out[i] = from_f<T>(to_f(Q8::raw{codes[i], s}));
-        else {
-            typedef signed char qvec __attribute__((ext_vector_type(V)));
-            typedef typename T::raw vec __attribute__((ext_vector_type(V)));
-            const qvec q = *reinterpret_cast<const qvec*>(codes + i * V);
-            vec o;
+        const signed char* p = codes + row * C + c;
+        R* o = out + row * C + c;
+        if (c + V <= C) {
+            const qvec q = load_any<qvec>(p);
+            vec v;
 #pragma unroll
-            for (int k = 0; k < V; ++k) o[k] = from_f<T>(to_f(Q8::raw{(signed char)q[k], s}));
-            *reinterpret_cast<vec*>(out + i * V) = o;
+            for (int k = 0; k < V; ++k) v[k] = from_f<T>(to_f(Q8::raw{(signed char)q[k], s}));
+            store_any(o, v);
+        } else {
+            for (int k = 0; c + k < C; ++k) o[k] = from_f<T>(to_f(Q8::raw{p[k], s}));
         }
     }
 }
@@ -122,15 +124,14 @@ __device__ __forceinline__ bf16x8 tr_frag(const char* img, int col0, int s, int 
 // the high halves of two floats as a pair of bf16 (cut, not rounded)
 __device__ __forceinline__ unsigned hi_pair(float a, float b) { return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u); }
 
-// T: type of dY; YV: dY is read 4 elements at a time (16 or 8 bytes); XV: codes 16 at a time
-template <class T, bool YV, bool XV>
-__global__ __launch_bounds__(256, 2)
+// T: type of dY
+template <class T>
+__global__ __launch_bounds__(256, 3)
 void wgrad8_kernel(const typename T::raw* __restrict__ dY, long long ldy, const signed char* __restrict__ codes,
-                   const unsigned char* __restrict__ scale, float* __restrict__ out, long long R, int N, int I, int ks, long long rows_per_slab,
-                   int want_db)
+                   const unsigned char* __restrict__ scale, float* __restrict__ out, long long R, int N, int I, int ks, int want_db)
 {
     constexpr int PL = __is_same(T, F32) ? 3 : 1;
-    __shared__ __align__(16) char lds[2][(PL + 1) * WG_IMG];
+    __shared__ __align__(16) char lds[(PL + 1) * WG_IMG];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wp = wave >> 1, wq = wave & 1;
     const int n_t = (N + WG_T - 1) / WG_T, i_t = (I + WG_T - 1) / WG_T, tiles = n_t * i_t;
@@ -138,42 +139,56 @@ void wgrad8_kernel(const typename T::raw* __restrict__ dY, long long ldy, const 
     const int rest = blockIdx.x >> 3, tile = rest % tiles, slab = rest / tiles * 8 + (blockIdx.x & 7);
     if (slab >= ks) return;
     const int n0 = tile % n_t * WG_T, i0 = tile / n_t * WG_T;
-    const long long r0 = slab * rows_per_slab, r1 = min(r0 + rows_per_slab, R);
+    const long long r1 = R;
+    const int all = (int)((R + WG_K - 1) / WG_K);       // stages, dealt to the slabs in turn
     const int nb = (I + BLK - 1) / BLK;
 
     const int yc = (tid & 31) * 4, yr = tid >> 5;       // dY: 4 columns, rows yr + 8 j
     const int xc = (tid & 7) * 16, xr = tid >> 3;       // codes: 16 columns of one row (half a block)
-    struct Stage { float y[4][4]; signed char q[16]; unsigned char s; };
+    typedef typename T::raw yvec __attribute__((ext_vector_type(4)));
+    typedef signed char qvec __attribute__((ext_vector_type(16)));
+    struct Stage { yvec y[4]; qvec q; unsigned char s; };
     float colsum[4] = {};
+    const bool y_in = n0 + yc + 4 <= N, x_in = i0 + xc + 16 <= I;
+    // uniform base of a stage + 32-bit offsets of the thread (launch_wgrad8 checks that they fit)
+    unsigned yoff[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) yoff[k] = (unsigned)((yr + 8 * k) * (int)ldy + yc) * sizeof(typename T::raw);
+    const unsigned qoff = xr * I + xc, soff = xr * nb + xc / BLK;
+    const bool inner = n0 + WG_T <= N && i0 + WG_T <= I;
     auto request = [&](Stage& st, long long r) {
+        const char* yp = uniform(reinterpret_cast<const char*>(dY + r * ldy + n0));
+        const signed char* qp = uniform(codes + r * I + i0);
+        const unsigned char* sp = uniform(scale + r * nb + i0 / BLK);
+        if (inner && r + WG_K <= r1) {                  // (uniform) a whole stage inside the matrices
+#pragma unroll
+            for (int j = 0; j < 4; ++j) st.y[j] = load_any<yvec>(reinterpret_cast<const typename T::raw*>(yp + yoff[j]));
+            st.q = load_any<qvec>(qp + qoff);
+            st.s = sp[soff];
+            return;
+        }
+        const int left = (int)(r1 - r < WG_K ? r1 - r : WG_K);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const long long rr = r + yr + 8 * j;
-            const bool in = rr < r1;
-            const typename T::raw* p = dY + rr * ldy + n0 + yc;
-            if constexpr (YV) {
+            const typename T::raw* p = reinterpret_cast<const typename T::raw*>(yp + yoff[j]);
+            st.y[j] = yvec{};
+            if (yr + 8 * j < left) {
+                if (y_in) st.y[j] = load_any<yvec>(p);
+                else {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) st.y[j][k] = 0.f;
-                if (in && n0 + yc < N) load_vec<T, 4>(p, st.y[j]);
-            } else {
-#pragma unroll
-                for (int k = 0; k < 4; ++k) st.y[j][k] = in && n0 + yc + k < N ? to_f(p[k]) : 0.f;
+                    for (int k = 0; k < 4; ++k) if (n0 + yc + k < N) st.y[j][k] = p[k];
+                }
             }
         }
-        const long long rr = r + xr;
-        const bool in = rr < r1 && i0 + xc < I;
         st.s = 127;
-        if (in) st.s = scale[rr * nb + (i0 + xc) / BLK];
-        const signed char* p = codes + rr * I + i0 + xc;
-        typedef signed char qvec __attribute__((ext_vector_type(16)));
-        if constexpr (XV) {
-            qvec v = {};
-            if (in) v = *reinterpret_cast<const qvec*>(p);
+        st.q = qvec{};
+        if (xr < left && i0 + xc < I) {
+            st.s = sp[soff];
+            if (x_in) st.q = load_any<qvec>(qp + qoff);
+            else {
 #pragma unroll
-            for (int k = 0; k < 16; ++k) st.q[k] = v[k];
-        } else {
-#pragma unroll
-            for (int k = 0; k < 16; ++k) st.q[k] = in && i0 + xc + k < I ? p[k] : (signed char)0;
+                for (int k = 0; k < 16; ++k) if (i0 + xc + k < I) st.q[k] = qp[qoff + k];
+            }
         }
     };
     auto put = [&](const Stage& st, char* img) {
@@ -182,7 +197,7 @@ void wgrad8_kernel(const typename T::raw* __restrict__ dY, long long ldy, const 
             const int row = yr + 8 * j;
             float v[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) { v[k] = st.y[j][k]; colsum[k] += v[k]; }
+            for (int k = 0; k < 4; ++k) { v[k] = to_f((typename T::raw)st.y[j][k]); colsum[k] += v[k]; }
 #pragma unroll
             for (int pl = 0; pl < PL; ++pl) {
                 uint2 w = make_uint2(hi_pair(v[0], v[1]), hi_pair(v[2], v[3]));
@@ -210,13 +225,9 @@ void wgrad8_kernel(const typename T::raw* __restrict__ dY, long long ldy, const 
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
-    Stage st;
-    const int nk = r1 > r0 ? (int)((r1 - r0 + WG_K - 1) / WG_K) : 0;
-    if (nk > 0) { request(st, r0); put(st, lds[0]); }
-    __syncthreads();
-    for (int t = 0; t < nk; ++t) {
-        if (t + 1 < nk) request(st, r0 + (long long)(t + 1) * WG_K);
-        const char* img = lds[t & 1];
+    const int nk = (all - slab + ks - 1) / ks;
+    auto at = [&](int t) { return (long long)(slab + t * ks) * WG_K; };
+    auto contract = [&](const char* img) {
 #pragma unroll
         for (int s = 0; s < WG_K / 16; ++s) {
             bf16x8 q[2];
@@ -233,8 +244,16 @@ void wgrad8_kernel(const typename T::raw* __restrict__ dY, long long ldy, const 
                     for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(p[i], q[j], acc[i][j], 0, 0, 0);
             }
         }
-        if (t + 1 < nk) put(st, lds[(t + 1) & 1]);
-        __syncthreads();                                // stage t + 1 is written; everybody is done with stage t
+    };
+    Stage st;
+    if (nk > 0) { request(st, at(0)); put(st, lds); }
+    __syncthreads();
+    for (int t = 0; t < nk; ++t) {
+        if (t + 1 < nk) request(st, at(t + 1));
+        contract(lds);
+        __syncthreads();                                // everybody is done with stage t
+        if (t + 1 < nk) put(st, lds);
+        __syncthreads();                                // stage t + 1 is written
     }
     const int lo = lane & 31, hi = lane >> 5;
     float* slab_out = out + (long long)slab * ((long long)N * I + N);
@@ -252,8 +271,7 @@ void wgrad8_kernel(const typename T::raw* __restrict__ dY, long long ldy, const 
         }
     }
     if (want_db && i0 == 0) {                           // (uniform) column sums: 8 row groups of 32 threads x 4 columns
-        float (*sum)[WG_T] = reinterpret_cast<float (*)[WG_T]>(lds[0]);
-        __syncthreads();
+        float (*sum)[WG_T] = reinterpret_cast<float (*)[WG_T]>(lds);
 #pragma unroll
         for (int k = 0; k < 4; ++k) sum[yr][yc + k] = colsum[k];
         __syncthreads();
@@ -266,31 +284,25 @@ void wgrad8_kernel(const typename T::raw* __restrict__ dY, long long ldy, const 
     }
 }
 
-// Slabs: two workgroups a CU in all, slabs of four stages or more
-void wgrad8_split(long long R, int N, int I, int& ks, long long& rows)
+// Slabs of four stages or more, three workgroups a CU in all (R=524288 N=512 I=128 fp32: three with one LDS image each 324 us, two
+// with two images, which need one barrier a stage, 342 us).  Alone, the contraction takes 200 us of these and the loads and
+// conversions 230 us; together the clock falls from 2.4 to 1.8 GHz.
+int wgrad8_slabs(long long R, int N, int I)
 {
     const long long tiles = (long long)((N + WG_T - 1) / WG_T) * ((I + WG_T - 1) / WG_T);
-    long long k = (512 + tiles - 1) / tiles;
+    long long k = (768 + tiles - 1) / tiles;
     const long long most = (R + 4 * WG_K - 1) / (4 * WG_K);
     if (k > most) k = most;
-    if (k < 1) k = 1;
-    rows = ((R + k - 1) / k + WG_K - 1) / WG_K * WG_K;
-    ks = (int)((R + rows - 1) / rows);
+    return (int)(k < 1 ? 1 : k);
 }
 
 template <class T> int launch_wgrad8(const void* dY, long long ldy, const signed char* codes, const unsigned char* scale, float* slab, long long R,
-                                     int N, int I, int ks, long long rows, int want_db, hipStream_t stream)
+                                     int N, int I, int ks, int want_db, hipStream_t stream)
 {
-    const bool yv = N % 4 == 0 && ldy % 4 == 0 && ((uintptr_t)dY % (4 * sizeof(typename T::raw))) == 0;
-    const bool xv = I % 16 == 0 && ((uintptr_t)codes & 15) == 0;
     const long long tiles = (long long)((N + WG_T - 1) / WG_T) * ((I + WG_T - 1) / WG_T), grid = 8 * tiles * ((ks + 7) / 8);
-    if (grid >= (1LL << 24)) return GMT_ERR_UNSUPPORTED;
-#define GMT_WG(YV, XV)                                                                                                         \
-    hipLaunchKernelGGL((wgrad8_kernel<T, YV, XV>), dim3((unsigned)grid), dim3(256), 0, stream, (const typename T::raw*)dY, ldy, codes, \
-                       scale, slab, R, N, I, ks, rows, want_db)
-    if (yv) { if (xv) GMT_WG(true, true); else GMT_WG(true, false); }
-    else { if (xv) GMT_WG(false, true); else GMT_WG(false, false); }
-#undef GMT_WG
+    if (grid >= (1LL << 24) || ldy >= (1LL << 24) || I >= (1 << 24)) return GMT_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL(wgrad8_kernel<T>, dim3((unsigned)grid), dim3(256), 0, stream, (const typename T::raw*)dY, ldy, codes, scale, slab, R, N, I,
+                       ks, want_db);
     GMT_LAUNCH_CHECK();
     return GMT_OK;
 }
@@ -301,17 +313,11 @@ extern "C" int gmt_ckpt8_pack(const void* x, long long x_t, long long x_b, signe
                               int C, int bf16, hipStream_t stream)
 {
     GMT_CHECK_ARG(x && codes && scale && T > 0 && B > 0 && C > 0);
-    const int esz = bf16 ? 2 : 4, V = 16 / esz, nb = (C + BLK - 1) / BLK;
-    const bool vec = C % V == 0 && x_t % V == 0 && x_b % V == 0 && ((uintptr_t)x & 15) == 0 && ((uintptr_t)codes % V) == 0;
+    const int V = bf16 ? 8 : 4, nb = (C + BLK - 1) / BLK;
     const long long rows = T * B;
-    const int grid = gmt_grid_1d(rows * nb * (vec ? BLK / V : BLK), 256, 256 * 16);
-    if (bf16) {
-        if (vec) hipLaunchKernelGGL((pack_kernel<B16, 8>), dim3(grid), dim3(256), 0, stream, (const unsigned short*)x, x_t, x_b, codes, scale, rows, B, C, nb);
-        else hipLaunchKernelGGL((pack_kernel<B16, 1>), dim3(grid), dim3(256), 0, stream, (const unsigned short*)x, x_t, x_b, codes, scale, rows, B, C, nb);
-    } else {
-        if (vec) hipLaunchKernelGGL((pack_kernel<F32, 4>), dim3(grid), dim3(256), 0, stream, (const float*)x, x_t, x_b, codes, scale, rows, B, C, nb);
-        else hipLaunchKernelGGL((pack_kernel<F32, 1>), dim3(grid), dim3(256), 0, stream, (const float*)x, x_t, x_b, codes, scale, rows, B, C, nb);
-    }
+    const int grid = gmt_grid_1d(rows * nb * (BLK / V), 256, 256 * 16);
+    if (bf16) hipLaunchKernelGGL(pack_kernel<B16>, dim3(grid), dim3(256), 0, stream, (const unsigned short*)x, x_t, x_b, codes, scale, rows, B, C, nb);
+    else hipLaunchKernelGGL(pack_kernel<F32>, dim3(grid), dim3(256), 0, stream, (const float*)x, x_t, x_b, codes, scale, rows, B, C, nb);
     GMT_LAUNCH_CHECK();
     return GMT_OK;
 }
@@ -320,15 +326,9 @@ extern "C" int gmt_ckpt8_unpack(const signed char* codes, const unsigned char* s
 {
     GMT_CHECK_ARG(out && codes && scale && rows > 0 && C > 0);
     const int V = bf16 ? 8 : 4, nb = (C + BLK - 1) / BLK;
-    const bool vec = C % V == 0 && ((uintptr_t)out & 15) == 0 && ((uintptr_t)codes % V) == 0;
-    const int grid = gmt_grid_1d(rows * (vec ? C / V : C), 256, 256 * 16);
-    if (bf16) {
-        if (vec) hipLaunchKernelGGL((unpack_kernel<B16, 8>), dim3(grid), dim3(256), 0, stream, codes, scale, (unsigned short*)out, rows, C, nb);
-        else hipLaunchKernelGGL((unpack_kernel<B16, 1>), dim3(grid), dim3(256), 0, stream, codes, scale, (unsigned short*)out, rows, C, nb);
-    } else {
-        if (vec) hipLaunchKernelGGL((unpack_kernel<F32, 4>), dim3(grid), dim3(256), 0, stream, codes, scale, (float*)out, rows, C, nb);
-        else hipLaunchKernelGGL((unpack_kernel<F32, 1>), dim3(grid), dim3(256), 0, stream, codes, scale, (float*)out, rows, C, nb);
-    }
+    const int grid = gmt_grid_1d(rows * ((C + V - 1) / V), 256, 256 * 16);
+    if (bf16) hipLaunchKernelGGL(unpack_kernel<B16>, dim3(grid), dim3(256), 0, stream, codes, scale, (unsigned short*)out, rows, C, nb);
+    else hipLaunchKernelGGL(unpack_kernel<F32>, dim3(grid), dim3(256), 0, stream, codes, scale, (float*)out, rows, C, nb);
     GMT_LAUNCH_CHECK();
     return GMT_OK;
 }
@@ -336,8 +336,7 @@ extern "C" int gmt_ckpt8_unpack(const signed char* codes, const unsigned char* s
 extern "C" int gmt_ckpt8_wgrad_workspace_floats(long long R, int N, int I, long long* floats_out)
 {
     GMT_CHECK_ARG(R > 0 && N > 0 && I > 0 && floats_out);
-    int ks; long long rows;
-    wgrad8_split(R, N, I, ks, rows);
+    const int ks = wgrad8_slabs(R, N, I);
     *floats_out = ks > 1 ? ks * ((long long)N * I + N) : 0;
     return GMT_OK;
 }
@@ -346,13 +345,12 @@ extern "C" int gmt_ckpt8_wgrad(const void* dY, long long ldy, const signed char*
                                int N, int I, int bf16, int want_db, float* workspace, long long workspace_floats, hipStream_t stream)
 {
     GMT_CHECK_ARG(dY && codes && scale && dW_db && R > 0 && N > 0 && I > 0 && ldy >= N);
-    int ks; long long rows;
-    wgrad8_split(R, N, I, ks, rows);
+    const int ks = wgrad8_slabs(R, N, I);
     const long long n = (long long)N * I + (want_db ? N : 0), pitch = (long long)N * I + N;
     if (ks > 1 && (!workspace || workspace_floats < ks * pitch)) return GMT_ERR_WORKSPACE;
     float* slab = ks > 1 ? workspace : dW_db;
-    const int rc = bf16 ? launch_wgrad8<B16>(dY, ldy, codes, scale, slab, R, N, I, ks, rows, want_db, stream)
-                        : launch_wgrad8<F32>(dY, ldy, codes, scale, slab, R, N, I, ks, rows, want_db, stream);
+    const int rc = bf16 ? launch_wgrad8<B16>(dY, ldy, codes, scale, slab, R, N, I, ks, want_db, stream)
+                        : launch_wgrad8<F32>(dY, ldy, codes, scale, slab, R, N, I, ks, want_db, stream);
     if (rc || ks == 1) return rc;
     return launch_slab_reduce(workspace, dW_db, n, pitch, ks, stream);
 }

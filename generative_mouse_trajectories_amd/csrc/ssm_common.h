@@ -46,6 +46,10 @@ __device__ __forceinline__ float softplus(float v, float& sig) {
 // silu(v) = v / (1 + exp(-v)).  exp(-v) overflows to inf below -88: rcp gives 0 and v * 0 = -0, the limit.
 __device__ __forceinline__ float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-v * LOG2E)); }
 
+// A pointer that is the same on all lanes, kept in scalar registers: `uniform(p) + 32-bit offset` is then one memory instruction
+// (otherwise the compiler adds the lane's offset first, in 64-bit vector arithmetic, and keeps the results).
+template <class P> __device__ __forceinline__ P* uniform(P* p) { asm("" : "+s"(p)); return p; }
+
 __device__ __forceinline__ int length_of(const int* lengths, int b, int L) {
     if (!lengths) return L;
     const int n = lengths[b];

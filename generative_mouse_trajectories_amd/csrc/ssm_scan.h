@@ -156,10 +156,6 @@ template <int PARTS> struct Lanes {
     __device__ __forceinline__ float sum(float v) const { if constexpr (PARTS == 1) return v; else return half32(v, v); }
 };
 
-// A pointer that is the same on all lanes, kept in scalar registers: `uniform(p) + 32-bit offset` is then one memory instruction
-// (otherwise the compiler adds the lane's offset first, in 64-bit vector arithmetic, and keeps the results).
-template <class P> __device__ __forceinline__ P* uniform(P* p) { asm("" : "+s"(p)); return p; }
-
 // One sequence of a row, as a lane sees it.  Uniform base of a step plus a 32-bit byte offset of the lane (its part's step and its
 // channel): the scalar-base form of the memory instructions, no 64-bit vector arithmetic.
 template <class T> struct Seq {
