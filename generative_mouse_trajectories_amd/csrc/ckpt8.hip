@@ -147,47 +147,45 @@ void wgrad8_kernel(const typename T::raw* __restrict__ dY, long long ldy, const 
     const int xc = (tid & 7) * 16, xr = tid >> 3;       // codes: 16 columns of one row (half a block)
     typedef typename T::raw yvec __attribute__((ext_vector_type(4)));
     typedef signed char qvec __attribute__((ext_vector_type(16)));
+    typedef yvec yvec_any __attribute__((aligned(sizeof(typename T::raw))));        // loads need not be aligned
+    typedef qvec qvec_any __attribute__((aligned(1)));
     struct Stage { yvec y[4]; qvec q; unsigned char s; };
     float colsum[4] = {};
     const bool y_in = n0 + yc + 4 <= N, x_in = i0 + xc + 16 <= I;
     // uniform base of a stage + 32-bit offsets of the thread (launch_wgrad8 checks that they fit)
-    unsigned yoff[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) yoff[k] = (unsigned)((yr + 8 * k) * (int)ldy + yc) * sizeof(typename T::raw);
+    const unsigned yoff = (unsigned)(yr * (int)ldy + yc) * sizeof(typename T::raw);
     const unsigned qoff = xr * I + xc, soff = xr * nb + xc / BLK;
     const bool inner = n0 + WG_T <= N && i0 + WG_T <= I;
     auto request = [&](Stage& st, long long r) {
-        const char* yp = uniform(reinterpret_cast<const char*>(dY + r * ldy + n0));
-        const signed char* qp = uniform(codes + r * I + i0);
-        const unsigned char* sp = uniform(scale + r * nb + i0 / BLK);
+        const Uniform qp = uniform(codes + r * I + i0), sp = uniform(scale + r * nb + i0 / BLK);
         if (inner && r + WG_K <= r1) {                  // (uniform) a whole stage inside the matrices
 #pragma unroll
-            for (int j = 0; j < 4; ++j) st.y[j] = load_any<yvec>(reinterpret_cast<const typename T::raw*>(yp + yoff[j]));
-            st.q = load_any<qvec>(qp + qoff);
-            st.s = sp[soff];
+            for (int j = 0; j < 4; ++j) st.y[j] = load_at<yvec_any>(uniform(dY + (r + 8 * j) * ldy + n0), yoff);
+            st.q = load_at<qvec_any>(qp, qoff);
+            st.s = load_at<unsigned char>(sp, soff);
             return;
         }
         const int left = (int)(r1 - r < WG_K ? r1 - r : WG_K);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const typename T::raw* p = reinterpret_cast<const typename T::raw*>(yp + yoff[j]);
+            const Uniform yp = uniform(dY + (r + 8 * j) * ldy + n0);
             st.y[j] = yvec{};
             if (yr + 8 * j < left) {
-                if (y_in) st.y[j] = load_any<yvec>(p);
+                if (y_in) st.y[j] = load_at<yvec_any>(yp, yoff);
                 else {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) if (n0 + yc + k < N) st.y[j][k] = p[k];
+                    for (int k = 0; k < 4; ++k) if (n0 + yc + k < N) st.y[j][k] = load_at<typename T::raw>(yp, yoff + k * sizeof(typename T::raw));
                 }
             }
         }
         st.s = 127;
         st.q = qvec{};
         if (xr < left && i0 + xc < I) {
-            st.s = sp[soff];
-            if (x_in) st.q = load_any<qvec>(qp + qoff);
+            st.s = load_at<unsigned char>(sp, soff);
+            if (x_in) st.q = load_at<qvec_any>(qp, qoff);
             else {
 #pragma unroll
-                for (int k = 0; k < 16; ++k) if (i0 + xc + k < I) st.q[k] = qp[qoff + k];
+                for (int k = 0; k < 16; ++k) if (i0 + xc + k < I) st.q[k] = load_at<signed char>(qp, qoff + k);
             }
         }
     };
@@ -284,9 +282,8 @@ void wgrad8_kernel(const typename T::raw* __restrict__ dY, long long ldy, const 
     }
 }
 
-// Slabs of four stages or more, three workgroups a CU in all (R=524288 N=512 I=128 fp32: three with one LDS image each 324 us, two
-// with two images, which need one barrier a stage, 342 us).  Alone, the contraction takes 200 us of these and the loads and
-// conversions 230 us; together the clock falls from 2.4 to 1.8 GHz.
+// Slabs of four stages or more, three workgroups a CU in all (R=524288 N=512 I=128 fp32, one box: three with one LDS image each
+// 314 us, two 359 us, two with two images, which need one barrier a stage, 362 us).
 int wgrad8_slabs(long long R, int N, int I)
 {
     const long long tiles = (long long)((N + WG_T - 1) / WG_T) * ((I + WG_T - 1) / WG_T);

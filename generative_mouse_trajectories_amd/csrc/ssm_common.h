@@ -46,9 +46,21 @@ __device__ __forceinline__ float softplus(float v, float& sig) {
 // silu(v) = v / (1 + exp(-v)).  exp(-v) overflows to inf below -88: rcp gives 0 and v * 0 = -0, the limit.
 __device__ __forceinline__ float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-v * LOG2E)); }
 
-// A pointer that is the same on all lanes, kept in scalar registers: `uniform(p) + 32-bit offset` is then one memory instruction
-// (otherwise the compiler adds the lane's offset first, in 64-bit vector arithmetic, and keeps the results).
-template <class P> __device__ __forceinline__ P* uniform(P* p) { asm("" : "+s"(p)); return p; }
+// A pointer to device memory that is the same on all lanes, kept in scalar registers: `at(uniform(p), 32-bit byte offset)` is then
+// one global memory instruction (otherwise the compiler adds the lane's offset first, in 64-bit vector arithmetic, and keeps the
+// results).
+typedef const __attribute__((address_space(1))) char* Uniform;
+__device__ __forceinline__ Uniform uniform(const void* p) {
+    Uniform g = (Uniform)p;
+    asm("" : "+s"(g));
+    return g;
+}
+template <class E> __device__ __forceinline__ E load_at(Uniform p, unsigned off) {
+    return *reinterpret_cast<const __attribute__((address_space(1))) E*>(p + off);
+}
+template <class E> __device__ __forceinline__ void store_at(Uniform p, unsigned off, E v) {
+    *(__attribute__((address_space(1))) E*)(p + off) = v;
+}
 
 __device__ __forceinline__ int length_of(const int* lengths, int b, int L) {
     if (!lengths) return L;

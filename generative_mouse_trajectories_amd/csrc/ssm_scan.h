@@ -184,20 +184,17 @@ template <class T, int PARTS> struct Own {
         for (int j = 0; j < OWN; ++j) {
             const int t = min(tc + j * PARTS, te - 1);
             const bool all = t + PARTS <= te;           // (uniform) every part's step exists
-            get(j, uniform(q.p + (long long)t * q.pt), all ? q.off : q.off0, __is_same(T, Q8) ? uniform(q.sp + (long long)t * q.spt) : nullptr,
-                all ? q.soff : q.soff0);
+            const Uniform p = uniform(q.p + (long long)t * q.pt);
+            if constexpr (__is_same(T, Q8)) {
+                v[j].q = load_at<signed char>(p, all ? q.off : q.off0);
+                v[j].s = load_at<unsigned char>(uniform(q.sp + (long long)t * q.spt), all ? q.soff : q.soff0);
+            } else v[j] = load_at<typename T::raw>(p, all ? q.off : q.off0);
         }
-    }
-    __device__ __forceinline__ void get(int j, const char* p, unsigned off, const char* sp, unsigned soff) {
-        if constexpr (__is_same(T, Q8)) {
-            v[j].q = *reinterpret_cast<const signed char*>(p + off);
-            v[j].s = *reinterpret_cast<const unsigned char*>(sp + soff);
-        } else v[j] = *reinterpret_cast<const typename T::raw*>(p + off);
     }
 };
 // the same for an output [L][B][C]
 template <class M> __device__ __forceinline__ void put_out(typename M::raw* base, long long uniform_elem, unsigned off_bytes, float v) {
-    *reinterpret_cast<typename M::raw*>(uniform(reinterpret_cast<char*>(base + uniform_elem)) + off_bytes) = from_f<M>(v);
+    store_at<typename M::raw>(uniform(base + uniform_elem), off_bytes, from_f<M>(v));
 }
 
 // NS floats of a channel's row, states n0 .. n0 + NS - 1 (state buffers [B][C][N], A [C][N]) <-> registers, zero-padded
@@ -229,13 +226,13 @@ template <int NP, int NS> __device__ __forceinline__ void load_kept(const float*
 {
     const char* k = reinterpret_cast<const char*>(p + (slot * B + b) * NP * C);
 #pragma unroll
-    for (int n = 0; n < NS; ++n) h[n] = *reinterpret_cast<const float*>(uniform(k + (long long)n * C * 4) + off);
+    for (int n = 0; n < NS; ++n) h[n] = load_at<float>(uniform(k + (long long)n * C * 4), off);
 }
 template <int NP, int NS> __device__ __forceinline__ void store_kept(float* p, long long slot, int B, int b, int C, unsigned off, const float (&h)[NS])
 {
     char* k = reinterpret_cast<char*>(p + (slot * B + b) * NP * C);
 #pragma unroll
-    for (int n = 0; n < NS; ++n) *reinterpret_cast<float*>(uniform(k + (long long)n * C * 4) + off) = h[n];
+    for (int n = 0; n < NS; ++n) store_at<float>(uniform(k + (long long)n * C * 4), off, h[n]);
 }
 
 // The chunk's B (or C) as fp32 [CH][NP] in LDS, by all threads of the workgroup: request() one chunk ahead, put() behind the wait.
@@ -243,13 +240,13 @@ template <class M, int NP> struct MapTile {
     static constexpr int PER = CH * NP / 64;            // (one wave; wider workgroups need fewer)
     typename M::raw v[PER];
     __device__ __forceinline__ void request(const typename M::raw* p, int pt, int t0, int t1, int N) {
-        const char* q = uniform(reinterpret_cast<const char*>(p + (long long)t0 * pt));
+        const Uniform q = uniform(p + (long long)t0 * pt);
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
             const int i = threadIdx.x + j * blockDim.x, s = i / NP, n = i % NP;
             v[j] = from_f<M>(0.f);
             if (s < CH && n < N && t0 + s < t1)
-                v[j] = *reinterpret_cast<const typename M::raw*>(q + (unsigned)((s * pt + n) * (int)sizeof(typename M::raw)));
+                v[j] = load_at<typename M::raw>(q, (unsigned)((s * pt + n) * (int)sizeof(typename M::raw)));
         }
     }
     __device__ __forceinline__ void put(float* lds) const {

@@ -196,7 +196,7 @@ void scan_bwd_kernel(ScanArgs<T, M> a)
         for (; k >= 0; --k) {
             const int tc = t0 + k * CH;
             float h[CH + 1][NS], ex[KE ? KE : 1][NS];
-            float xv[OWN], st[OWN], sig[OWN], d[OWN], dyv[OWN], zv[OWN], out[OWN], gBk[OWN], qAk[OWN];
+            float xv[OWN], st[OWN], sig[OWN], d[OWN], dzf[OWN], out[OWN], gBk[OWN], qAk[OWN];        // dzf: dy silu'(z)
 #pragma unroll
             for (int j = 0; j < OWN; ++j) {
                 const bool live = tc + j * PARTS + ln.part < te;        // behind the row's end: a step of 0 with no adjoint of its own
@@ -204,8 +204,12 @@ void scan_bwd_kernel(ScanArgs<T, M> a)
                 const float v = softplus(to_f(dr.v[j]) + bias, sig[j]);
                 st[j] = live ? v : 0.f;
                 sig[j] = live ? sig[j] : 0.f;
-                dyv[j] = d[j] = live && on ? to_f(yr.v[j]) : 0.f;
-                if (GATED) { zv[j] = live ? to_f(zr.v[j]) : 0.f; d[j] *= zv[j] * sigmoid(zv[j]); }
+                d[j] = live && on ? to_f(yr.v[j]) : 0.f;
+                if (GATED) {
+                    const float zv = live ? to_f(zr.v[j]) : 0.f, sz = sigmoid(zv);
+                    dzf[j] = d[j] * sz * fmaf(zv, 1.0f - sz, 1.0f);
+                    d[j] *= zv * sz;
+                }
                 out[j] = gBk[j] = qAk[j] = 0.f;
             }
 #pragma unroll
@@ -239,12 +243,9 @@ void scan_bwd_kernel(ScanArgs<T, M> a)
                 }
                 if (GATED) {
 #pragma unroll
-                    for (int j = 0; j < OWN; ++j) {
-                        const float sz = sigmoid(zv[j]);
+                    for (int j = 0; j < OWN; ++j)
                         if (tc + j * PARTS + ln.part < t1 && on)
-                            put_out<M>(a.dz, ((long long)(tc + j * PARTS) * a.B + b) * a.C, ooff,
-                                       dyv[j] * fmaf(Dc, xv[j], out[j]) * sz * fmaf(zv[j], 1.0f - sz, 1.0f));
-                    }
+                            put_out<M>(a.dz, ((long long)(tc + j * PARTS) * a.B + b) * a.C, ooff, dzf[j] * fmaf(Dc, xv[j], out[j]));
                     step_fence();
                 }
 #pragma unroll
