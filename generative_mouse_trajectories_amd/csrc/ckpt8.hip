@@ -155,10 +155,13 @@ void wgrad8_kernel(const typename T::raw* __restrict__ dY, long long ldy, const 
     // uniform base of a stage + 32-bit offsets of the thread (launch_wgrad8 checks that they fit)
     const unsigned yoff = (unsigned)(yr * (int)ldy + yc) * sizeof(typename T::raw);
     const unsigned qoff = xr * I + xc, soff = xr * nb + xc / BLK;
-    const bool inner = n0 + WG_T <= N && i0 + WG_T <= I;
     auto request = [&](Stage& st, long long r) {
         const Uniform qp = uniform(codes + r * I + i0), sp = uniform(scale + r * nb + i0 / BLK);
-        if (inner && r + WG_K <= r1) {                  // (uniform) a whole stage inside the matrices
+        // (uniform) Whole rows of tiles whose last element lies within the buffers.  Beyond column N or I of a row that reads the next
+        // row (or what lies between rows): it ends in rows and columns of the tile that are not stored.
+        const long long last = r + WG_K - 1;
+        if (last < r1 && last * ldy + n0 + WG_T <= (R - 1) * ldy + N && last * I + i0 + WG_T <= R * I &&
+            last * nb + i0 / BLK + WG_T / BLK <= R * nb) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) st.y[j] = load_at<yvec_any>(uniform(dY + (r + 8 * j) * ldy + n0), yoff);
             st.q = load_at<qvec_any>(qp, qoff);

@@ -72,7 +72,7 @@ def pack(x: torch.Tensor) -> Ckpt8:
         codes = x.new_empty(x.shape, dtype=torch.int8)
         exps = x.new_empty((*x.shape[:-1], (C + BLOCK - 1) // BLOCK), dtype=torch.uint8)
         L_.call('gmt_ckpt8_pack', x.data_ptr(), st, sb, codes.data_ptr(), exps.data_ptr(), T, B, C, int(x.dtype == torch.bfloat16),
-                L_.stream(), nbytes=float(x.numel() * (x.element_size() + 1)))
+                L_.stream_of(dev), nbytes=float(x.numel() * (x.element_size() + 1)))
     return Ckpt8(codes, exps, x.dtype)
 
 
@@ -95,7 +95,7 @@ def unpack(p: Ckpt8, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     with on(dev):
         out = p.codes.new_empty(p.codes.shape, dtype=dtype)
         L_.call('gmt_ckpt8_unpack', p.codes.data_ptr(), p.exponents.data_ptr(), out.data_ptr(), out.numel() // C, C,
-                int(dtype == torch.bfloat16), L_.stream(), nbytes=float(out.numel() * (out.element_size() + 1)))
+                int(dtype == torch.bfloat16), L_.stream_of(dev), nbytes=float(out.numel() * (out.element_size() + 1)))
     return out
 
 
@@ -123,6 +123,6 @@ def wgrad(dY: torch.Tensor, p: Ckpt8, want_db: bool = False) -> Tuple[torch.Tens
         ws = dY.new_empty(need.value, dtype=torch.float32)
         out = dY.new_empty(N * I + N, dtype=torch.float32)
         L_.call('gmt_ckpt8_wgrad', dY.data_ptr(), max(dY.stride(0), N), p.codes.data_ptr(), p.exponents.data_ptr(), out.data_ptr(), R,
-                N, I, int(dY.dtype == torch.bfloat16), int(want_db), L_.ptr(ws), need.value, L_.stream(),
+                N, I, int(dY.dtype == torch.bfloat16), int(want_db), L_.ptr(ws), need.value, L_.stream_of(dev),
                 label=f'wgrad8_N{N}_I{I}', flops=2.0 * R * N * I)
     return out[:N * I].view(N, I), (out[N * I:] if want_db else None)

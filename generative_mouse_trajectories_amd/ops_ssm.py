@@ -119,7 +119,7 @@ def _conv_forward(x, weight, bias, state, lengths, silu):
     y = x.new_empty(x.shape)
     last = x.new_empty((weight.shape[1] - 1, x.shape[1], x.shape[2]))
     a = _conv_args(x, weight, bias, state, lengths, silu, y=y.data_ptr(), state_out=last.data_ptr())
-    L_.call('gmt_causal_conv_fwd', ctypes.addressof(a), L_.stream(), nbytes=2.0 * x.numel() * x.element_size())
+    L_.call('gmt_causal_conv_fwd', ctypes.addressof(a), L_.stream_of(x.get_device()), nbytes=2.0 * x.numel() * x.element_size())
     return y, last
 
 
@@ -140,7 +140,8 @@ class CausalConvFn(torch.autograd.Function):
         shape, dtype, K = x.shape, ctx.dtype, weight.shape[1]
         if ctx.ckpt8:
             x = Ckpt8(x, exps, dtype)
-        with on(weight.get_device()):
+        dev = weight.get_device()
+        with on(dev):
             dy = weight.new_zeros(shape, dtype=dtype) if dy is None else time_major(dy)
             dlast = _whole(dlast)
             dx = weight.new_empty(shape, dtype=dtype)
@@ -153,7 +154,7 @@ class CausalConvFn(torch.autograd.Function):
             L_.call('gmt_causal_conv_bwd_workspace_floats', ctypes.addressof(a), ctypes.addressof(need), label='skip')
             ws = _space(need.value, weight)
             a.workspace, a.workspace_floats = _at(ws), need.value
-            L_.call('gmt_causal_conv_bwd', ctypes.addressof(a), L_.stream(), nbytes=3.0 * dx.numel() * dx.element_size())
+            L_.call('gmt_causal_conv_bwd', ctypes.addressof(a), L_.stream_of(dev), nbytes=3.0 * dx.numel() * dx.element_size())
         return dx, dparam[:K].t().contiguous(), (None if bias is None else dparam[K]), dstate, None, None, None
 
 
@@ -200,7 +201,7 @@ def causal_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor,
         y = x.new_empty((B, C))
         a = L_.ConvArgs(x=x.data_ptr(), w=weight.data_ptr(), bias=_at(bias), state=state.data_ptr(), y=y.data_ptr(), state_out=out.data_ptr(),
                         x_b=x.stride()[0], L=1, B=B, C=C, K=K, bf16=x.dtype == torch.bfloat16, silu=bool(silu))
-        L_.call('gmt_causal_conv_step', ctypes.addressof(a), _at(active), L_.stream(), nbytes=2.0 * K * B * C * x.element_size())
+        L_.call('gmt_causal_conv_step', ctypes.addressof(a), _at(active), L_.stream_of(dev), nbytes=2.0 * K * B * C * x.element_size())
     torch.autograd.graph.increment_version(out)
     return y
 
@@ -247,7 +248,7 @@ def _scan_forward(x, dt, A, B, C, D, z, dt_bias, state, lengths, keep):
     n_ck, n_fwd, _ = _workspace(a)
     ck, ws = _space(n_ck if keep else 0, A), _space(n_fwd, A)
     a.ck, a.workspace, a.workspace_floats = _at(ck), _at(ws), n_fwd
-    L_.call('gmt_selective_scan_fwd', ctypes.addressof(a), L_.stream(), nbytes=float((3 + (z is not None)) * x.numel() * x.element_size()))
+    L_.call('gmt_selective_scan_fwd', ctypes.addressof(a), L_.stream_of(x.get_device()), nbytes=float((3 + (z is not None)) * x.numel() * x.element_size()))
     return y, last, ck
 
 
@@ -273,7 +274,8 @@ class SelectiveScanFn(torch.autograd.Function):
         if ctx.ckpt8:
             x, dt = Ckpt8(x, xe, dtype), Ckpt8(dt, dte, dtype)
             z = None if z is None else Ckpt8(z, ze, dtype)
-        with on(A.get_device()):
+        dev = A.get_device()
+        with on(dev):
             dy = A.new_zeros(shape, dtype=dtype) if dy is None else time_major(dy)
             dlast = _whole(dlast)
             dx, ddt = A.new_empty(shape, dtype=dtype), A.new_empty(shape, dtype=dtype)
@@ -290,7 +292,7 @@ class SelectiveScanFn(torch.autograd.Function):
                 ck = _space(n_ck, A)
             ws = _space(n_bwd, A)
             a.ck, a.workspace, a.workspace_floats = ck.data_ptr(), _at(ws), n_bwd
-            L_.call('gmt_selective_scan_bwd', ctypes.addressof(a), L_.stream(),
+            L_.call('gmt_selective_scan_bwd', ctypes.addressof(a), L_.stream_of(dev),
                     nbytes=float((5 + 2 * (z is not None)) * dx.numel() * dx.element_size()))
         return (dx, ddt, dparam[:Ch * N].view(Ch, N), dB, dC, None if D is None else dparam[Ch * N:Ch * (N + 1)], dz,
                 None if dt_bias is None else dparam[Ch * (N + 1):], dstate, None, None)
@@ -362,6 +364,6 @@ def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: t
                         dt_bias=_at(dt_bias), state=state.data_ptr(), y=y.data_ptr(), state_out=out.data_ptr(), x_b=x.stride()[0],
                         dt_b=dt.stride()[0], z_b=0 if z is None else z.stride()[0], B_b=Bp[1], B_g=Bp[2], C_b=Cp[1], C_g=Cp[2],
                         L=1, B=Bt, C=Ch, N=N, G=1 if B.dim() == 2 else B.shape[1], bf16=x.dtype == torch.bfloat16)
-        L_.call('gmt_selective_scan_step', ctypes.addressof(a), _at(active), L_.stream(), nbytes=8.0 * Bt * Ch * N)
+        L_.call('gmt_selective_scan_step', ctypes.addressof(a), _at(active), L_.stream_of(dev), nbytes=8.0 * Bt * Ch * N)
     torch.autograd.graph.increment_version(out)
     return y
