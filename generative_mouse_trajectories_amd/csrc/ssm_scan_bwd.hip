@@ -8,7 +8,7 @@
 // operator at the values the checkpoints stand for).
 //
 // dB and dC are sums over lanes: 2 N values a step.  They leave by halving exchanges - a lane hands half of its values to its
-// partner and keeps the partner's other half, v_permlane16_swap then DPP - 38 instructions for 16 values over 32 lanes where 16
+// partner and keeps the partner's other half, by DPP and v_permlane16_swap - 32 instructions for 16 values over 32 lanes where 16
 // separate sums take 80.  The waves of a workgroup meet in LDS, workgroups of one group through slabs: no float atomics, results
 // do not depend on the order of execution.
 #include "ssm_scan.h"
@@ -28,18 +28,42 @@ template <int CTRL> __device__ __forceinline__ float half_dpp(float a, float b, 
     const float keep = upper ? b : a, send = upper ? a : b;
     return keep + dpp<CTRL>(send);
 }
+// The same for bits 3 and 2 of the lane, which are banks of four lanes that a DPP instruction can leave out: a + its partner on all
+// lanes, then b + its partner on the upper ones - two instructions a value instead of three.  The wait at the front is the one
+// that a DPP operand needs behind the instruction that wrote it, which the compiler does not see in here.
+__device__ __forceinline__ void half_rows8(float& a0, float& a1, float& a2, float& a3, float b0, float b1, float b2, float b3) {
+    asm("s_nop 1\n\t"
+        "v_add_f32_dpp %0, %0, %0 row_ror:8 row_mask:0xf bank_mask:0xf\n\t"
+        "v_add_f32_dpp %1, %1, %1 row_ror:8 row_mask:0xf bank_mask:0xf\n\t"
+        "v_add_f32_dpp %2, %2, %2 row_ror:8 row_mask:0xf bank_mask:0xf\n\t"
+        "v_add_f32_dpp %3, %3, %3 row_ror:8 row_mask:0xf bank_mask:0xf\n\t"
+        "v_add_f32_dpp %0, %4, %4 row_ror:8 row_mask:0xf bank_mask:0xc\n\t"
+        "v_add_f32_dpp %1, %5, %5 row_ror:8 row_mask:0xf bank_mask:0xc\n\t"
+        "v_add_f32_dpp %2, %6, %6 row_ror:8 row_mask:0xf bank_mask:0xc\n\t"
+        "v_add_f32_dpp %3, %7, %7 row_ror:8 row_mask:0xf bank_mask:0xc"
+        : "+v"(a0), "+v"(a1), "+v"(a2), "+v"(a3) : "v"(b0), "v"(b1), "v"(b2), "v"(b3));
+}
+__device__ __forceinline__ void half_rows4(float& a0, float& a1, float b0, float b1) {
+    asm("s_nop 1\n\t"
+        "v_add_f32_dpp %0, %0, %0 row_half_mirror row_mask:0xf bank_mask:0xf\n\t"
+        "v_add_f32_dpp %1, %1, %1 row_half_mirror row_mask:0xf bank_mask:0xf\n\t"
+        "v_add_f32_dpp %0, %2, %2 row_half_mirror row_mask:0xf bank_mask:0xa\n\t"
+        "v_add_f32_dpp %1, %3, %3 row_half_mirror row_mask:0xf bank_mask:0xa"
+        : "+v"(a0), "+v"(a1) : "v"(b0), "v"(b1));
+}
 // v[0 .. NV) summed over the 32 lanes of one part: lane l returns value index_of(l).  (row_half_mirror also turns bits 0 and 1
 // round: all lanes that it mixes are summed later on.)
 template <int NV> __device__ __forceinline__ float part_sums(float (&v)[NV], int lane)
 {
     static_assert(NV == 8 || NV == 16 || NV == 32, "values per lane");
-    const bool b3 = lane & 8, b2 = lane & 4, b1 = lane & 2, b0 = lane & 1;
+    const bool b1 = lane & 2, b0 = lane & 1;
 #pragma unroll
-    for (int i = 0; i < NV / 2; ++i) v[i] = half16(v[i], v[i + NV / 2]);
+    for (int i = 0; i < NV / 2; i += 4)
+        half_rows8(v[i], v[i + 1], v[i + 2], v[i + 3], v[i + NV / 2], v[i + NV / 2 + 1], v[i + NV / 2 + 2], v[i + NV / 2 + 3]);
 #pragma unroll
-    for (int i = 0; i < NV / 4; ++i) v[i] = half_dpp<DPP_XOR8>(v[i], v[i + NV / 4], b3);
+    for (int i = 0; i < NV / 4; i += 2) half_rows4(v[i], v[i + 1], v[i + NV / 4], v[i + NV / 4 + 1]);
 #pragma unroll
-    for (int i = 0; i < NV / 8; ++i) v[i] = half_dpp<DPP_XOR7>(v[i], v[i + NV / 8], b2);
+    for (int i = 0; i < NV / 8; ++i) v[i] = half16(v[i], v[i + NV / 8]);
     if constexpr (NV >= 16) {
 #pragma unroll
         for (int i = 0; i < NV / 16; ++i) v[i] = half_dpp<DPP_XOR2>(v[i], v[i + NV / 16], b1);
@@ -47,7 +71,10 @@ template <int NV> __device__ __forceinline__ float part_sums(float (&v)[NV], int
     if constexpr (NV == 32) return half_dpp<DPP_XOR1>(v[0], v[1], b0);
     else return v[0] + dpp<DPP_XOR1>(v[0]);
 }
-template <int NV> __device__ __forceinline__ int index_of(int lane) { return (lane & 31) >> (NV == 32 ? 0 : NV == 16 ? 1 : 2); }
+template <int NV> __device__ __forceinline__ int index_of(int lane) {        // bits 3, 2, 4, 1, 0, the first log2(NV) of them
+    const int hi = (lane >> 3 & 1) << 2 | (lane >> 2 & 1) << 1 | (lane >> 4 & 1);
+    return NV == 8 ? hi : NV == 16 ? hi << 1 | (lane >> 1 & 1) : hi << 2 | (lane >> 1 & 1) << 1 | (lane & 1);
+}
 
 // a segment's adjoint: (adjoint of its incoming state for a zero adjoint behind it, S)
 template <class T, class M, int NP, bool GATED>
