@@ -364,10 +364,11 @@ void bc_reduce_kernel(const float* __restrict__ part, typename M::raw* __restric
     }
 }
 
-// Slabs of parameter-gradient sums: enough workgroups for two a CU, no more than rows x segments
+// Slabs of parameter-gradient sums, a workgroup each: rows x segments, at most 512 workgroups of 8 waves (two rounds of the machine:
+// rows in descending order of length even out, L=129 B=512 C=256 fp32 with lengths of 64 .. 129 256 us against 263 us with one).
 int slabs(const ScanPlan& p, int B, int G)
 {
-    const long long units = (long long)B * p.nseg, want = (2048 / p.waves + p.cblk * G - 1) / (p.cblk * G);
+    const long long units = (long long)B * p.nseg, want = (4096 / p.waves + p.cblk * G - 1) / (p.cblk * G);
     return (int)(units < want ? units : want);
 }
 
