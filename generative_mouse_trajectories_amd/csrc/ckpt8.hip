@@ -135,9 +135,10 @@ void wgrad8_kernel(const typename T::raw* __restrict__ dY, long long ldy, const 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wp = wave >> 1, wq = wave & 1;
     const int n_t = (N + WG_T - 1) / WG_T, i_t = (I + WG_T - 1) / WG_T, tiles = n_t * i_t;
-    // block = xcd + 8 (tile + tiles * group), slab = 8 group + xcd: the tiles of one slab share an XCD's L2
-    const int rest = blockIdx.x >> 3, tile = rest % tiles, slab = rest / tiles * 8 + (blockIdx.x & 7);
-    if (slab >= ks) return;
+    // 8 slabs or more (then a multiple of 8): block = xcd + 8 (tile + tiles * group), slab = 8 group + xcd, so that the tiles of one slab
+    // share an XCD's L2.  Fewer: there are tiles enough for all XCDs.
+    const int rest = blockIdx.x >> 3;
+    const int tile = ks >= 8 ? rest % tiles : blockIdx.x % tiles, slab = ks >= 8 ? rest / tiles * 8 + (blockIdx.x & 7) : blockIdx.x / tiles;
     const int n0 = tile % n_t * WG_T, i0 = tile / n_t * WG_T;
     const long long r1 = R;
     const int all = (int)((R + WG_K - 1) / WG_K);       // stages, dealt to the slabs in turn
@@ -293,13 +294,13 @@ int wgrad8_slabs(long long R, int N, int I)
     long long k = (768 + tiles - 1) / tiles;
     const long long most = (R + 4 * WG_K - 1) / (4 * WG_K);
     if (k > most) k = most;
-    return (int)(k < 1 ? 1 : k);
+    return (int)(k < 1 ? 1 : k >= 8 ? k / 8 * 8 : k);
 }
 
 template <class T> int launch_wgrad8(const void* dY, long long ldy, const signed char* codes, const unsigned char* scale, float* slab, long long R,
                                      int N, int I, int ks, int want_db, hipStream_t stream)
 {
-    const long long tiles = (long long)((N + WG_T - 1) / WG_T) * ((I + WG_T - 1) / WG_T), grid = 8 * tiles * ((ks + 7) / 8);
+    const long long tiles = (long long)((N + WG_T - 1) / WG_T) * ((I + WG_T - 1) / WG_T), grid = tiles * ks;
     if (grid >= (1LL << 24) || ldy >= (1LL << 24) || I >= (1 << 24)) return GMT_ERR_UNSUPPORTED;
     hipLaunchKernelGGL(wgrad8_kernel<T>, dim3((unsigned)grid), dim3(256), 0, stream, (const typename T::raw*)dY, ldy, codes, scale, slab, R, N, I,
                        ks, want_db);

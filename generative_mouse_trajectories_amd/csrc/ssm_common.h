@@ -98,6 +98,7 @@ __global__ __launch_bounds__(1024) void slab_reduce_kernel(const float* __restri
 }
 static inline int launch_slab_reduce(const float* slab, float* out, long long n, long long pitch, int P, hipStream_t stream)
 {
+    if (n >= (1LL << 27)) return GMT_ERR_UNSUPPORTED;   // (16 threads a column: 2^31 threads)
     hipLaunchKernelGGL(slab_reduce_kernel<0>, dim3((unsigned)((n + 63) / 64)), dim3(1024), 0, stream, slab, out, n, pitch, P);
     GMT_LAUNCH_CHECK();
     return GMT_OK;

@@ -55,7 +55,7 @@ def test_pack_of_views():
 
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize('Rows,N,I', [(1, 1, 1), (5, 3, 33), (32, 128, 128), (33, 129, 127), (257, 515, 250), (1000, 64, 9), (4096, 96, 160),
-                                      (20000, 130, 64)])
+                                      (20000, 130, 64), (700, 2100, 2001), (90, 4000, 3000)])
 def test_weight_gradient(Rows, N, I, dtype):
     """Products are exact: the error is that of fp32 sums.  A slab adds its rows 16 at a time (Rows / 16 + 16 roundings at most),
     then slabs add up (512 / 16 + 16 at most), each a half step of the sum of magnitudes."""

@@ -381,6 +381,104 @@ def test_other_stream_and_graph_replays():
         assert torch.equal(token(), y) and torch.equal(state_h, h)
 
 
+def test_two_streams_at_once_and_inference_mode():
+    """Training passes on two streams without a wait between them; the same call under inference_mode."""
+    from generative_mouse_trajectories_amd import ops_ssm
+    L, B, C, N = 150, 6, 96, 16
+    runs = []
+    for seed in (31, 32):
+        t, ay, al = scan_inputs(L, B, C, N, 1, torch.float32, True, True, True, seed)
+        runs.append(({k: a.to(DEV).requires_grad_(True) for k, a in t.items()}, ay.to(DEV), al.to(DEV)))
+
+    def run(leaves, ay, al):
+        y, h = ops_ssm.selective_scan(*(leaves[k] for k in NAMES[:5]), **{k: leaves[k] for k in NAMES[5:]})
+        return (y, h, *torch.autograd.grad([y, h], list(leaves.values()), [ay, al]))
+    alone = [run(*r) for r in runs]
+    streams = [torch.cuda.Stream() for _ in runs]
+    torch.cuda.synchronize()
+    both = [[], []]
+    for _ in range(3):
+        for s, r, out in zip(streams, runs, both):
+            with torch.cuda.stream(s):
+                out.append(run(*r))
+    torch.cuda.synchronize()
+    for want, outs in zip(alone, both):
+        for got in outs:
+            assert all(torch.equal(a, b) for a, b in zip(want, got))
+    leaves = runs[0][0]
+    with torch.inference_mode():
+        y, h = ops_ssm.selective_scan(*(leaves[k] for k in NAMES[:5]), **{k: leaves[k] for k in NAMES[5:]})
+        assert torch.equal(y, alone[0][0]) and torch.equal(h, alone[0][1])
+        ops_ssm.selective_scan_step(*(leaves[k][0] if k in 'xBC' or k == 'dt' else leaves[k] for k in NAMES[:5]), h, D=leaves['D'],
+                                    z=leaves['z'][0], dt_bias=leaves['dt_bias'])
+
+
+def test_second_derivatives_are_refused_and_changed_inputs_noticed():
+    from generative_mouse_trajectories_amd import ops, ops_ssm
+    x = torch.randn(5, 2, 8, device=DEV, requires_grad=True)
+    w = torch.randn(8, 3, device=DEV, requires_grad=True)
+    A, Bm = -torch.ones(8, 4, device=DEV), torch.randn(5, 2, 4, device=DEV)
+    h0 = torch.randn(2, 8, 4, device=DEV)
+    lin = torch.randn(6, 8, device=DEV, requires_grad=True)
+    for y in (ops_ssm.causal_conv(x, w)[0], ops_ssm.selective_scan(x, x, A, Bm, Bm)[0], ops.linear(x, lin, None, ckpt8=True)):
+        g, = torch.autograd.grad((y ** 2).sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match='once_differentiable'):
+            g.sum().backward()
+    y, _ = ops_ssm.selective_scan(x, x, A, Bm, Bm, state=h0)
+    with torch.no_grad():                                 # a single step in place on a state that the backward pass needs
+        ops_ssm.selective_scan_step(x[0].detach(), x[0].detach(), A, Bm[0], Bm[0], h0)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        y.sum().backward()
+
+
+@pytest.mark.parametrize('B,C,N', [(70000, 3, 2), (3, 2050, 16)])
+def test_many_rows_and_wide_rows(B, C, N):
+    from generative_mouse_trajectories_amd import ops_ssm
+    L = 3
+    t, ay, al = scan_inputs(L, B, C, N, 1, torch.float32, True, True, True, 4)
+    w = torch.randn(C, 4, generator=torch.Generator().manual_seed(2))
+    leaves = {k: a.to(DEV).requires_grad_(True) for k, a in t.items()}
+    gw = w.to(DEV).requires_grad_(True)
+    u, _ = ops_ssm.causal_conv(leaves['x'], gw)
+    y, h = ops_ssm.selective_scan(u, *(leaves[k] for k in NAMES[1:5]), **{k: leaves[k] for k in NAMES[5:]})
+    got = torch.autograd.grad([y, h], [gw, *leaves.values()], [ay.to(DEV), al.to(DEV)])
+    ref = {k: R.d(a).requires_grad_(True) for k, a in t.items()}
+    rw = R.d(w).requires_grad_(True)
+    ru, _ = R.conv(ref['x'], rw, None, None, None)
+    ry, rh = R.scan(ru, *(ref[k] for k in NAMES[1:8]), None, ref['state'])
+    want = torch.autograd.grad([ry, rh], [rw, *ref.values()], [R.d(ay), R.d(al)])
+    R.close(y, ry, 200, 'y')
+    R.close(h, rh, 200, 'state')
+    for k, a, b in zip(('weight', *leaves), got, want):
+        # sums over B * L rows: partial sums over at most 1024 slabs of the rows, B / 1024 rows each and then 64 + 16 slabs
+        R.close(a, b, 400 + (L * (B // 256 + 2) + 80 if k in ('weight', 'A', 'D', 'dt_bias') else 0) + (C if k in 'BC' else 0), k)
+
+
+def test_offsets_beyond_32_bits():
+    """2.2e9 elements a sequence: the last steps agree with calls on the last steps alone."""
+    from generative_mouse_trajectories_amd import ops_ckpt8, ops_ssm
+    L, B, C, N = 70000, 32, 1000, 4
+    x = torch.empty(L, B, C, device=DEV, dtype=torch.bfloat16).normal_(generator=torch.Generator(DEV).manual_seed(1))
+    assert x.numel() > 2 ** 31
+    w = torch.randn(C, 4, generator=torch.Generator().manual_seed(2)).to(DEV)
+    y, last = ops_ssm.causal_conv(x, w)
+    y2, last2 = ops_ssm.causal_conv(x[-64:], w, state=x[-67:-64])
+    assert torch.equal(y[-64:], y2) and torch.equal(last, last2) and torch.equal(last, x[-3:])
+    del y
+    p = ops_ckpt8.pack(x)
+    q = ops_ckpt8.pack(x[-64:])
+    assert torch.equal(p.codes[-64:], q.codes) and torch.equal(p.exponents[-64:], q.exponents)
+    del p, q
+    A = -torch.rand(C, N, generator=torch.Generator().manual_seed(3)).to(DEV) * 4
+    Bm = torch.randn(L, B, N, generator=torch.Generator(DEV).manual_seed(4), device=DEV).to(torch.bfloat16)
+    y, h = ops_ssm.selective_scan(x, x, A, Bm, Bm)
+    _, h1 = ops_ssm.selective_scan(x[:-640], x[:-640], A, Bm[:-640], Bm[:-640])
+    y2, h2 = ops_ssm.selective_scan(x[-640:], x[-640:], A, Bm[-640:], Bm[-640:], state=h1)
+    # two partitions of the same recurrence; the memory of a state is 1 / (step A), at most a few hundred steps of 3 roundings
+    R.close(h, R.d(h2), 2000, 'state')
+    R.close(y[-640:], R.d(y2), 2000, 'y')
+
+
 def test_layer_run_training_prompt_and_sampling():
     """The operators as they are used together: projection -> convolution -> maps and steps -> scan -> projection, trained with its
     activations in 8 bits and whole, against float64; then a prompt and single steps."""
