@@ -4,7 +4,7 @@
 //     h[t][n] = exp(step[t] A[n]) h[t-1][n] + step[t] x[t] B[t][n]                                N states per channel
 //     y[t]    = (sum_n C[t][n] h[t][n] + D x[t]) silu(z[t])
 //
-// B and C are shared by the channels of a group.  Time-major [L][B][..].  PARTS = 1 or 2 lanes hold a channel with N / PARTS
+// B and C are shared by the channels of a group.  Time-major [L][B][..].  PARTS = 1, 2 or 4 lanes hold a channel with N / PARTS
 // states each in registers; a workgroup is up to 8 waves of one row and one group, which share B[t] and C[t] through LDS as fp32.
 // Time runs in chunks of CH steps, requested one chunk ahead, in three phases: what depends on (t, channel) alone - softplus,
 // gate - for all steps at once, divided between a channel's lanes; the recurrence, step by step; the outputs, divided again.
@@ -57,7 +57,9 @@ static inline ScanPlan fwd_plan(int L, int B, int C, int N, int G)
     const ScanPlan p = scan_plan(L, B, C, N, G, 1, 4);
     return (long long)B * G * p.cblk * p.waves >= 4096 ? p : scan_plan(L, B, C, N, G, 2, 4);
 }
-static inline ScanPlan bwd_plan(int L, int B, int C, int N, int G) { return scan_plan(L, B, C, N, G, 2, BWD_WAVES); }
+// 4 .. 8 states a lane: what the backward pass can keep of a chunk in registers (N=32, L=256 B=128 C=512 bf16: 16 states a lane 760 us,
+// 8 states 505 us; N=16, B=256: 4 states a lane 536 us, 8 states 473 us)
+static inline ScanPlan bwd_plan(int L, int B, int C, int N, int G) { return scan_plan(L, B, C, N, G, N > 16 ? 4 : 2, BWD_WAVES); }
 
 static inline int scan_check(const gmt_scan_args* a)
 {
@@ -65,8 +67,8 @@ static inline int scan_check(const gmt_scan_args* a)
     GMT_CHECK_ARG(a->C % a->G == 0);
     GMT_CHECK_ARG((a->x_scale != nullptr) == (a->dt_scale != nullptr) && (a->z == nullptr || (a->x_scale != nullptr) == (a->z_scale != nullptr)));
     if (a->N > 32) return GMT_ERR_UNSUPPORTED;
-    // byte offsets within a pair of steps (B and C: a chunk) and within a row's kept states are 31 bits
-    const long long lim = 1LL << 28;
+    // byte offsets within four steps (B and C: a chunk) and within a row's kept states are 31 bits
+    const long long lim = 1LL << 27;
     if ((long long)a->C * 128 >= 1LL << 31 || a->x_t < 0 || a->dt_t < 0 || a->z_t < 0 || a->dy_t < 0 ||
         a->B_t < 0 || a->C_t < 0 || a->B_t >= lim / 4 || a->C_t >= lim / 4) return GMT_ERR_UNSUPPORTED;
     if (a->C >= lim || a->x_t >= lim || a->dt_t >= lim || a->z_t >= lim || a->dy_t >= lim || (long long)a->B * a->C >= lim) return GMT_ERR_UNSUPPORTED;
@@ -130,30 +132,51 @@ __device__ __forceinline__ float half32(float a, float b) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// ---- lanes of a channel.  With two parts, the halves of the wave: 32 neighbouring channels each, whole memory sectors, and
-// one v_permlane32_swap spreads the values of two steps or gathers their sums.
+// (a, b) -> lanes with bit 4 clear: a summed over that bit, set: b
+__device__ __forceinline__ float half16(float a, float b) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// ---- lanes of a channel.  With PARTS parts, the halves or quarters of the wave: neighbouring channels each, whole memory sectors.
+// Few permlane swaps spread the values of PARTS steps over the parts or gather their sums.
 template <int PARTS> struct Lanes {
     static constexpr int OWN = CH / PARTS;              // a lane's own steps of a chunk: j * PARTS + part
     int part; unsigned chan;                            // chan: channel within the workgroup
     __device__ __forceinline__ Lanes() {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        part = PARTS == 1 ? 0 : lane >> 5;
-        chan = wave * (64 / PARTS) + (PARTS == 1 ? lane : lane & 31);
+        part = lane / (64 / PARTS);
+        chan = wave * (64 / PARTS) + lane % (64 / PARTS);
     }
     // a lane's value for its own step -> those of the PARTS neighbouring steps, on every lane of the channel
     __device__ __forceinline__ void spread(float own, float (&v)[PARTS]) const {
         if constexpr (PARTS == 1) v[0] = own;
         else {
             const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(own), __float_as_uint(own), false, false);
-            v[0] = __uint_as_float(r[0]);
-            v[1] = __uint_as_float(r[1]);
+            if constexpr (PARTS == 2) {
+                v[0] = __uint_as_float(r[0]);
+                v[1] = __uint_as_float(r[1]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const auto q = __builtin_amdgcn_permlane16_swap(r[k], r[k], false, false);
+                    v[2 * k] = __uint_as_float(q[0]);
+                    v[2 * k + 1] = __uint_as_float(q[1]);
+                }
+            }
         }
     }
     // the lanes' terms for PARTS neighbouring steps -> the sum for a lane's own step
     __device__ __forceinline__ float gather(const float (&v)[PARTS]) const {
-        if constexpr (PARTS == 1) return v[0]; else return half32(v[0], v[1]);
+        if constexpr (PARTS == 1) return v[0];
+        else if constexpr (PARTS == 2) return half32(v[0], v[1]);
+        else return half16(half32(v[0], v[2]), half32(v[1], v[3]));
     }
-    __device__ __forceinline__ float sum(float v) const { if constexpr (PARTS == 1) return v; else return half32(v, v); }
+    __device__ __forceinline__ float sum(float v) const {
+        if constexpr (PARTS > 1) v = half32(v, v);
+        if constexpr (PARTS > 2) v = half16(v, v);
+        return v;
+    }
 };
 
 // One sequence of a row, as a lane sees it.  Uniform base of a step plus a 32-bit byte offset of the lane (its part's step and its
@@ -179,16 +202,19 @@ template <class T> struct Seq {
 template <class T, int PARTS> struct Own {
     static constexpr int OWN = CH / PARTS;
     typename T::raw v[OWN];
-    __device__ __forceinline__ void request(const Seq<T>& q, int tc, int te) {
+    __device__ __forceinline__ void request(const Seq<T>& q, int tc, int te, int part) {
 #pragma unroll
         for (int j = 0; j < OWN; ++j) {
             const int t = min(tc + j * PARTS, te - 1);
-            const bool all = t + PARTS <= te;           // (uniform) every part's step exists
+            // (uniform) every part's step exists; else the parts without one take the last one that does
+            const bool all = t + PARTS <= te;
+            const int back = PARTS > 2 ? min(part, te - 1 - t) : 0;
+            const unsigned off = all ? q.off : q.off0 + back * q.pt, soff = all ? q.soff : q.soff0 + back * q.spt;
             const Uniform p = uniform(q.p + (long long)t * q.pt);
             if constexpr (__is_same(T, Q8)) {
-                v[j].q = load_at<signed char>(p, all ? q.off : q.off0);
-                v[j].s = load_at<unsigned char>(uniform(q.sp + (long long)t * q.spt), all ? q.soff : q.soff0);
-            } else v[j] = load_at<typename T::raw>(p, all ? q.off : q.off0);
+                v[j].q = load_at<signed char>(p, off);
+                v[j].s = load_at<unsigned char>(uniform(q.sp + (long long)t * q.spt), soff);
+            } else v[j] = load_at<typename T::raw>(p, off);
         }
     }
 };

@@ -17,13 +17,6 @@ namespace {
 
 using namespace gmt_ssm;
 
-constexpr int PARTS = 2;                                // lanes per channel (ssm_scan.h): the halves of the wave
-
-// (a, b) -> lanes with bit 4 clear: a summed over that bit, set: b
-__device__ __forceinline__ float half16(float a, float b) {
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
-    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
 template <int CTRL> __device__ __forceinline__ float half_dpp(float a, float b, bool upper) {
     const float keep = upper ? b : a, send = upper ? a : b;
     return keep + dpp<CTRL>(send);
@@ -51,29 +44,34 @@ __device__ __forceinline__ void half_rows4(float& a0, float& a1, float b0, float
         "v_add_f32_dpp %1, %3, %3 row_half_mirror row_mask:0xf bank_mask:0xa"
         : "+v"(a0), "+v"(a1) : "v"(b0), "v"(b1));
 }
-// v[0 .. NV) summed over the 32 lanes of one part: lane l returns value index_of(l).  (row_half_mirror also turns bits 0 and 1
-// round: all lanes that it mixes are summed later on.)
-template <int NV> __device__ __forceinline__ float part_sums(float (&v)[NV], int lane)
+// v[0 .. NV) summed over the lanes of one part: lane l returns value index_of(l).  (row_half_mirror also turns bits 0 and 1 round: all
+// lanes that it mixes are summed later on.)
+template <int NV, int PARTS> __device__ __forceinline__ float part_sums(float (&v)[NV], int lane)
 {
-    static_assert(NV == 8 || NV == 16 || NV == 32, "values per lane");
-    const bool b1 = lane & 2, b0 = lane & 1;
+    static_assert((PARTS == 2 || PARTS == 4) && (NV == 8 || NV == 16), "values per lane");
+    constexpr int N4 = NV / 4, N2 = PARTS == 2 ? N4 / 2 : N4;          // values left behind bits 3 and 2, and behind bit 4
 #pragma unroll
     for (int i = 0; i < NV / 2; i += 4)
         half_rows8(v[i], v[i + 1], v[i + 2], v[i + 3], v[i + NV / 2], v[i + NV / 2 + 1], v[i + NV / 2 + 2], v[i + NV / 2 + 3]);
 #pragma unroll
-    for (int i = 0; i < NV / 4; i += 2) half_rows4(v[i], v[i + 1], v[i + NV / 4], v[i + NV / 4 + 1]);
+    for (int i = 0; i < N4; i += 2) half_rows4(v[i], v[i + 1], v[i + N4], v[i + N4 + 1]);
+    if constexpr (PARTS == 2) {
 #pragma unroll
-    for (int i = 0; i < NV / 8; ++i) v[i] = half16(v[i], v[i + NV / 8]);
-    if constexpr (NV >= 16) {
+        for (int i = 0; i < N2; ++i) v[i] = half16(v[i], v[i + N2]);
+    }
+    if constexpr (N2 == 1) v[0] += dpp<DPP_XOR2>(v[0]);
+    else {
 #pragma unroll
-        for (int i = 0; i < NV / 16; ++i) v[i] = half_dpp<DPP_XOR2>(v[i], v[i + NV / 16], b1);
-    } else v[0] += dpp<DPP_XOR2>(v[0]);
-    if constexpr (NV == 32) return half_dpp<DPP_XOR1>(v[0], v[1], b0);
+        for (int i = 0; i < N2 / 2; ++i) v[i] = half_dpp<DPP_XOR2>(v[i], v[i + N2 / 2], lane & 2);
+    }
+    if constexpr (N2 == 4) return half_dpp<DPP_XOR1>(v[0], v[1], lane & 1);
     else return v[0] + dpp<DPP_XOR1>(v[0]);
 }
-template <int NV> __device__ __forceinline__ int index_of(int lane) {        // bits 3, 2, 4, 1, 0, the first log2(NV) of them
-    const int hi = (lane >> 3 & 1) << 2 | (lane >> 2 & 1) << 1 | (lane >> 4 & 1);
-    return NV == 8 ? hi : NV == 16 ? hi << 1 | (lane >> 1 & 1) : hi << 2 | (lane >> 1 & 1) << 1 | (lane & 1);
+template <int NV, int PARTS> __device__ __forceinline__ int index_of(int lane) {     // bits 3, 2, (4,) 1, 0, the first log2(NV) of them
+    constexpr int LOG = NV == 8 ? 3 : 4;
+    const int hi = lane >> 2 & 3;
+    const int all = PARTS == 2 ? hi << 3 | (lane >> 4 & 1) << 2 | (lane & 3) : hi << 2 | (lane & 3);
+    return all >> ((PARTS == 2 ? 5 : 4) - LOG);
 }
 
 // a segment's adjoint: (adjoint of its incoming state for a zero adjoint behind it, S)
@@ -81,7 +79,7 @@ template <class T, class M, int NP, bool GATED>
 __global__ __launch_bounds__(64 * BWD_WAVES)
 void scan_bwd_local_kernel(ScanArgs<T, M> a)
 {
-    constexpr int NS = NP / PARTS, OWN = CH / PARTS;
+    constexpr int PARTS = NP == 32 ? 4 : 2, NS = NP / PARTS, OWN = CH / PARTS;
     __shared__ __align__(16) float sC[2][CH * NP];
     const int cb = blockIdx.x % a.p.cblk, rest = blockIdx.x / a.p.cblk;
     const int gr = rest % a.G, rest2 = rest / a.G;
@@ -105,9 +103,9 @@ void scan_bwd_local_kernel(ScanArgs<T, M> a)
     Own<M, PARTS> yr;
     MapTile<M, NP> mC;
     auto request = [&](int tc) {
-        dr.request(dq, tc, te);
-        if (GATED) zr.request(zq, tc, te);
-        yr.request(yq, tc, te);
+        dr.request(dq, tc, te, ln.part);
+        if (GATED) zr.request(zq, tc, te, ln.part);
+        yr.request(yq, tc, te, ln.part);
         mC.request(Cp, a.C_t, tc, te, a.N);
     };
     int buf = 0, k = te > t0 ? (te - t0 + CH - 1) / CH - 1 : -1;
@@ -149,11 +147,11 @@ template <class T, class M, int NP, bool GATED>
 __global__ __launch_bounds__(64 * BWD_WAVES, 2)
 void scan_bwd_kernel(ScanArgs<T, M> a)
 {
-    constexpr int NS = NP / PARTS, OWN = CH / PARTS;
+    constexpr int PARTS = NP == 32 ? 4 : 2, NS = NP / PARTS, OWN = CH / PARTS;
     // The exponentials of the last KE steps of a chunk stay in registers, those of the others are computed twice: as many as fit
-    // beside the states (N = 16, L=256 B=256 C=512 bf16: 8 kept 499 us, 4 kept 518 us, none 538 us; from 8-bit codes, whose
-    // exponents take registers too, L=129: 506, 390, 399 us).
-    constexpr int KE = NP == 8 ? CH : NP == 32 ? 0 : __is_same(T, Q8) ? CH / 2 : CH;
+    // beside the states (N = 16, L=256 B=256 C=512 bf16: 8 kept 478 us, 4 kept 504 us; from 8-bit codes, whose exponents take
+    // registers too, 4).
+    constexpr int KE = NS == 8 && __is_same(T, Q8) ? CH / 2 : CH;
     __shared__ __align__(16) float sB[2][CH * NP], sC[2][CH * NP];
     __shared__ float red[2][BWD_WAVES][CH][2 * NP];             // [wave][step][part][dB, dC of the part's states]
     const int cb = blockIdx.x % a.p.cblk, rest = blockIdx.x / a.p.cblk;
@@ -210,10 +208,10 @@ void scan_bwd_kernel(ScanArgs<T, M> a)
         MapTile<M, NP> mB, mC;
         float hk[NS];
         auto request = [&](int tc) {
-            xr.request(xq, tc, te);
-            dr.request(dq, tc, te);
-            if (GATED) zr.request(zq, tc, te);
-            yr.request(yq, tc, te);
+            xr.request(xq, tc, te, ln.part);
+            dr.request(dq, tc, te, ln.part);
+            if (GATED) zr.request(zq, tc, te, ln.part);
+            yr.request(yq, tc, te, ln.part);
             mB.request(Bp, a.B_t, tc, te, a.N);
             mC.request(Cp, a.C_t, tc, te, a.N);
             load_kept<NP, NS>(a.ck, tc / CH, a.B, b, a.C, koff, hk);
@@ -302,7 +300,7 @@ void scan_bwd_kernel(ScanArgs<T, M> a)
 #pragma unroll
                     for (int n = 0; n < NS; ++n) pin(dA[n]);
                     if (q == 0) { gBk[j] = ln.gather(va); qAk[j] = ln.gather(vb); }
-                    red[buf][wave][s][ln.part * 2 * NS + index_of<2 * NS>(lane)] = part_sums<2 * NS>(v, lane);
+                    red[buf][wave][s][ln.part * 2 * NS + index_of<2 * NS, PARTS>(lane)] = part_sums<2 * NS, PARTS>(v, lane);
                     step_fence();
                 }
 #pragma unroll

@@ -45,9 +45,9 @@ void scan_fwd_kernel(ScanArgs<T, M> a)
     Own<T, PARTS> xr, dr, zr;
     MapTile<M, NP> mB, mC;
     auto request = [&](int tc) {
-        xr.request(xq, tc, te);
-        dr.request(dq, tc, te);
-        if (GATED) zr.request(zq, tc, te);
+        xr.request(xq, tc, te, ln.part);
+        dr.request(dq, tc, te, ln.part);
+        if (GATED) zr.request(zq, tc, te, ln.part);
         mB.request(Bp, a.B_t, tc, te, a.N);
         if (Y) mC.request(Cp, a.C_t, tc, te, a.N);
     };
