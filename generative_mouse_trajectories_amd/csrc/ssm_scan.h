@@ -8,8 +8,9 @@
 // states each in registers; a workgroup is up to 8 waves of one row and one group, which share B[t] and C[t] through LDS as fp32.
 // Time runs in chunks of CH steps, requested one chunk ahead, in three phases: what depends on (t, channel) alone - softplus,
 // gate - for all steps at once, divided between a channel's lanes; the recurrence, step by step; the outputs, divided again.
-// The recurrence is 5 instructions a state and step, one of them an exponential at half rate: VALU issue bounds these kernels
-// (N = 16: 5.3 cycles of a SIMD per state, against 0.2 bytes), not HBM.
+// The recurrence is 5 instructions a state and step, one of them an exponential at half rate, and VALU issue is what bounds these
+// kernels: N = 16 forward 150 issue slots for a step of 64 channels, 88 % of them filled (L=256 B=256 C=512 bf16 160 us = 210e9
+// elements a second, 2.7 TB/s); backward 440, 82 % filled (465 us).
 //
 // Few rows (long prompts) do not fill 1024 SIMDs: time is then cut into segments.  A segment maps its incoming state
 // linearly, h_out = exp(A S) h_in + h_loc, S = the sum of its steps - one float per channel holds the whole decay.  Pass 1 finds

@@ -22,8 +22,9 @@ template <int CTRL> __device__ __forceinline__ float half_dpp(float a, float b, 
     return keep + dpp<CTRL>(send);
 }
 // The same for bits 3 and 2 of the lane, which are banks of four lanes that a DPP instruction can leave out: a + its partner on all
-// lanes, then b + its partner on the upper ones - two instructions a value instead of three.  The wait at the front is the one
-// that a DPP operand needs behind the instruction that wrote it, which the compiler does not see in here.
+// lanes, then b + its partner on the upper ones - two instructions a value instead of three.  The waits at the front (and at the end of
+// half_rows4, whose results go to permlane swaps) are those that a DPP or permlane operand needs behind the instruction that wrote
+// it; the compiler does not see into these blocks.
 __device__ __forceinline__ void half_rows8(float& a0, float& a1, float& a2, float& a3, float b0, float b1, float b2, float b3) {
     asm("s_nop 1\n\t"
         "v_add_f32_dpp %0, %0, %0 row_ror:8 row_mask:0xf bank_mask:0xf\n\t"
@@ -34,15 +35,16 @@ __device__ __forceinline__ void half_rows8(float& a0, float& a1, float& a2, floa
         "v_add_f32_dpp %1, %5, %5 row_ror:8 row_mask:0xf bank_mask:0xc\n\t"
         "v_add_f32_dpp %2, %6, %6 row_ror:8 row_mask:0xf bank_mask:0xc\n\t"
         "v_add_f32_dpp %3, %7, %7 row_ror:8 row_mask:0xf bank_mask:0xc"
-        : "+v"(a0), "+v"(a1), "+v"(a2), "+v"(a3) : "v"(b0), "v"(b1), "v"(b2), "v"(b3));
+        : "+&v"(a0), "+&v"(a1), "+&v"(a2), "+&v"(a3) : "v"(b0), "v"(b1), "v"(b2), "v"(b3));
 }
 __device__ __forceinline__ void half_rows4(float& a0, float& a1, float b0, float b1) {
     asm("s_nop 1\n\t"
         "v_add_f32_dpp %0, %0, %0 row_half_mirror row_mask:0xf bank_mask:0xf\n\t"
         "v_add_f32_dpp %1, %1, %1 row_half_mirror row_mask:0xf bank_mask:0xf\n\t"
         "v_add_f32_dpp %0, %2, %2 row_half_mirror row_mask:0xf bank_mask:0xa\n\t"
-        "v_add_f32_dpp %1, %3, %3 row_half_mirror row_mask:0xf bank_mask:0xa"
-        : "+v"(a0), "+v"(a1) : "v"(b0), "v"(b1));
+        "v_add_f32_dpp %1, %3, %3 row_half_mirror row_mask:0xf bank_mask:0xa\n\t"
+        "s_nop 1"
+        : "+&v"(a0), "+&v"(a1) : "v"(b0), "v"(b1));
 }
 // v[0 .. NV) summed over the lanes of one part: lane l returns value index_of(l).  (row_half_mirror also turns bits 0 and 1 round: all
 // lanes that it mixes are summed later on.)
