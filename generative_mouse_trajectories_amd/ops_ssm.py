@@ -245,18 +245,18 @@ def _scan_forward(x, dt, A, B, C, D, z, dt_bias, state, lengths, keep):
     y = x.new_empty(x.shape)
     last = A.new_empty((x.shape[1], *A.shape))
     a = _scan_args(x, dt, z, A, B, C, D, dt_bias, state, lengths, y=y.data_ptr(), state_out=last.data_ptr())
-    n_ck, n_fwd, _ = _workspace(a)
+    n_ck, n_fwd, n_bwd = _workspace(a)
     ck, ws = _space(n_ck if keep else 0, A), _space(n_fwd, A)
     a.ck, a.workspace, a.workspace_floats = _at(ck), _at(ws), n_fwd
     L_.call('gmt_selective_scan_fwd', ctypes.addressof(a), L_.stream_of(x.get_device()), nbytes=float((3 + (z is not None)) * x.numel() * x.element_size()))
-    return y, last, ck
+    return y, last, ck, (n_ck, n_bwd)
 
 
 class SelectiveScanFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, dt, A, B, C, D, z, dt_bias, state, lengths, ckpt8):
         # the state before every eighth step; from 8-bit checkpoints the backward pass finds them itself
-        y, last, ck = _scan_forward(x, dt, A, B, C, D, z, dt_bias, state, lengths, not ckpt8)
+        y, last, ck, ctx.floats = _scan_forward(x, dt, A, B, C, D, z, dt_bias, state, lengths, not ckpt8)
         seqs = []
         for t in (x, dt, z):
             p = ops_ckpt8.pack(t) if ckpt8 and t is not None else None
@@ -287,7 +287,7 @@ class SelectiveScanFn(torch.autograd.Function):
             a = _scan_args(x, dt, z, A, B, C, D, dt_bias, state, lengths, dy=dy.data_ptr(), dstate_out=_at(dlast), dx=dx.data_ptr(),
                            ddt=ddt.data_ptr(), dz=_at(dz), dB=dB.data_ptr(), dC=dC.data_ptr(), dparam=dparam.data_ptr(), dstate=_at(dstate),
                            dy_t=st[0], dy_b=st[1])
-            n_ck, _, n_bwd = _workspace(a)
+            n_ck, n_bwd = ctx.floats
             if ctx.ckpt8:
                 ck = _space(n_ck, A)
             ws = _space(n_bwd, A)
