@@ -158,7 +158,7 @@ void scan_bwd_kernel(ScanArgs<T, M> a)
     __shared__ float red[2][BWD_WAVES][CH][2 * NP];             // [wave][step][part][dB, dC of the part's states]
     const int cb = blockIdx.x % a.p.cblk, rest = blockIdx.x / a.p.cblk;
     const int gr = rest % a.G, slab = rest / a.G;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Lanes<PARTS> ln;
     const int cg = a.C / a.G, ci = cb * a.p.chans + ln.chan, n0 = ln.part * NS;
     const bool on = ci < cg, wave_on = cb * a.p.chans + wave * (64 / PARTS) < cg;
@@ -169,7 +169,8 @@ void scan_bwd_kernel(ScanArgs<T, M> a)
     for (int n = 0; n < NS; ++n) { A2[n] *= LOG2E; dA[n] = 0.f; }
     const float bias = a.dt_bias ? a.dt_bias[c] : 0.f, Dc = a.D ? a.D[c] : 0.f;
     const long long tbg = (long long)a.L * a.B * a.G * a.N;
-    const unsigned koff = (unsigned)(n0 * a.C + c) * 4, ooff = (unsigned)((ln.part * a.B * a.C + c) * sizeof(typename M::raw));
+    const unsigned koff = (unsigned)(n0 * a.C + c) * 4;
+    const int o_t = a.B * a.C;                          // pitch of a step of the outputs
 
     auto put_bc = [&](int t, int b, bool is_c, int n, float v) {
         const long long at = (((long long)t * a.B + b) * a.G + gr) * a.N + n;
@@ -177,13 +178,19 @@ void scan_bwd_kernel(ScanArgs<T, M> a)
         else (is_c ? a.dC : a.dB)[at] = from_f<M>(v);
     };
     int buf = 0, p_tc = 0, p_te = 0, p_b = 0;           // the chunk whose sums wait in red[buf ^ 1]: steps p_tc .. p_te - 1
+    const int bc_t = a.B * a.G * a.N;                   // pitch of a step of dB and dC
     auto flush = [&]() {
-        for (int i = threadIdx.x; i < CH * 2 * NP; i += a.p.width) {
-            const int s = i / (2 * NP), j = i % (2 * NP), n = j / (2 * NS) * NS + j % NS;
+        static_assert(CH * NP % 64 == 0, "a wave's 64 sums are all dB or all dC");
+        const long long row = (((long long)p_tc * a.B + p_b) * a.G + gr) * a.N;
+        for (int i0 = wave * 64; i0 < 2 * CH * NP; i0 += a.p.width) {
+            const bool is_c = i0 >= CH * NP;
+            const int i = i0 % (CH * NP) + lane, s = i / NP, n = i % NP;
             if (p_tc + s >= p_te || n >= a.N) continue;
             float v = 0.f;
-            for (int w = 0; w < a.p.waves; ++w) v += red[buf ^ 1][w][s][j];
-            put_bc(p_tc + s, p_b, j % (2 * NS) >= NS, n, v);
+            for (int w = 0; w < a.p.waves; ++w) v += red[buf ^ 1][w][s][n / NS * 2 * NS + (is_c ? NS : 0) + n % NS];
+            const unsigned at = (unsigned)(s * bc_t + n);
+            if (a.p.cblk > 1) store_at<float>(uniform(a.bc_part + (long long)cb * 2 * tbg + (is_c ? tbg : 0) + row), at * 4, v);
+            else store_at<typename M::raw>(uniform((is_c ? a.dC : a.dB) + row), at * (unsigned)sizeof(typename M::raw), from_f<M>(v));
         }
     };
 
@@ -198,6 +205,7 @@ void scan_bwd_kernel(ScanArgs<T, M> a)
         const Seq<T> xq(a.x, a.xs, a.x_t, a.x_b, b, ln.part, c, a.B, a.C), dq(a.dt, a.dts, a.dt_t, a.dt_b, b, ln.part, c, a.B, a.C),
             zq(a.z, a.zs, a.z_t, a.z_b, b, ln.part, c, a.B, a.C);
         const Seq<M> yq(a.dy, nullptr, a.dy_t, a.dy_b, b, ln.part, c, a.B, a.C);
+        const unsigned ooff = (unsigned)((ln.part * o_t + b * a.C + c) * sizeof(typename M::raw));
         float gc[NS];                                   // exp(step[t+1] A) g[t+1]
 #pragma unroll
         for (int n = 0; n < NS; ++n) gc[n] = 0.f;
@@ -272,7 +280,7 @@ void scan_bwd_kernel(ScanArgs<T, M> a)
 #pragma unroll
                     for (int j = 0; j < OWN; ++j)
                         if (tc + j * PARTS + ln.part < t1 && on)
-                            put_out<M>(a.dz, ((long long)(tc + j * PARTS) * a.B + b) * a.C, ooff, dzf[j] * fmaf(Dc, xv[j], out[j]));
+                            put_out<M>(a.dz, (long long)(tc + j * PARTS) * o_t, ooff, dzf[j] * fmaf(Dc, xv[j], out[j]));
                     step_fence();
                 }
 #pragma unroll
@@ -312,7 +320,7 @@ void scan_bwd_kernel(ScanArgs<T, M> a)
                     dbias += dstep;
                     dD = fmaf(d[j], xv[j], dD);
                     if (t < t1 && on) {
-                        const long long base = ((long long)(tc + j * PARTS) * a.B + b) * a.C;
+                        const long long base = (long long)(tc + j * PARTS) * o_t;
                         put_out<M>(a.dx, base, ooff, fmaf(gBk[j], st[j], Dc * d[j]));
                         put_out<M>(a.ddt, base, ooff, dstep);
                     }
