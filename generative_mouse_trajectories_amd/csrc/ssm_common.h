@@ -68,6 +68,29 @@ __device__ __forceinline__ int length_of(const int* lengths, int b, int L) {
     return n < 0 ? 0 : n > L ? L : n;               // a length outside 0 .. L cannot lead outside the buffers
 }
 
+// The row whose length is number `rank` in descending order (rows of one length: the lower number first), found by every wave
+// for itself: bit by bit the largest key that more than `rank` keys reach.  For up to ORDERED rows of fewer than 2^21 steps; 16 keys a lane.
+constexpr int ORDERED = 1024;
+__device__ __forceinline__ int row_of_rank(const int* lengths, int rank, int B, int L) {
+    const int lane = threadIdx.x & 63;
+    unsigned key[ORDERED / 64];
+#pragma unroll
+    for (int k = 0; k < ORDERED / 64; ++k) {
+        const int i = k * 64 + lane;
+        key[k] = i < B ? (unsigned)length_of(lengths, i, L) * ORDERED + (ORDERED - 1 - i) : 0;
+    }
+    unsigned top = 0;
+    for (int bit = 41 - __builtin_clz(L); bit >= 0; --bit) {
+        const unsigned want = top | 1u << bit;
+        int n = 0;
+#pragma unroll
+        for (int k = 0; k < ORDERED / 64; ++k)
+            if (k * 64 < B) n += __popcll(__ballot(key[k] >= want));
+        if (n > rank) top = want;
+    }
+    return ORDERED - 1 - (int)(top % ORDERED);
+}
+
 // ---- sum of P slabs, `pitch` floats apart, in a fixed order: out[i] = sum_p slab[p][i], i < n.  64 columns x 16 slab groups a workgroup,
 // eight loads in flight a thread.
 template <int UNUSED = 0>

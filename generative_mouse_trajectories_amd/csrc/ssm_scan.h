@@ -79,6 +79,14 @@ static inline int scan_check(const gmt_scan_args* a)
     return GMT_OK;
 }
 
+// Rows of unequal length, if they fill more than 2048 waves (what the backward pass keeps on the machine), are taken in descending order,
+// so that the last ones are short: L=129 B=512 C=256 fp32 with lengths of 64 .. 129, backward 276 -> 256 us, forward 88 -> 85 us (rows that
+// come in descending order: 247 and 78 us).
+static inline bool by_length(const gmt_scan_args* a, const ScanPlan& p)
+{
+    return a->lengths && p.nseg == 1 && a->B <= ORDERED && a->L < 1 << 21 && (long long)a->B * a->G * p.cblk * p.waves > 2048;
+}
+
 // pointers and pitches of one launch by value; T / M: element types of x, dt, z / of everything else
 template <class T, class M> struct ScanArgs {
     const void *x, *dt, *z; const unsigned char *xs, *dts, *zs;           // elements, or codes and exponents of 8-bit checkpoints
@@ -89,6 +97,7 @@ template <class T, class M> struct ScanArgs {
     typename M::raw *dx, *ddt, *dz, *dB, *dC; float* dstate; float* part; float* bc_part;
     long long x_t, x_b, dt_t, dt_b, z_t, z_b, B_t, B_b, B_g, C_t, C_b, C_g, dy_t, dy_b;
     int L, B, C, N, G, P;
+    int sorted;                                         // rows are taken by length
     ScanPlan p;
 };
 
@@ -107,6 +116,7 @@ template <class T, class M> ScanArgs<T, M> scan_args(const gmt_scan_args* a, con
     s.B_t = a->B_t; s.B_b = a->B_b; s.B_g = a->B_g; s.C_t = a->C_t; s.C_b = a->C_b; s.C_g = a->C_g;
     s.dy_t = a->dy_t; s.dy_b = a->dy_b;
     s.L = a->L; s.B = a->B; s.C = a->C; s.N = a->N; s.G = a->G; s.P = 0;
+    s.sorted = by_length(a, p);
     s.p = p;
     return s;
 }

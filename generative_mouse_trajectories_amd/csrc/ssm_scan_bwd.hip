@@ -152,12 +152,21 @@ void scan_bwd_kernel(ScanArgs<T, M> a)
     constexpr int PARTS = NP == 32 ? 4 : 2, NS = NP / PARTS, OWN = CH / PARTS;
     // The exponentials of the last KE steps of a chunk stay in registers, those of the others are computed twice: as many as fit
     // beside the states (N = 16, L=256 B=256 C=512 bf16: 8 kept 478 us, 4 kept 504 us; from 8-bit codes, whose exponents take
-    // registers too, 4).
-    constexpr int KE = NS == 8 && __is_same(T, Q8) ? CH / 2 : CH;
+    // registers too, L=129 B=256 C=512: 8 kept 425 us, 6 375, 5 372, 4 388).
+    constexpr int KE = NS == 8 && __is_same(T, Q8) ? 5 : CH;
     __shared__ __align__(16) float sB[2][CH * NP], sC[2][CH * NP];
     __shared__ float red[2][BWD_WAVES][CH][2 * NP];             // [wave][step][part][dB, dC of the part's states]
     const int cb = blockIdx.x % a.p.cblk, rest = blockIdx.x / a.p.cblk;
     const int gr = rest % a.G, slab = rest / a.G;
+    __shared__ unsigned short rows[ORDERED];            // the slab's rows, if they are taken by length
+    if (a.sorted) {                                     // every other round from the other end: a slab's sum of lengths evens out
+        for (int lo = 0; lo + slab < a.B; lo += a.P) {
+            const int r = lo / a.P & 1 ? min(lo + a.P, a.B) - 1 - slab : lo + slab;
+            rows[lo / a.P] = (unsigned short)row_of_rank(a.lengths, r, a.B, a.L);     // every wave the same
+        }
+        lds_barrier();
+    }
+    step_fence();
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Lanes<PARTS> ln;
     const int cg = a.C / a.G, ci = cb * a.p.chans + ln.chan, n0 = ln.part * NS;
@@ -196,7 +205,9 @@ void scan_bwd_kernel(ScanArgs<T, M> a)
 
     const int units = a.B * a.p.nseg;
     for (int u = slab; u < units; u += a.P) {
-        const int b = u % a.B, seg = u / a.B;
+        const int seg = u / a.B;
+        int b = u % a.B;
+        if (a.sorted) b = __builtin_amdgcn_readfirstlane(rows[u / a.P]);
         const int len = length_of(a.lengths, b, a.L);
         const int t0 = seg * a.p.seglen, t1 = min(t0 + a.p.seglen, a.L), te = min(t1, len);
         const long long row = (long long)b * a.C + c;

@@ -18,7 +18,7 @@ void scan_fwd_kernel(ScanArgs<T, M> a)
     __shared__ __align__(16) float sB[2][CH * NP], sC[Y ? 2 : 1][Y ? CH * NP : 1];
     const int cb = blockIdx.x % a.p.cblk, rest = blockIdx.x / a.p.cblk;
     const int g = rest % a.G, rest2 = rest / a.G;
-    const int b = rest2 % a.B, seg = rest2 / a.B;
+    const int seg = rest2 / a.B, b = a.sorted ? row_of_rank(a.lengths, rest2, a.B, a.L) : rest2 % a.B;
     const Lanes<PARTS> ln;
     const int cg = a.C / a.G, ci = cb * a.p.chans + ln.chan, n0 = ln.part * NS;
     const bool on = ci < cg, wave_on = cb * a.p.chans + (int)(threadIdx.x >> 6) * (64 / PARTS) < cg;

@@ -147,6 +147,37 @@ def test_scan_forward_backward(L, B, C, N, G, dtype, gate, extras, rag, with_sta
         R.close(got[k], torch.zeros_like(R.d(t[k])) if want[k] is None else want[k], 2 * chain + 45 + extra, 'd' + k)
 
 
+@pytest.mark.parametrize('B,C,N,G,ckpt8', [(600, 256, 3, 1, False), (1024, 250, 2, 1, True), (1025, 256, 2, 1, False), (700, 512, 2, 2, False)])
+def test_many_rows_of_unequal_length(B, C, N, G, ckpt8):
+    """Rows are taken in another order than they are stored in, several to a workgroup; the inputs of equal and empty rows stay apart; a
+    workgroup sums the parameters' gradients over at most two or three rows."""
+    from generative_mouse_trajectories_amd import ops_ssm
+    L = 10
+    t, ay, al = scan_inputs(L, B, C, N, G, torch.float32, True, True, True, B + N)
+    if ckpt8:                                                # values that 8-bit checkpoints hold exactly
+        t.update({k: (t[k] * 32).round().clamp(-100, 100) / 32 for k in ('x', 'dt', 'z')})
+    lengths = torch.randint(0, L + 1, (B,), generator=torch.Generator().manual_seed(B), dtype=torch.int32)
+    lengths[0], lengths[1], lengths[B - 2], lengths[B - 1] = 0, L, L, 0
+    leaves = {k: t[k].to(DEV).requires_grad_(True) for k in NAMES}
+    outside = lengths.clone()
+    outside[0], outside[1] = -7, L + 100                     # read as 0 and L
+    y, last = ops_ssm.selective_scan(*(leaves[k] for k in ('x', 'dt', 'A', 'B', 'C')), D=leaves['D'], z=leaves['z'],
+                                     dt_bias=leaves['dt_bias'], state=leaves['state'], ckpt8=ckpt8, lengths=outside.to(DEV))
+    got = dict(zip(NAMES, grads([y, last], [leaves[k] for k in NAMES], [ay.to(DEV), al.to(DEV)])))
+    ref = {k: R.d(t[k]) for k in NAMES}
+    chain = 3 * L + N + 45
+    with torch.no_grad():
+        wy, wl = R.scan(*(ref[k] for k in NAMES[:8]), lengths, ref['state'])
+    R.close(y, wy, chain, 'y')
+    R.close(last, wl, chain, 'final state')
+    rl = {k: ref[k].clone().requires_grad_(True) for k in NAMES}
+    outs = R.scan(*(rl[k] for k in NAMES[:8]), lengths, rl['state'])
+    want = dict(zip(NAMES, grads(outs, [rl[k] for k in NAMES], [R.d(ay), R.d(al)])))
+    for k in NAMES:
+        extra = {'A': 3 * L + 80, 'D': 3 * L + 80, 'dt_bias': 3 * L + 80, 'B': C // G, 'C': C // G}.get(k, 0)
+        R.close(got[k], want[k], 2 * chain + 45 + extra, 'd' + k)
+
+
 def test_gradients_against_differences():
     """Directional derivatives of the operators' own outputs (fp32, summed in float64): central differences of width h err by
     h^2 / 6 of the third derivative plus the outputs' rounding over h; h = 2^-6 and outputs of size 1 leave under 2e-3."""
