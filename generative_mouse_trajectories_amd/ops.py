@@ -327,7 +327,8 @@ class LinearCkpt8Fn(torch.autograd.Function):
 def linear(x: torch.Tensor, w: torch.Tensor, b: Optional[torch.Tensor], ckpt8: bool = False) -> torch.Tensor:
     """ckpt8: x is kept for the backward pass in 8 bits (LinearCkpt8Fn)."""
     if ckpt8 and torch.is_grad_enabled() and (w.requires_grad or (b is not None and b.requires_grad)):
-        return LinearCkpt8Fn.apply(x, w, b)
+        from . import ops_ckpt8
+        return ops_ckpt8.apply(LinearCkpt8Fn, ops_ckpt8.on_device(x, w, b), x, w, b)
     return LinearFn.apply(x, w, b)
 
 

@@ -54,6 +54,41 @@ def time_major(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride()[-1] == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+# Autograd brings a leaf's gradient to the stream on which the first graph of that leaf was made.  While such a graph from the default
+# stream lives, a captured backward pass would have the default stream wait for the capture, which breaks it beyond an ordinary error.
+_DEFAULT = 'gmt_default_stream'
+_LEAF = type(torch.autograd.graph.get_gradient_edge(torch.zeros(1, requires_grad=True)).node)
+
+
+def refuse_capture_beside(tensors) -> None:
+    """Before a pass that may be differentiated is captured: GmtError if a leaf behind it has a live graph from the default stream."""
+    todo = [torch.autograd.graph.get_gradient_edge(t).node for t in tensors if torch.is_tensor(t) and t.requires_grad]
+    seen = set(todo)
+    while todo:
+        node = todo.pop()
+        if type(node) is _LEAF and node.metadata.get(_DEFAULT):
+            raise L_.GmtError(f'a leaf of shape {tuple(node.variable.shape)} has a graph that was made eagerly on the default stream and is still '
+                              'alive: its backward pass cannot be captured.  Drop that graph (its outputs), run it under another '
+                              'stream, or capture under torch.no_grad()')
+        for n, _ in node.next_functions:
+            if n is not None and n not in seen:
+                seen.add(n)
+                todo.append(n)
+
+
+def apply(fn, dev: int, *args):
+    """fn.apply(*args) for a differentiable operator of device `dev`, which must not be captured beside an eager graph of its leaves."""
+    default = L_.stream_of(dev) == 0
+    if not default and torch.cuda.is_current_stream_capturing():
+        refuse_capture_beside(args)
+    out = fn.apply(*args)
+    # the leaves that the operator reads directly are marked with the stream of their first graph, until their last graph has gone
+    for node, _ in (out[0] if type(out) is tuple else out).grad_fn.next_functions:
+        if type(node) is _LEAF:
+            node.metadata.setdefault(_DEFAULT, default)
+    return out
+
+
 def pack(x: torch.Tensor) -> Ckpt8:
     """x [..., C] fp32 or bf16 -> its 8-bit checkpoint."""
     dev = on_device(x)

@@ -181,7 +181,7 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     args = time_major(x), _whole(weight), _whole(bias), _whole(state), lengths, bool(silu)
     with on(dev):
         if _any_grad(x, weight, bias, state):
-            return CausalConvFn.apply(*args, bool(ckpt8))
+            return ops_ckpt8.apply(CausalConvFn, dev, *args, bool(ckpt8))
         return _conv_forward(*args)
 
 
@@ -336,7 +336,7 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
             _whole(dt_bias), _whole(state), lengths)
     with on(dev):
         if _any_grad(x, dt, A, B, C, D, z, dt_bias, state):
-            return SelectiveScanFn.apply(*args, bool(ckpt8))
+            return ops_ckpt8.apply(SelectiveScanFn, dev, *args, bool(ckpt8))
         return _scan_forward(*args, False)[:2]
 
 

@@ -412,6 +412,38 @@ def test_other_stream_and_graph_replays():
         assert torch.equal(token(), y) and torch.equal(state_h, h)
 
 
+def test_capture_beside_a_live_eager_graph_is_refused():
+    """... before anything is captured; once the eager graph has gone the same pass is captured and replayed."""
+    from generative_mouse_trajectories_amd import ops, ops_ssm
+    from generative_mouse_trajectories_amd._lib import GmtError
+    t, ay, al = scan_inputs(9, 3, 40, 5, 1, torch.float32, True, True, True, 21)
+    leaves = {k: a.to(DEV).requires_grad_(True) for k, a in t.items()}
+    w, conv = (torch.randn(40, n, generator=torch.Generator().manual_seed(n)).to(DEV).requires_grad_(True) for n in (40, 4))
+    ay = ay.to(DEV)
+
+    def passes():
+        u, _ = ops_ssm.causal_conv(ops.linear(leaves['x'], w, None, ckpt8=True), conv)
+        return ops_ssm.selective_scan(u, *(leaves[k] for k in NAMES[1:5]), **{k: leaves[k] for k in NAMES[5:]})[0]
+
+    def train():
+        return torch.autograd.grad(passes(), [w, conv, *leaves.values()], ay)
+    eager = passes()
+    for call in (passes, lambda: ops.linear(leaves['x'].detach(), w, None, ckpt8=True), lambda: ops_ssm.causal_conv(leaves['z'] * 2, conv)):
+        with pytest.raises(GmtError, match='eagerly on the default stream'):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
+    want = torch.autograd.grad(eager, [w, conv, *leaves.values()], ay)
+    del eager
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = train()
+    for _ in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        want = train()
+
+
 def test_two_streams_at_once_and_inference_mode():
     """Training passes on two streams without a wait between them; the same call under inference_mode."""
     from generative_mouse_trajectories_amd import ops_ssm

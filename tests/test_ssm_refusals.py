@@ -128,3 +128,37 @@ def test_library_entry_points_check_their_arguments():
     assert L.gmt_ckpt8_pack(None, 1, 1, None, None, 1, 1, 1, 0, None) == -1
     assert L.gmt_ckpt8_wgrad(16, 128, 16, 16, 16, 1 << 20, 128, 128, 0, 0, None, 0, None) == -4
     assert L.gmt_ckpt8_wgrad(16, 4, 16, 16, 16, 1, 8, 8, 0, 0, None, 0, None) == -1
+
+
+def test_capture_beside_a_live_eager_graph(monkeypatch):
+    """A pass that may be differentiated is not captured while a graph from the default stream holds one of its leaves."""
+    stream, capturing = [0], [False]
+    monkeypatch.setattr(_lib, 'stream_of', lambda dev: stream[0])
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: capturing[0])
+
+    class Twice(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, w):
+            return x * w, x + w
+
+        @staticmethod
+        def backward(ctx, a, b):
+            return a, b
+
+    def run(where, captured, x, w):
+        stream[0], capturing[0] = where, captured
+        return ops_ckpt8.apply(Twice, 0, x, w)
+
+    x, w = torch.ones(3, requires_grad=True), torch.ones(3, requires_grad=True)
+    run(7, True, x, w)                                       # nothing lives: captured
+    eager = run(0, False, x, w)
+    for inputs in ((x, w), (x.detach(), w), (x * 2, torch.ones(3)), ((x * 2).view(3) + 1, torch.ones(3))):
+        with pytest.raises(GmtError, match='eagerly on the default stream'):
+            run(7, True, *inputs)
+        run(7, False, *inputs)                               # another stream, no capture
+    run(7, True, x.detach(), torch.ones(3, requires_grad=True))
+    assert eager[0].grad_fn is not None
+    del eager, inputs
+    beside = run(5, False, x, w)                             # the first graph of its leaves is another stream's
+    run(0, False, x, w)
+    assert len(run(7, True, x, w)) == len(beside) == 2
