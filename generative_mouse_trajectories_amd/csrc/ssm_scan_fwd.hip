@@ -349,7 +349,8 @@ extern "C" int gmt_selective_scan_workspace(const gmt_scan_args* a, long long* c
     const ScanPlan p = fwd_plan(a->L, a->B, a->C, a->N, a->G);
     *ck_floats = (long long)p.nck * a->B * p.np * a->C;
     *fwd_floats = p.nseg > 1 ? (long long)p.nseg * a->B * a->C * (p.np + 1) : 0;
-    *bwd_floats = scan_bwd_floats(a);
+    const long long bwd = scan_bwd_floats(a);
+    *bwd_floats = bwd > *fwd_floats ? bwd : *fwd_floats;    // from 8-bit checkpoints the states are found again in it first
     return GMT_OK;
 }
 

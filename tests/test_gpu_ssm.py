@@ -178,6 +178,25 @@ def test_many_rows_of_unequal_length(B, C, N, G, ckpt8):
         R.close(got[k], want[k], 2 * chain + 45 + extra, 'd' + k)
 
 
+def test_states_found_again_in_segments_that_the_backward_pass_does_not_have():
+    """38 rows of 273 channels: the forward pass is cut into segments, the backward pass from 8-bit checkpoints is not."""
+    from generative_mouse_trajectories_amd import ops_ssm
+    L, B, C, N = 197, 38, 273, 2
+    t, ay, al = scan_inputs(L, B, C, N, 1, torch.float32, True, True, True, 5)
+    t.update({k: (t[k] * 32).round().clamp(-100, 100) / 32 for k in ('x', 'dt', 'z')})       # held exactly by the checkpoints
+    lengths = ragged(L, B)
+    leaves = {k: t[k].to(DEV).requires_grad_(True) for k in NAMES}
+    outs = ops_ssm.selective_scan(*(leaves[k] for k in ('x', 'dt', 'A', 'B', 'C')), D=leaves['D'], z=leaves['z'], dt_bias=leaves['dt_bias'],
+                                  state=leaves['state'], lengths=lengths.to(DEV), ckpt8=True)
+    got = grads(outs, list(leaves.values()), [ay.to(DEV), al.to(DEV)])
+    rl = {k: R.d(t[k]).requires_grad_(True) for k in NAMES}
+    want = grads(R.scan(*(rl[k] for k in NAMES[:8]), lengths, rl['state']), list(rl.values()), [R.d(ay), R.d(al)])
+    chain = 3 * L + N + 45
+    for k, g, w in zip(NAMES, got, want):
+        extra = {'A': L + 80, 'D': L + 80, 'dt_bias': L + 80, 'B': C, 'C': C}.get(k, 0)
+        R.close(g, w, 2 * chain + 45 + extra, 'd' + k)
+
+
 def test_gradients_against_differences():
     """Directional derivatives of the operators' own outputs (fp32, summed in float64): central differences of width h err by
     h^2 / 6 of the third derivative plus the outputs' rounding over h; h = 2^-6 and outputs of size 1 leave under 2e-3."""

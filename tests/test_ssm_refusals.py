@@ -130,6 +130,19 @@ def test_library_entry_points_check_their_arguments():
     assert L.gmt_ckpt8_wgrad(16, 4, 16, 16, 16, 1, 8, 8, 0, 0, None, 0, None) == -1
 
 
+@pytest.mark.parametrize('L', [1, 130, 197, 5000])
+def test_a_backward_workspace_holds_what_finding_the_states_again_takes(L):
+    """From 8-bit checkpoints the backward call runs the forward pass's segments in its own workspace."""
+    import ctypes
+    lib, n = _lib.lib(), [ctypes.c_longlong(0) for _ in range(3)]
+    for B in (1, 3, 17, 33, 38, 42, 43, 130, 600):
+        for C in (1, 40, 96, 128, 273, 520, 1000):
+            for N in (2, 8, 16, 32):
+                a = _lib.ScanArgs(x=16, dt=16, A=16, Bm=16, Cm=16, L=L, B=B, C=C, N=N, G=1)
+                assert lib.gmt_selective_scan_workspace(ctypes.addressof(a), *(ctypes.addressof(v) for v in n)) == 0
+                assert n[2].value >= n[1].value, (B, C, N)
+
+
 def test_capture_beside_a_live_eager_graph(monkeypatch):
     """A pass that may be differentiated is not captured while a graph from the default stream holds one of its leaves."""
     stream, capturing = [0], [False]
