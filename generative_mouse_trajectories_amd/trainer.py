@@ -136,7 +136,7 @@ def _host_backend(group=None) -> bool:
     pool streams of its own - and with a deep queue of persistent kernels ahead of it that staging never gets its
     turn (measured on MI355X, two ranks sharing the card at B = 4096: the GPU sits at 100 % busy and the event
     recorded before the FIRST collective is never reached, on either rank, while the same step with the collective
-    on an explicit host copy runs at full speed; tools/two_rank_diag.py).  So device tensors
+    on an explicit host copy runs at full speed).  So device tensors
     are never handed to gloo: all_reduce_sum / broadcast_ stage them through the host on the caller's own stream."""
     import torch.distributed as dist
     return dist.get_backend(group) == 'gloo'
