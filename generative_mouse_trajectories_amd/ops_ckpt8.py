@@ -13,6 +13,7 @@ import ctypes
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L_
 
@@ -31,7 +32,12 @@ _HERE = contextlib.nullcontext()
 
 
 def on_device(*tensors) -> int:
-    """Index of the one GPU that all of them (None: left out) are on."""
+    """Index of the one GPU that all of them (None: left out) are on.  Every entry point passes its tensors through here: one with a
+    forward-mode tangent is refused, which a kernel called beside autograd would drop without a word."""
+    if forward_ad._current_level >= 0:                   # (looked at only within a dual level: 0.5 us a tensor)
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise L_.GmtError(f'a tensor of shape {tuple(t.shape)} has a forward-mode tangent: these operators have no forward-mode derivatives')
     dev = None
     for t in tensors:
         if t is not None:

@@ -8,7 +8,7 @@ causal convolution in front of them and the single-step forms of both for sampli
 Sequences are fp32 or bf16 (all of one call alike); parameters, the scan's states and every sum are fp32.  The last axis is
 contiguous (it is copied if not), steps and rows may have any pitch: slices of one projection's output go in without a copy.
 `lengths` [B] are the rows' numbers of steps, 0 .. L: what lies behind them may hold anything, outputs and gradients there are zero,
-and the final state is the one after the row's last step.  Gradients are first-order.  GPU only.
+and the final state is the one after the row's last step.  Gradients are first-order and reverse-mode.  GPU only.
 """
 from __future__ import annotations
 

@@ -175,3 +175,21 @@ def test_capture_beside_a_live_eager_graph(monkeypatch):
     beside = run(5, False, x, w)                             # the first graph of its leaves is another stream's
     run(0, False, x, w)
     assert len(run(7, True, x, w)) == len(beside) == 2
+
+
+@pytest.mark.parametrize('grad', [False, True])
+def test_forward_mode_tangents(no_launch, grad):
+    """A dual tensor is refused by every entry, with and without a leaf that requires a gradient, rather than come back without its tangent."""
+    from torch.autograd import forward_ad
+    w, lin = torch.zeros(8, 4, requires_grad=grad), torch.zeros(5, 8, requires_grad=True)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(seq(), torch.ones(4, 3, 8))
+        one = forward_ad.make_dual(torch.zeros(3, 8), torch.ones(3, 8))
+        A = forward_ad.make_dual(torch.zeros(8, 5), torch.ones(8, 5))
+        for call in (lambda: ops_ssm.causal_conv(dual, w), lambda: ops_ssm.causal_conv(seq(), w, bias=one[0]),
+                     lambda: scan_call(z=dual), lambda: scan_call(A=A, D=torch.zeros(8, requires_grad=grad)), lambda: step_call(dt=one),
+                     lambda: ops_ssm.causal_conv_step(one, torch.zeros(3, 3, 8), w.detach()), lambda: ops_ckpt8.pack(dual),
+                     lambda: ops_ckpt8.wgrad(one, ops_ckpt8.Ckpt8(torch.zeros(3, 40, dtype=torch.int8), torch.zeros(3, 2, dtype=torch.uint8), torch.float32)),
+                     lambda: ops.linear(dual, lin, None, ckpt8=True)):
+            with pytest.raises(GmtError, match='forward-mode'):
+                call()
