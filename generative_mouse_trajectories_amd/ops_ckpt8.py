@@ -63,7 +63,8 @@ def time_major(t: torch.Tensor) -> torch.Tensor:
 # Autograd brings a leaf's gradient to the stream on which the first graph of that leaf was made.  While such a graph from the default
 # stream lives, a captured backward pass would have the default stream wait for the capture, which breaks it beyond an ordinary error.
 _DEFAULT = 'gmt_default_stream'
-_LEAF = type(torch.autograd.graph.get_gradient_edge(torch.zeros(1, requires_grad=True)).node)
+with torch.inference_mode(False), torch.enable_grad():     # (whatever mode the package is imported in)
+    _LEAF = type(torch.autograd.graph.get_gradient_edge(torch.zeros(1, requires_grad=True)).node)
 
 
 def refuse_capture_beside(tensors) -> None:

@@ -193,3 +193,15 @@ def test_forward_mode_tangents(no_launch, grad):
                      lambda: ops.linear(dual, lin, None, ckpt8=True)):
             with pytest.raises(GmtError, match='forward-mode'):
                 call()
+
+
+def test_import_under_inference_mode():
+    """The package can be imported (first) within torch.inference_mode() or no_grad()."""
+    import os
+    import subprocess
+    import sys
+    code = 'import torch\nwith torch.{}():\n    import generative_mouse_trajectories_amd as g\nprint(g.ops_ckpt8._LEAF.__name__)'
+    for mode in ('inference_mode', 'no_grad'):
+        r = subprocess.run([sys.executable, '-c', code.format(mode)], capture_output=True, text=True, timeout=300,
+                           cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+        assert r.returncode == 0 and r.stdout.strip() == 'AccumulateGrad', r.stderr[-500:]
