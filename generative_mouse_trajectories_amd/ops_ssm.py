@@ -64,8 +64,6 @@ def _step_states(state: torch.Tensor, state_out: Optional[torch.Tensor], shape: 
     _want(state, 'state', shape, dtype)
     if not state.is_contiguous():
         _fail('state: the state of a single step is updated where it is and must be contiguous')
-    if (state if state_out is None else state_out).is_inference() and not torch.is_inference_mode_enabled():
-        _fail('state: a tensor that was made under torch.inference_mode() is updated only there')
     if state_out is None:
         return state
     _want(state_out, 'state_out', shape, dtype)

@@ -205,13 +205,3 @@ def test_import_under_inference_mode():
         r = subprocess.run([sys.executable, '-c', code.format(mode)], capture_output=True, text=True, timeout=300,
                            cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
         assert r.returncode == 0 and r.stdout.strip() == 'AccumulateGrad', r.stderr[-500:]
-
-
-def test_step_on_a_state_of_inference_mode(no_launch):
-    """A state that was made under inference_mode is updated there alone: outside, the step is refused before anything is written."""
-    with torch.inference_mode():
-        h, c = torch.zeros(3, 8, 5), torch.zeros(3, 3, 8)
-    with torch.no_grad():
-        for call in (lambda: step_call(state=h), lambda: step_call(state_out=h), lambda: ops_ssm.causal_conv_step(torch.zeros(3, 8), c, torch.zeros(8, 4))):
-            with pytest.raises(GmtError, match='inference_mode'):
-                call()
