@@ -62,6 +62,9 @@ template <class E> __device__ __forceinline__ void store_at(Uniform p, unsigned 
     *(__attribute__((address_space(1))) E*)(p + off) = v;
 }
 
+// steps of a sequence, at most: sums of a step and a segment's length (fewer than 2^18 beyond the last step) are 32-bit
+constexpr int MAX_STEPS = 0x7fffffff - (1 << 18) + 1;
+
 __device__ __forceinline__ int length_of(const int* lengths, int b, int L) {
     if (!lengths) return L;
     const int n = lengths[b];

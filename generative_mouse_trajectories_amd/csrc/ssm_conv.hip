@@ -362,7 +362,7 @@ int check(const gmt_conv_args* a)
 {
     GMT_CHECK_ARG(a && a->x && a->w && a->L > 0 && a->B > 0 && a->C > 0);
     GMT_CHECK_ARG((long long)a->B * a->C < (1LL << 31));
-    if (a->K < 2 || a->K > 4) return GMT_ERR_UNSUPPORTED;
+    if (a->K < 2 || a->K > 4 || a->L > MAX_STEPS) return GMT_ERR_UNSUPPORTED;
     return GMT_OK;
 }
 

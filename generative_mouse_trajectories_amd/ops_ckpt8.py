@@ -19,6 +19,13 @@ from . import _lib as L_
 
 BLOCK = 32
 DTYPES = (torch.float32, torch.bfloat16)
+MAX_SIZE = (1 << 31) - (1 << 18)             # the kernels' sizes are 32-bit, and so are their sums with a tile's or a segment's
+
+
+def fits(shape, name: str) -> None:
+    """GmtError if one of these sizes would not arrive at the kernels as it is."""
+    if max(shape) > MAX_SIZE:
+        raise L_.GmtError(f'{name}: sizes of at most 2^31 - 2^18 expected, got {tuple(shape)}')
 
 
 class Ckpt8(NamedTuple):
@@ -103,6 +110,7 @@ def pack(x: torch.Tensor) -> Ckpt8:
         raise L_.GmtError(f'ckpt8 packs float32 and bfloat16, not {x.dtype}')
     if x.dim() < 1 or x.numel() == 0:
         raise L_.GmtError(f'ckpt8: nothing to pack in a tensor of shape {tuple(x.shape)}')
+    fits(x.shape[-2:] if x.dim() == 3 else x.shape[-1:], 'ckpt8')
     x = time_major(x.detach()) if x.requires_grad else time_major(x)
     C = x.shape[-1]
     if x.dim() == 3:
@@ -121,6 +129,7 @@ def pack(x: torch.Tensor) -> Ckpt8:
 def check(p: Ckpt8) -> int:
     dev = on_device(p.codes, p.exponents)
     C = p.codes.shape[-1]
+    fits((C,), 'ckpt8')
     if (p.codes.dtype != torch.int8 or p.exponents.dtype != torch.uint8 or p.codes.numel() == 0 or not p.codes.is_contiguous()
             or not p.exponents.is_contiguous() or p.exponents.shape != (*p.codes.shape[:-1], (C + BLOCK - 1) // BLOCK)):
         raise L_.GmtError('not an 8-bit checkpoint: contiguous int8 codes [..., C] and uint8 exponents [..., ceil(C / 32)] expected')
@@ -152,6 +161,7 @@ def wgrad(dY: torch.Tensor, p: Ckpt8, want_db: bool = False) -> Tuple[torch.Tens
         raise L_.GmtError(f'wgrad: dY must be float32 or bfloat16, not {dY.dtype}')
     N, I = dY.shape[-1], p.codes.shape[-1]
     R = p.codes.numel() // I
+    fits((N,), 'wgrad')
     if N == 0 or dY.numel() // N != R:
         raise L_.GmtError(f'wgrad: dY {tuple(dY.shape)} and the checkpoint {tuple(p.codes.shape)} have different rows')
     dY = time_major(dY.detach()) if dY.requires_grad else time_major(dY)

@@ -39,6 +39,7 @@ def _seq(x: torch.Tensor, name: str, dims: int) -> None:
         _fail(f'{name}: a {dims}-dimensional tensor with at least one element expected, got {tuple(x.shape)}')
     if x.dtype not in ops_ckpt8.DTYPES:
         _fail(f'{name}: float32 or bfloat16 expected, got {x.dtype}')
+    ops_ckpt8.fits(x.shape, name)
 
 
 def _lengths(lengths: Optional[torch.Tensor], B: int, L: int, x: torch.Tensor) -> Optional[torch.Tensor]:

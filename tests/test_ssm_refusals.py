@@ -205,3 +205,35 @@ def test_import_under_inference_mode():
         r = subprocess.run([sys.executable, '-c', code.format(mode)], capture_output=True, text=True, timeout=300,
                            cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
         assert r.returncode == 0 and r.stdout.strip() == 'AccumulateGrad', r.stderr[-500:]
+
+
+def test_sizes_beyond_32_bits(no_launch):
+    """The kernels' sizes are 32-bit: a larger one is refused (taken modulo 2^32 it would be a much smaller call that succeeds)."""
+    big = 2 ** 32 + 64
+    one = torch.zeros(1)
+    codes, scale = torch.zeros(1, dtype=torch.int8), torch.zeros(1, dtype=torch.uint8)
+    wide = one.expand(1, big)                               # (one element: every call is refused by its shape)
+    for call in (lambda: ops_ckpt8.pack(wide[0]), lambda: ops_ckpt8.pack(wide), lambda: ops_ckpt8.pack(wide.view(1, big, 1)),
+                 lambda: ops_ckpt8.pack(wide.view(1, 1, big)),
+                 lambda: ops_ckpt8.unpack(ops_ckpt8.Ckpt8(codes.expand(1, big), scale.expand(1, big // 32), torch.float32)),
+                 lambda: ops_ckpt8.wgrad(wide, ops_ckpt8.Ckpt8(codes.view(1, 1), scale.view(1, 1), torch.float32)),
+                 lambda: ops_ssm.causal_conv(wide.view(big, 1, 1), torch.zeros(1, 4)), lambda: ops_ssm.causal_conv(wide.view(1, big, 1), torch.zeros(1, 4)),
+                 lambda: ops_ssm.causal_conv(wide.view(1, 1, big), one.expand(big, 4)),
+                 lambda: ops_ssm.causal_conv_step(wide.view(big, 1), one.expand(3, big, 1), torch.zeros(1, 4)),
+                 lambda: scan_call(x=wide.view(big, 1, 1), dt=wide.view(big, 1, 1), A=torch.zeros(1, 1), B=wide.view(big, 1, 1), C=wide.view(big, 1, 1)),
+                 lambda: step_call(x=wide.view(big, 1), dt=wide.view(big, 1), A=torch.zeros(1, 1), B=wide.view(big, 1), C=wide.view(big, 1),
+                                   state=wide.view(big, 1, 1))):
+        with pytest.raises(GmtError, match='2\\^31'):
+            call()
+
+
+def test_library_entry_points_check_the_number_of_steps():
+    """... whose sums with a segment's length must stay within 32 bits."""
+    import ctypes
+    lib, n = _lib.lib(), ctypes.c_longlong(0)
+    for L, want in ((2 ** 31 - 2 ** 18, 0), (2 ** 31 - 2 ** 18 + 1, -2), (2 ** 31 - 1, -2)):
+        a = _lib.ConvArgs(x=16, w=16, L=L, B=1, C=4, K=4, dy=16, dx=16, dparam=16)
+        assert lib.gmt_causal_conv_bwd_workspace_floats(ctypes.addressof(a), ctypes.addressof(n)) == want
+        s = _lib.ScanArgs(x=16, dt=16, A=16, Bm=16, Cm=16, y=16, L=L, B=1, C=1, N=1, G=1)
+        sizes = [ctypes.c_longlong(0) for _ in range(3)]
+        assert lib.gmt_selective_scan_workspace(ctypes.addressof(s), *(ctypes.addressof(v) for v in sizes)) == want
