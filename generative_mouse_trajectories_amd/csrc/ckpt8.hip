@@ -7,8 +7,9 @@
 // for, a normal number.  A block that holds an infinity or a NaN stands for NaN throughout: s = 255, q = 0.
 //
 // Weight gradient: dW[n][i] = sum_r dY[r][n] Xhat[r][i], db[n] = sum_r dY[r][n].  Xhat is exact in bf16; an fp32 dY is exactly
-// the sum of three bf16 numbers (its 24 mantissa bits cut into 8 + 8 + 8), so three bf16 MFMAs give the products without a
-// rounding, accumulated in fp32, at 16 / 3 the rate of the fp32 matrix instruction.  A bf16 dY is one.
+// the sum of three bf16 numbers (its 24 mantissa bits cut into 8 + 8 + 8; all of them normal numbers from |dY| = 2^-102 on, below
+// up to 2^-126 of each may be lost), so three bf16 MFMAs give the products without a rounding, accumulated in fp32, at 16 / 3 the
+// rate of the fp32 matrix instruction.  A bf16 dY is one, and so is an infinite one.
 #include "ssm_common.h"
 #include "bf16_maps.h"
 
@@ -208,6 +209,21 @@ void wgrad8_kernel(const typename T::raw* __restrict__ dY, long long ldy, const 
 #pragma unroll
                     for (int k = 0; k < 4; ++k) v[k] -= __uint_as_float(__float_as_uint(v[k]) & 0xffff0000u);
                 }
+            }
+        }
+        if constexpr (PL > 1) {
+            // An infinity is its first number alone, but inf - inf was a NaN.  Looked for only where the column sums show one (or a NaN, or
+            // overflow): 345 -> 347 us at R=524288 N=512 I=128 with the packing, where a test of every value takes 352.
+            if (__any(!(fabsf(colsum[0]) + fabsf(colsum[1]) + fabsf(colsum[2]) + fabsf(colsum[3]) < __builtin_inff()))) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (__builtin_isinf(to_f((typename T::raw)st.y[j][k]))) {
+#pragma unroll
+                            for (int pl = 1; pl < PL; ++pl)
+                                *reinterpret_cast<unsigned short*>(img + pl * WG_IMG + img_addr(yr + 8 * j, yc + k)) = 0;
+                        }
             }
         }
         const float sc = __uint_as_float((unsigned)st.s << 23);

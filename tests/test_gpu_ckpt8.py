@@ -120,3 +120,35 @@ def test_linear_with_checkpointed_input(dtype):
     with torch.no_grad():
         assert torch.equal(ops.linear(x, w, b, ckpt8=True), y)
     assert ops.linear(x, w.detach(), None, ckpt8=True).requires_grad
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_weight_gradient_of_infinite_and_tiny_dy(dtype):
+    """An infinite dY gives what the definition gives: an infinity, NaN where x is zero or infinities of both signs meet, and NaN gives NaN
+    (also one whose mark is in the low half of an fp32 number).  The three bf16 numbers that an fp32 dY is cut into reach down to 2^-24 of it:
+    from 2^-102 on all of them are normal, below each (and each product and sum) may lose 2^-126."""
+    from generative_mouse_trajectories_amd import ops_ckpt8
+    Rows, N, I = 70, 16, 40
+    gen = torch.Generator().manual_seed(11)
+    x = torch.randint(-100, 101, (Rows, I), generator=gen).float() / 32               # held exactly
+    x[3, 4] = x[9, 35] = 0
+    p = ops_ckpt8.pack(x.to(DEV))
+    dy = torch.randn(Rows, N, generator=gen).to(dtype)
+    dy[3, 5], dy[9, 7], dy[20, 9], dy[30, 11], dy[31, 11] = float('inf'), -float('inf'), float('nan'), float('inf'), -float('inf')
+    if dtype == torch.float32:
+        dy.view(torch.int32)[40, 13] = 0x7f800001
+    dW, db = ops_ckpt8.wgrad(dy.to(DEV), p, want_db=True)
+    want = (R.d(dy)[:, :, None] * x.double()[:, None, :]).sum(0)
+    for got, ref in ((R.d(dW), want), (R.d(db), R.d(dy).sum(0))):
+        assert torch.equal(torch.isnan(got), torch.isnan(ref))
+        assert torch.equal(torch.isinf(got), torch.isinf(ref)) and torch.equal(got[torch.isinf(got)], ref[torch.isinf(ref)])
+    assert int(torch.isinf(want[5]).sum()) > 30 and int(torch.isnan(want[5]).sum()) >= 1 and bool(torch.isnan(want[11]).any())
+    fin = torch.isfinite(want)
+    mag = torch.nan_to_num(R.d(dy), 0.0, 0.0, 0.0).abs().t() @ x.double().abs()
+    assert bool(((R.d(dW) - want)[fin].abs() <= (Rows / 16 + 64) * R.U32 * mag[fin]).all())
+    for scale in (2.0 ** -100, 2.0 ** -120):
+        small = (torch.randn(Rows, N, generator=gen).double().clamp(0.25, 4.0) * scale).to(dtype)
+        dW, _ = ops_ckpt8.wgrad(small.to(DEV), p)
+        mag = R.d(small).abs().t() @ x.double().abs()
+        lost = 3 * 2.0 ** -126 * (x.double().abs().sum(0) + Rows) if scale < 2.0 ** -102 else 0.0
+        assert bool(((R.d(dW) - R.d(small).t() @ x.double()).abs() <= (Rows / 16 + 64) * R.U32 * mag + lost).all()), scale
