@@ -1,5 +1,6 @@
 // Selective scan, forward (ssm_scan.h has the formulas and the layout), its single-step form, and the segment chain that the
 // backward pass shares.
+#include <type_traits>
 #include "ssm_scan.h"
 
 namespace {
@@ -121,6 +122,14 @@ void scan_fwd_kernel(ScanArgs<T, M> a)
         for (int t = t0 + (max(te - t0, 0) + CH - 1) / CH * CH + ln.part; t < t1; t += PARTS) a.y[((long long)t * a.B + b) * a.C + c] = from_f<M>(0.f);
 }
 
+// exp(A S) h + loc of a segment, x = A S in base 2.  A growing state (A > 0) can have a decay beyond fp32 over a segment while the state itself,
+// zero or small, stays finite, as it does step by step: the factor is then taken in three parts (x >= 378 overflows for every h but 0).
+template <bool GROWS> __device__ __forceinline__ float chain_step(float x, float h, float loc) {
+    if (!GROWS) return fmaf(__builtin_amdgcn_exp2f(x), h, loc);
+    const float e = __builtin_amdgcn_exp2f(fminf(x, 378.f) * (1.0f / 3.0f));
+    return fmaf(e, e * (e * h), loc);
+}
+
 // seg_h: (h_loc of every segment) -> (its incoming state), in place.  The chain of a state is cut into 8 runs: each is joined to one
 // link by a thread of its own, the 8 links are chained through LDS, and each thread walks its run again from where it
 // starts.  Latency is all of the cost: 16 segments are requested at once (128 segments x 16384 states: a single walk 78 us, with 16
@@ -148,7 +157,7 @@ void scan_chain_kernel(float* seg_h, const float* __restrict__ seg_s, const floa
             step[j] = seg_s[((long long)s * B + b) * C + c];
         }
     };
-    auto walk = [&](float& h, float& S, bool store) {   // (a run of AHEAD segments or fewer is requested once)
+    auto walk = [&](float& h, float& S, bool store, auto grows) {       // (a run of AHEAD segments or fewer is requested once)
         for (int kb = k0; kb < k1; kb += AHEAD) {
             if (!store || per > AHEAD) request(kb);
 #pragma unroll
@@ -156,20 +165,25 @@ void scan_chain_kernel(float* seg_h, const float* __restrict__ seg_s, const floa
                 if (kb + j >= k1) break;
                 const int s = reverse ? nseg - 1 - (kb + j) : kb + j;
                 if (store) seg_h[s * n_all + i] = h;
-                h = fmaf(__builtin_amdgcn_exp2f(A2 * step[j]), h, loc[j]);
+                h = chain_step<grows>(A2 * step[j], h, loc[j]);
                 S += step[j];
             }
         }
     };
-    float h = 0.f, S = 0.f;
-    if (on) walk(h, S, false);
-    run_h[run][lane] = h;
-    run_s[run][lane] = S;
-    __syncthreads();
-    if (!on) return;
-    h = first ? first[(b * C + c) * N + n] : 0.f;
-    for (int r = 0; r < run; ++r) h = fmaf(__builtin_amdgcn_exp2f(A2 * run_s[r][lane]), h, run_h[r][lane]);
-    walk(h, S, true);
+    auto chain = [&](auto grows) {
+        float h = 0.f, S = 0.f;
+        if (on) walk(h, S, false, grows);
+        run_h[run][lane] = h;
+        run_s[run][lane] = S;
+        __syncthreads();
+        if (!on) return;
+        h = first ? first[(b * C + c) * N + n] : 0.f;
+        for (int r = 0; r < run; ++r) h = chain_step<grows>(A2 * run_s[r][lane], h, run_h[r][lane]);
+        walk(h, S, true, grows);
+    };
+    // the same for the whole workgroup (it has a barrier inside): its runs hold the same 32 states
+    if (__any(A2 > 0.f)) chain(std::true_type{});
+    else chain(std::false_type{});
 }
 
 // One step of every row: state [B][C][N] -> state_out (may be the same buffer).  The state, read and written once, is all of the

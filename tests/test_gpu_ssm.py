@@ -624,3 +624,36 @@ def test_layer_run_training_prompt_and_sampling():
                                                                                      dt_bias=q['dt_bias']), h))
             steps.append(o[None])
         R.close(torch.cat(steps), full, 8 * (3 * L + E + 45), 'prompt and single steps')
+
+
+def test_growing_states_in_segments():
+    """A > 0: over a segment the decay exp(A S) exceeds fp32, but a state that is zero (or tiny) there stays finite, as it does step by step."""
+    from generative_mouse_trajectories_amd import ops_ssm
+    L, B, C, N = 260, 2, 40, 4
+    t, ay, _ = scan_inputs(L, B, C, N, 1, torch.float32, True, False, True, 3)
+    t['A'] = 0.5 + torch.rand(C, N, generator=torch.Generator().manual_seed(1))
+    t['dt'] = t['dt'] + 2.0
+    t['x'][:L - 4] = 0                                       # nothing enters before the last steps, no adjoint behind the first ones
+    ay[4:] = 0
+    for state in (None, torch.full((B, C, N), 1e-30)):
+        t['state'] = state
+        if state is not None:                                # a small state that grows by up to e^128
+            t['dt'] = torch.full_like(t['dt'], -5.0)
+            t['dt'][:40] = 2.0
+        ref = {k: R.d(t[k]) for k in NAMES}
+        wy, wl = R.scan(*(ref[k] for k in NAMES[:8]), None, ref['state'])
+        assert float(wl.abs().max()) < 1e38
+        leaves = {k: t[k].to(DEV).requires_grad_(True) for k in NAMES if t[k] is not None}
+        y, h = ops_ssm.selective_scan(*(leaves[k] for k in NAMES[:5]), z=leaves['z'], state=leaves.get('state'))
+        # on top of the chain: an exponent of up to 128 with 40 roundings of a segment's sum of steps and 8 of softplus, scale and product
+        assert torch.isfinite(h).all() and torch.isfinite(y).all()
+        _, mag = R.scan(ref['x'].abs(), ref['dt'], ref['A'], ref['B'].abs(), *(ref[k] for k in NAMES[4:8]), None, ref['state'])
+        rel = ((R.d(h) - wl).abs() / mag).max()
+        assert float(rel) <= (3 * L + N + 45 + 128 * 48) * R.U32, float(rel)
+        if state is None:
+            gx, = torch.autograd.grad(y, leaves['x'], ay.to(DEV))
+            rx = ref['x'].clone().requires_grad_(True)
+            ry, _ = R.scan(rx, *(ref[k] for k in NAMES[1:8]), None, None)
+            want, = torch.autograd.grad(ry, rx, R.d(ay))
+            assert torch.isfinite(gx).all()
+            R.close(gx, want, 2 * (3 * L + N + 45) + 45, 'dx')
