@@ -18,6 +18,7 @@
 // does the same with the adjoint.  It costs the recurrence twice, so segments are cut only where half of the machine or more
 // would stand idle (scan_plan).
 #pragma once
+#include <cfloat>
 #include "ssm_common.h"
 
 namespace gmt_ssm {
@@ -258,6 +259,12 @@ template <int NS> __device__ __forceinline__ void store_states(float* p, int n0,
 #pragma unroll
         for (int n = 0; n < NS; ++n) if (n0 + n < N) p[n0 + n] = h[n];
     }
+}
+// A for exponentials in base 2.  A masked step is one of length 0, which must leave a state as it is: -inf (a state without memory, or what
+// base 2 makes of the lowest numbers) becomes the lowest number, because 0 * -inf is NaN.
+__device__ __forceinline__ float base2(float A) {
+    const float a = A * LOG2E;
+    return a < -FLT_MAX ? -FLT_MAX : a;
 }
 // The kept states (slot k: before step k CH) and the segments' states: [..][B][NP][C], N padded to NP with zeros.  off: (n0 C + c) * 4
 template <int NP, int NS> __device__ __forceinline__ void load_kept(const float* p, long long slot, int B, int b, int C, unsigned off, float (&h)[NS])

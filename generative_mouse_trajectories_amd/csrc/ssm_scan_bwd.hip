@@ -95,7 +95,7 @@ void scan_bwd_local_kernel(ScanArgs<T, M> a)
     float A2[NS], g[NS];
     load_states<NS>(a.A + (long long)c * a.N, n0, a.N, A2);
 #pragma unroll
-    for (int n = 0; n < NS; ++n) { A2[n] *= LOG2E; g[n] = 0.f; }
+    for (int n = 0; n < NS; ++n) { A2[n] = base2(A2[n]); g[n] = 0.f; }
     const float bias = a.dt_bias ? a.dt_bias[c] : 0.f;
     const typename M::raw* Cp = a.Cm + b * a.C_b + gr * a.C_g;
     const Seq<T> dq(a.dt, a.dts, a.dt_t, a.dt_b, b, ln.part, c, a.B, a.C), zq(a.z, a.zs, a.z_t, a.z_b, b, ln.part, c, a.B, a.C);
@@ -175,7 +175,7 @@ void scan_bwd_kernel(ScanArgs<T, M> a)
     float A2[NS], dA[NS], dD = 0.f, dbias = 0.f;
     load_states<NS>(a.A + (long long)c * a.N, n0, a.N, A2);
 #pragma unroll
-    for (int n = 0; n < NS; ++n) { A2[n] *= LOG2E; dA[n] = 0.f; }
+    for (int n = 0; n < NS; ++n) { A2[n] = base2(A2[n]); dA[n] = 0.f; }
     const float bias = a.dt_bias ? a.dt_bias[c] : 0.f, Dc = a.D ? a.D[c] : 0.f;
     const long long tbg = (long long)a.L * a.B * a.G * a.N;
     const unsigned koff = (unsigned)(n0 * a.C + c) * 4;
@@ -327,7 +327,8 @@ void scan_bwd_kernel(ScanArgs<T, M> a)
 #pragma unroll
                 for (int j = 0; j < OWN; ++j) {
                     const int t = tc + j * PARTS + ln.part;
-                    const float dstep = fmaf(gBk[j], xv[j], qAk[j] * LN2) * sig[j];
+                    // (a masked step's sum over A may overflow: 0, not 0 * inf)
+                    const float dstep = sig[j] == 0.f ? 0.f : fmaf(gBk[j], xv[j], qAk[j] * LN2) * sig[j];
                     dbias += dstep;
                     dD = fmaf(d[j], xv[j], dD);
                     if (t < t1 && on) {

@@ -30,7 +30,7 @@ void scan_fwd_kernel(ScanArgs<T, M> a)
     float A2[NS], h[NS];
     load_states<NS>(a.A + (long long)c * a.N, n0, a.N, A2);
 #pragma unroll
-    for (int n = 0; n < NS; ++n) { A2[n] *= LOG2E; h[n] = 0.f; }
+    for (int n = 0; n < NS; ++n) { A2[n] = base2(A2[n]); h[n] = 0.f; }
     const long long row = (long long)b * a.C + c;
     const unsigned koff = (unsigned)(n0 * a.C + c) * 4, yoff = (unsigned)((ln.part * a.B * a.C + c) * sizeof(typename M::raw));
     if (MODE != LOCAL) {
@@ -145,7 +145,7 @@ void scan_chain_kernel(float* seg_h, const float* __restrict__ seg_s, const floa
     const int c = (int)(i % C), n = (int)(i / C % np);
     const long long b = i / C / np;
     const bool on = i < n_all && n < N;                 // (padding: zeros in every segment)
-    const float A2 = on ? A[(long long)c * N + n] * LOG2E : 0.f;
+    const float A2 = on ? base2(A[(long long)c * N + n]) : 0.f;
     const int per = (nseg + RUNS - 1) / RUNS, k0 = run * per, k1 = min(k0 + per, nseg);
     constexpr int AHEAD = 16;
     float loc[AHEAD], step[AHEAD];

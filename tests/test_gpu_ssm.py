@@ -657,3 +657,25 @@ def test_growing_states_in_segments():
             want, = torch.autograd.grad(ry, rx, R.d(ay))
             assert torch.isfinite(gx).all()
             R.close(gx, want, 2 * (3 * L + N + 45) + 45, 'dx')
+
+
+@pytest.mark.parametrize('L,B', [(13, 9), (150, 9), (13, 2100)])
+def test_states_without_memory(L, B):
+    """A = -inf (or so low that base 2 takes it there): a state holds the last step alone, and what lies behind a row's end leaves it as it is."""
+    from generative_mouse_trajectories_amd import ops_ssm
+    C, N = 40, 6
+    t, ay, al = scan_inputs(L, B, C, N, 1, torch.float32, True, True, True, 4)
+    t['A'][3, 2], t['A'][7], t['A'][11, 0] = -float('inf'), -float('inf'), -3e38
+    lengths = ragged(L, B)
+    ref = {k: R.d(t[k]) for k in NAMES}
+    wy, wl = R.scan(*(ref[k] for k in NAMES[:8]), lengths, ref['state'])
+    leaves = {k: t[k].to(DEV).requires_grad_(True) for k in NAMES}
+    y, h = ops_ssm.selective_scan(*(leaves[k] for k in NAMES[:5]), D=leaves['D'], z=leaves['z'], dt_bias=leaves['dt_bias'], state=leaves['state'],
+                                  lengths=lengths.to(DEV))
+    R.close(y, wy, 3 * L + N + 45, 'y')
+    R.close(h, wl, 3 * L + N + 45, 'final state')
+    rx = ref['x'].clone().requires_grad_(True)
+    want, = torch.autograd.grad(R.scan(rx, *(ref[k] for k in NAMES[1:8]), lengths, ref['state']), rx, [R.d(ay), R.d(al)])
+    got = torch.autograd.grad([y, h], list(leaves.values()), [ay.to(DEV), al.to(DEV)])
+    R.close(got[0], want, 2 * (3 * L + N + 45) + 45, 'dx')
+    assert all(torch.isfinite(g).all() for g in got)
