@@ -72,7 +72,7 @@ static inline int scan_check(const gmt_scan_args* a)
     // byte offsets within four steps (B and C: a chunk) and within a row's kept states are 31 bits
     const long long lim = 1LL << 27;
     if ((long long)a->C * 128 >= 1LL << 31 || a->x_t < 0 || a->dt_t < 0 || a->z_t < 0 || a->dy_t < 0 ||
-        a->B_t < 0 || a->C_t < 0 || a->B_t >= lim / 4 || a->C_t >= lim / 4) return GMT_ERR_UNSUPPORTED;
+        a->B_t < 0 || a->C_t < 0 || a->B_t >= lim / 2 || a->C_t >= lim / 2) return GMT_ERR_UNSUPPORTED;
     if (a->C >= lim || a->x_t >= lim || a->dt_t >= lim || a->z_t >= lim || a->dy_t >= lim || (long long)a->B * a->C >= lim ||
         (long long)a->B * a->G * a->N >= lim / 2) return GMT_ERR_UNSUPPORTED;
     for (const ScanPlan& p : {fwd_plan(a->L, a->B, a->C, a->N, a->G), bwd_plan(a->L, a->B, a->C, a->N, a->G)})

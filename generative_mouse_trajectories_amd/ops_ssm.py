@@ -6,7 +6,8 @@ causal convolution in front of them and the single-step forms of both for sampli
     step = softplus(dt + dt_bias);  h[t] = exp(step A) h[t-1] + step x B;  y = (sum_n C h + D x) silu(z)        selective_scan
 
 Sequences are fp32 or bf16 (all of one call alike); parameters, the scan's states and every sum are fp32.  The last axis is
-contiguous (it is copied if not), steps and rows may have any pitch: slices of one projection's output go in without a copy.
+contiguous (it is copied if not), steps and rows may have any pitch: slices of one projection's output go in without a copy (but for the scan's
+sequences whose steps lie 2^27 elements or more apart, and its maps B and C from 2^26 on).
 `lengths` [B] are the rows' numbers of steps, 0 .. L: what lies behind them may hold anything, outputs and gradients there are zero,
 and the final state is the one after the row's last step.  Gradients are first-order and reverse-mode.  GPU only.
 """
@@ -23,6 +24,7 @@ from . import ops_ckpt8
 from .ops_ckpt8 import Ckpt8, on, on_device, time_major
 
 MAX_STATES = 32
+FAR_SEQ, FAR_MAP = 1 << 27, 1 << 26          # elements from one step to the next that the scan's 32-bit offsets within a chunk do not reach
 
 
 def _fail(msg: str):
@@ -96,6 +98,12 @@ def _whole(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
 
 def _at(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
+
+
+def _near(t: torch.Tensor, far: int) -> torch.Tensor:
+    """time_major(t), as a contiguous copy if its steps lie `far` or more apart."""
+    t = time_major(t)
+    return t if t.stride(0) < far or t.shape[0] == 1 else t.contiguous()
 
 
 def _space(n: int, like: torch.Tensor) -> Optional[torch.Tensor]:
@@ -211,9 +219,9 @@ def causal_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor,
 # selective scan
 # ----------------------------------------------------------------------------------------
 def _map_pitches(m: torch.Tensor, lead: int):
-    """Pitches of B or C [.., N] or [.., G, N]: (step, row, group), the step's 0 without a step axis."""
+    """Pitches of B or C [.., N] or [.., G, N]: (step, row, group), the step's 0 without a second step."""
     st = m.stride()
-    return (st[0] if lead == 2 else 0), st[lead - 1], (st[lead] if m.dim() == lead + 2 else 0)
+    return (st[0] if lead == 2 and m.shape[0] > 1 else 0), st[lead - 1], (st[lead] if m.dim() == lead + 2 else 0)
 
 
 def _scan_args(x, dt, z, A, B, C, D, dt_bias, state, lengths, **more) -> L_.ScanArgs:
@@ -224,10 +232,11 @@ def _scan_args(x, dt, z, A, B, C, D, dt_bias, state, lengths, **more) -> L_.Scan
             more.update(z=z.codes.data_ptr(), z_scale=z.exponents.data_ptr())
     else:
         shape, xs, ds = x.shape, x.stride(), dt.stride()
-        more.update(x=x.data_ptr(), x_t=xs[0], x_b=xs[1], dt=dt.data_ptr(), dt_t=ds[0], dt_b=ds[1])
+        steps = shape[0] > 1                             # (the pitch of a single step may be anything)
+        more.update(x=x.data_ptr(), x_t=xs[0] if steps else 0, x_b=xs[1], dt=dt.data_ptr(), dt_t=ds[0] if steps else 0, dt_b=ds[1])
         if z is not None:
             zs = z.stride()
-            more.update(z=z.data_ptr(), z_t=zs[0], z_b=zs[1])
+            more.update(z=z.data_ptr(), z_t=zs[0] if steps else 0, z_b=zs[1])
     Bp, Cp = _map_pitches(B, 2), _map_pitches(C, 2)
     return L_.ScanArgs(A=A.data_ptr(), Bm=B.data_ptr(), Cm=C.data_ptr(), D=_at(D), dt_bias=_at(dt_bias), state=_at(state), lengths=_at(lengths),
                        B_t=Bp[0], B_b=Bp[1], B_g=Bp[2], C_t=Cp[0], C_b=Cp[1], C_g=Cp[2], L=shape[0], B=shape[1], C=shape[2], N=A.shape[1],
@@ -277,7 +286,7 @@ class SelectiveScanFn(torch.autograd.Function):
             z = None if z is None else Ckpt8(z, ze, dtype)
         dev = A.get_device()
         with on(dev):
-            dy = A.new_zeros(shape, dtype=dtype) if dy is None else time_major(dy)
+            dy = A.new_zeros(shape, dtype=dtype) if dy is None else _near(dy, FAR_SEQ)
             dlast = _whole(dlast)
             dx, ddt = A.new_empty(shape, dtype=dtype), A.new_empty(shape, dtype=dtype)
             dz = None if z is None else A.new_empty(shape, dtype=dtype)
@@ -287,7 +296,7 @@ class SelectiveScanFn(torch.autograd.Function):
             st = dy.stride()
             a = _scan_args(x, dt, z, A, B, C, D, dt_bias, state, lengths, dy=dy.data_ptr(), dstate_out=_at(dlast), dx=dx.data_ptr(),
                            ddt=ddt.data_ptr(), dz=_at(dz), dB=dB.data_ptr(), dC=dC.data_ptr(), dparam=dparam.data_ptr(), dstate=_at(dstate),
-                           dy_t=st[0], dy_b=st[1])
+                           dy_t=st[0] if shape[0] > 1 else 0, dy_b=st[1])
             n_ck, n_bwd = ctx.floats
             if ctx.ckpt8:
                 ck = _space(n_ck, A)
@@ -333,7 +342,7 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     _scan_checks(x, dt, A, B, C, D, z, dt_bias, (L, Bt))
     _want(state, 'state', (Bt, Ch, A.shape[1]), torch.float32)
     lengths = _lengths(lengths, Bt, L, x)
-    args = (time_major(x), time_major(dt), _whole(A), time_major(B), time_major(C), _whole(D), None if z is None else time_major(z),
+    args = (_near(x, FAR_SEQ), _near(dt, FAR_SEQ), _whole(A), _near(B, FAR_MAP), _near(C, FAR_MAP), _whole(D), None if z is None else _near(z, FAR_SEQ),
             _whole(dt_bias), _whole(state), lengths)
     with on(dev):
         if _any_grad(x, dt, A, B, C, D, z, dt_bias, state):

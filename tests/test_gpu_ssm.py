@@ -679,3 +679,30 @@ def test_states_without_memory(L, B):
     got = torch.autograd.grad([y, h], list(leaves.values()), [ay.to(DEV), al.to(DEV)])
     R.close(got[0], want, 2 * (3 * L + N + 45) + 45, 'dx')
     assert all(torch.isfinite(g).all() for g in got)
+
+
+@pytest.mark.parametrize('seq,maps', [(2 ** 27 - 24, 2 ** 26 - 1), (2 ** 27 + 8, 2 ** 26 + 3)])
+def test_steps_far_apart(seq, maps):
+    """Steps at the largest pitch that is read in place, and beyond it (copied): what contiguous sequences give, to the bit."""
+    from generative_mouse_trajectories_amd import ops_ssm
+    L, B, C, N = 11, 2, 40, 5
+    t, ay, al = scan_inputs(L, B, C, N, 1, torch.bfloat16, True, True, True, 6)
+    far = torch.zeros(10 * max(seq, maps) + 2 * B * C, device=DEV, dtype=torch.bfloat16)
+
+    def apart(a, pitch, at):
+        v = far[at:].as_strided(a.shape, (pitch, *a.stride()[1:]))
+        v.copy_(a)
+        return v
+    flat = {k: v.to(DEV) for k, v in t.items()}
+    for name in ('x', 'dt', 'z', 'B', 'C', 'ay'):
+        near, adj = dict(flat), ay.to(DEV)
+        if name == 'ay':
+            adj = apart(adj, seq, 0)
+        else:
+            near[name] = apart(flat[name], maps if name in 'BC' else seq, 3)
+        out = []
+        for vals, a in ((near, adj), (flat, ay.to(DEV))):
+            v = [vals[k].detach().requires_grad_(True) for k in NAMES]
+            y, h = ops_ssm.selective_scan(*v[:5], D=v[5], z=v[6], dt_bias=v[7], state=v[8])
+            out.append((y, h, *torch.autograd.grad([y, h], v, [a, al.to(DEV)])))
+        assert all(torch.equal(p, q) for p, q in zip(*out)), name

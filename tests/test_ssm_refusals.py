@@ -237,3 +237,49 @@ def test_library_entry_points_check_the_number_of_steps():
         s = _lib.ScanArgs(x=16, dt=16, A=16, Bm=16, Cm=16, y=16, L=L, B=1, C=1, N=1, G=1)
         sizes = [ctypes.c_longlong(0) for _ in range(3)]
         assert lib.gmt_selective_scan_workspace(ctypes.addressof(s), *(ctypes.addressof(v) for v in sizes)) == want
+
+
+def scan_sizes(**over):
+    """Return code of the workspace entry (which makes the checks of forward and backward calls) and the sizes."""
+    import ctypes
+    a = dict(x=16, dt=16, A=16, Bm=16, Cm=16, L=2, B=1, C=1, N=1, G=1)
+    a.update(over)
+    s = _lib.ScanArgs(**a)
+    n = [ctypes.c_longlong(0) for _ in range(3)]
+    return _lib.lib().gmt_selective_scan_workspace(ctypes.addressof(s), *(ctypes.addressof(v) for v in n))
+
+
+@pytest.mark.parametrize('inside,outside', [
+    (dict(B=2 ** 17, C=2 ** 10 - 1), dict(B=2 ** 17, C=2 ** 10)),                                      # B C < 2^27
+    (dict(C=2 ** 24 - 1), dict(C=2 ** 24)),                                                            # C < 2^24
+    (dict(B=4, N=16, B_t=2 ** 26 - 1, C_t=2 ** 26 - 1), dict(B=4, N=16, B_t=2 ** 26)),                 # pitches of a step
+    (dict(x_t=2 ** 27 - 1, dt_t=2 ** 27 - 1, z=16, z_t=2 ** 27 - 1, dy_t=2 ** 27 - 1), dict(dy_t=2 ** 27))])
+def test_the_limits_of_a_scan_are_the_documented_ones(inside, outside):
+    assert scan_sizes(**inside) == 0
+    assert scan_sizes(**outside) == -2
+
+
+def test_sequences_with_far_steps_are_copied(no_launch, monkeypatch):
+    """A pitch of a step that the kernels do not reach is no refusal: the sequence is copied, and the pitch of a single step does not count."""
+    seen = {}
+
+    def launch(name, args, *a, **k):
+        if name == 'gmt_selective_scan_fwd':
+            s = _lib.ScanArgs.from_address(args)
+            seen.update({n: getattr(s, n) for n in ('x_t', 'dt_t', 'z_t', 'B_t', 'C_t', 'x_b', 'B_b')})
+    monkeypatch.setattr(_lib, 'call', launch)
+    monkeypatch.setattr(_lib, 'stream_of', lambda dev: 0)
+    monkeypatch.setattr(ops_ssm, 'on', lambda dev: ops_ckpt8._HERE)
+    far = torch.empty(2 ** 27 + 64)                         # (untouched memory but for its ends)
+    far[:64] = 1
+    far[-64:] = 2
+
+    def steps(L, pitch, *rest):
+        t = torch.zeros(rest)
+        return far.as_strided((L, *rest), (pitch, *t.stride()))
+    with torch.no_grad():
+        for L, pitch, mapped in ((2, 2 ** 27, 2 ** 26), (2, 2 ** 27 - 1, 2 ** 26 - 1), (1, 2 ** 27, 2 ** 27)):
+            x, m = steps(L, pitch, 3, 8), steps(L, mapped, 3, 5)
+            ops_ssm.selective_scan(x, x, torch.zeros(8, 5), m, m, z=x)
+            want = dict(x_t=24, B_t=15) if pitch == 2 ** 27 and L > 1 else dict(x_t=pitch, B_t=mapped) if L > 1 else dict(x_t=0, B_t=0)
+            assert seen == dict(x_t=want['x_t'], dt_t=want['x_t'], z_t=want['x_t'], B_t=want['B_t'], C_t=want['B_t'], x_b=8, B_b=5), (L, pitch)
