@@ -75,8 +75,8 @@ static inline int scan_check(const gmt_scan_args* a)
         a->B_t < 0 || a->C_t < 0 || a->B_t >= lim / 2 || a->C_t >= lim / 2) return GMT_ERR_UNSUPPORTED;
     if (a->C >= lim || a->x_t >= lim || a->dt_t >= lim || a->z_t >= lim || a->dy_t >= lim || (long long)a->B * a->C >= lim ||
         (long long)a->B * a->G * a->N >= lim / 2) return GMT_ERR_UNSUPPORTED;
-    for (const ScanPlan& p : {fwd_plan(a->L, a->B, a->C, a->N, a->G), bwd_plan(a->L, a->B, a->C, a->N, a->G)})
-        if ((long long)p.cblk * a->G * a->B * p.nseg >= (1LL << 22)) return GMT_ERR_UNSUPPORTED;
+    // A launch stays below 2^32 threads: B G C / G channels padded to whole waves, at most 64 for each of fewer than 2^26 (row, group) pairs of
+    // up to 64 channels, at most twice the 2^27 channels of wider groups; segments and two lanes a channel come with few waves only.
     return GMT_OK;
 }
 

@@ -706,3 +706,20 @@ def test_steps_far_apart(seq, maps):
             y, h = ops_ssm.selective_scan(*v[:5], D=v[5], z=v[6], dt_bias=v[7], state=v[8])
             out.append((y, h, *torch.autograd.grad([y, h], v, [a, al.to(DEV)])))
         assert all(torch.equal(p, q) for p, q in zip(*out)), name
+
+
+def test_more_than_four_million_workgroups():
+    """A group per channel and 4100 rows: 2^22 + 4096 workgroups in the forward pass."""
+    from generative_mouse_trajectories_amd import ops_ssm
+    L, B, C, N = 2, 4100, 1024, 2
+    t, ay, al = scan_inputs(L, B, C, N, C, torch.float32, True, True, True, 9)
+    leaves = {k: t[k].to(DEV).requires_grad_(True) for k in NAMES}
+    outs = ops_ssm.selective_scan(*(leaves[k] for k in NAMES[:5]), D=leaves['D'], z=leaves['z'], dt_bias=leaves['dt_bias'], state=leaves['state'])
+    got = grads(outs, list(leaves.values()), [ay.to(DEV), al.to(DEV)])
+    rl = {k: R.d(t[k]).requires_grad_(True) for k in NAMES}
+    want = R.scan(*(rl[k] for k in NAMES[:8]), None, rl['state'])
+    for what, g, w in zip(('y', 'state'), outs, want):
+        R.close(g, w, 3 * L + N + 45, what)
+    for k, g, w in zip(NAMES, got, grads(want, list(rl.values()), [R.d(ay), R.d(al)])):
+        # a workgroup sums the parameters' gradients over 1025 rows of L steps
+        R.close(g, w, 2 * (3 * L + N + 45) + 45 + (1025 * L + 80 if k in ('A', 'D', 'dt_bias') else 0), 'd' + k)

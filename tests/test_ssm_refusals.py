@@ -252,8 +252,11 @@ def scan_sizes(**over):
 @pytest.mark.parametrize('inside,outside', [
     (dict(B=2 ** 17, C=2 ** 10 - 1), dict(B=2 ** 17, C=2 ** 10)),                                      # B C < 2^27
     (dict(C=2 ** 24 - 1), dict(C=2 ** 24)),                                                            # C < 2^24
+    (dict(B=2 ** 16, C=64, G=64, N=15), dict(B=2 ** 16, C=64, G=64, N=16)),                            # B G N < 2^26
     (dict(B=4, N=16, B_t=2 ** 26 - 1, C_t=2 ** 26 - 1), dict(B=4, N=16, B_t=2 ** 26)),                 # pitches of a step
-    (dict(x_t=2 ** 27 - 1, dt_t=2 ** 27 - 1, z=16, z_t=2 ** 27 - 1, dy_t=2 ** 27 - 1), dict(dy_t=2 ** 27))])
+    (dict(x_t=2 ** 27 - 1, dt_t=2 ** 27 - 1, z=16, z_t=2 ** 27 - 1, dy_t=2 ** 27 - 1), dict(dy_t=2 ** 27)),
+    (dict(B=4096, C=1024, G=1024, N=8), dict(B=4096, C=1024, G=1024, N=16)),                           # a workgroup per row and group: no limit of its own
+    (dict(B=2 ** 25, C=2), dict(B=2 ** 26, C=2))])
 def test_the_limits_of_a_scan_are_the_documented_ones(inside, outside):
     assert scan_sizes(**inside) == 0
     assert scan_sizes(**outside) == -2
