@@ -63,12 +63,18 @@ static inline ScanPlan fwd_plan(int L, int B, int C, int N, int G)
 // 8 states 505 us; N=16, B=256: 4 states a lane 536 us, 8 states 473 us)
 static inline ScanPlan bwd_plan(int L, int B, int C, int N, int G) { return scan_plan(L, B, C, N, G, N > 16 ? 4 : 2, BWD_WAVES); }
 
-static inline int scan_check(const gmt_scan_args* a)
+// what holds of whole sequences and of a single step
+static inline int scan_check_any(const gmt_scan_args* a)
 {
     GMT_CHECK_ARG(a && a->x && a->dt && a->A && a->Bm && a->Cm && a->L > 0 && a->B > 0 && a->C > 0 && a->N > 0 && a->G > 0);
     GMT_CHECK_ARG(a->C % a->G == 0);
     GMT_CHECK_ARG((a->x_scale != nullptr) == (a->dt_scale != nullptr) && (a->z == nullptr || (a->x_scale != nullptr) == (a->z_scale != nullptr)));
-    if (a->N > 32 || a->L > MAX_STEPS) return GMT_ERR_UNSUPPORTED;
+    return a->N > 32 ? GMT_ERR_UNSUPPORTED : GMT_OK;
+}
+static inline int scan_check(const gmt_scan_args* a)
+{
+    if (int rc = scan_check_any(a)) return rc;
+    if (a->L > MAX_STEPS) return GMT_ERR_UNSUPPORTED;
     // byte offsets within four steps (B and C: a chunk) and within a row's kept states are 31 bits
     const long long lim = 1LL << 27;
     if ((long long)a->C * 128 >= 1LL << 31 || a->x_t < 0 || a->dt_t < 0 || a->z_t < 0 || a->dy_t < 0 ||

@@ -378,7 +378,9 @@ extern "C" int gmt_selective_scan_fwd(const gmt_scan_args* a, hipStream_t stream
 
 extern "C" int gmt_selective_scan_step(const gmt_scan_args* a, const unsigned char* active, hipStream_t stream)
 {
-    if (int rc = scan_check(a)) return rc;
+    if (int rc = scan_check_any(a)) return rc;
+    // rows are 64-bit offsets and a loop; 8 channels a workgroup or more, fewer than 2^24 workgroups of 256 threads
+    if (a->C >= 1 << 26 || a->B > MAX_STEPS) return GMT_ERR_UNSUPPORTED;
     GMT_CHECK_ARG(a->y && a->state && a->state_out && a->L == 1 && !a->x_scale);
     return a->bf16 ? step<B16>(a, active, stream) : step<F32>(a, active, stream);
 }

@@ -723,3 +723,19 @@ def test_more_than_four_million_workgroups():
     for k, g, w in zip(NAMES, got, grads(want, list(rl.values()), [R.d(ay), R.d(al)])):
         # a workgroup sums the parameters' gradients over 1025 rows of L steps
         R.close(g, w, 2 * (3 * L + N + 45) + 45 + (1025 * L + 80 if k in ('A', 'D', 'dt_bias') else 0), 'd' + k)
+
+
+@pytest.mark.parametrize('B,C,N,dtype', [(2 ** 22 + 3, 16, 8, 'fp32'), (2 ** 20 + 1, 256, 2, 'bf16')])
+def test_single_steps_of_millions_of_rows(B, C, N, dtype):
+    """The last and the first rows of a step are what a step on these rows alone gives."""
+    from generative_mouse_trajectories_amd import ops_ssm
+    dt = {'fp32': torch.float32, 'bf16': torch.bfloat16}[dtype]
+    gen = torch.Generator(DEV).manual_seed(1)
+    r = lambda *s: torch.randn(*s, device=DEV, generator=gen)  # noqa: E731
+    x, d, z, Bm, Cm, h = r(B, C).to(dt), r(B, C).to(dt), r(B, C).to(dt), r(B, N).to(dt), r(B, N).to(dt), r(B, C, N)
+    A, D, bias = -torch.exp(r(C, N)), r(C), r(C)
+    ends = [h[s].clone() for s in (slice(0, 5), slice(B - 77, B))]
+    y = ops_ssm.selective_scan_step(x, d, A, Bm, Cm, h, D=D, z=z, dt_bias=bias)
+    for s, h0 in zip((slice(0, 5), slice(B - 77, B)), ends):
+        want = ops_ssm.selective_scan_step(x[s], d[s], A, Bm[s], Cm[s], h0, D=D, z=z[s], dt_bias=bias)
+        assert torch.equal(y[s], want) and torch.equal(h[s], h0)

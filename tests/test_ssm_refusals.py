@@ -286,3 +286,14 @@ def test_sequences_with_far_steps_are_copied(no_launch, monkeypatch):
             ops_ssm.selective_scan(x, x, torch.zeros(8, 5), m, m, z=x)
             want = dict(x_t=24, B_t=15) if pitch == 2 ** 27 and L > 1 else dict(x_t=pitch, B_t=mapped) if L > 1 else dict(x_t=0, B_t=0)
             assert seen == dict(x_t=want['x_t'], dt_t=want['x_t'], z_t=want['x_t'], B_t=want['B_t'], C_t=want['B_t'], x_b=8, B_b=5), (L, pitch)
+
+
+def test_the_limits_of_a_single_scan_step_are_its_own():
+    """64-bit indexing over rows: neither a whole sequence's limits nor its workgroups' count.  (-1: past the limits, the output is missing.)"""
+    import ctypes
+    for want, over in ((-1, dict(B=2 ** 20, C=256)), (-1, dict(B=2 ** 22, C=16, N=8)), (-1, dict(B=2 ** 31 - 2 ** 18, C=1, N=32)),
+                       (-1, dict(B=1, C=2 ** 26 - 1, N=32)), (-2, dict(B=1, C=2 ** 26)), (-2, dict(B=1, C=4, N=33)), (-1, dict(B=1, C=4, G=3))):
+        a = dict(x=16, dt=16, A=16, Bm=16, Cm=16, state=16, state_out=16, L=1, N=16, G=1)
+        a.update(over)
+        s = _lib.ScanArgs(**a)
+        assert _lib.lib().gmt_selective_scan_step(ctypes.addressof(s), None, None) == want, over
