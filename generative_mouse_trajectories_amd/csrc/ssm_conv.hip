@@ -358,11 +358,17 @@ Map conv_map(int L, int B, int C, int V)
     return m;
 }
 
-int check(const gmt_conv_args* a)
+int check_any(const gmt_conv_args* a)
 {
     GMT_CHECK_ARG(a && a->x && a->w && a->L > 0 && a->B > 0 && a->C > 0);
-    GMT_CHECK_ARG((long long)a->B * a->C < (1LL << 31));
-    if (a->K < 2 || a->K > 4 || a->L > MAX_STEPS) return GMT_ERR_UNSUPPORTED;
+    return a->K < 2 || a->K > 4 ? GMT_ERR_UNSUPPORTED : GMT_OK;
+}
+// Whole sequences: a launch stays below 2^24 workgroups (vectors and rows are padded to at most twice as many threads; segments come with few
+// threads only).  A single step walks over any number of elements.
+int check(const gmt_conv_args* a)
+{
+    if (int rc = check_any(a)) return rc;
+    if (a->L > MAX_STEPS || (long long)a->B * a->C >= (1LL << 31) || a->C > (1 << 30) - 64) return GMT_ERR_UNSUPPORTED;
     return GMT_OK;
 }
 
@@ -371,7 +377,6 @@ template <class T, int V, int K> int run_fwd(const gmt_conv_args* a, hipStream_t
     using R = typename T::raw;
     const Map m = conv_map(a->L, a->B, a->C, V);
     const long long blocks = (m.units + m.rpb - 1) / m.rpb * m.gx;
-    if (blocks >= (1LL << 24)) return GMT_ERR_UNSUPPORTED;
     auto k = conv_fwd_kernel<T, V, K>;
     hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(THREADS), 0, stream, (const R*)a->x, a->x_t, a->x_b, a->w, a->bias,
                        (const R*)a->state, a->lengths, (R*)a->y, (R*)a->state_out, a->L, a->B, a->C, a->silu, m);
@@ -440,7 +445,7 @@ extern "C" int gmt_causal_conv_bwd(const gmt_conv_args* a, hipStream_t stream)
 
 extern "C" int gmt_causal_conv_step(const gmt_conv_args* a, const unsigned char* active, hipStream_t stream)
 {
-    if (int rc = check(a)) return rc;
+    if (int rc = check_any(a)) return rc;
     GMT_CHECK_ARG(a->y && a->state && a->state_out);
     const int grid = gmt_grid_1d((long long)a->B * a->C, THREADS, 256 * 16);
 #define GMT_STEP(T, K)                                                                                                     \

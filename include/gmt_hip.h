@@ -625,7 +625,8 @@ int gmt_bf16_gen_rollout_bwd(const gmt_bf16_gen_bwd_args* args, hipStream_t stre
  * at or behind a row's length are never read as numbers; y and the gradients are zero there.
  * x_scale (dt_scale, z_scale): exponents of 8-bit checkpoints (gmt_ckpt8_pack); x (dt, z) are then their codes, contiguous.
  * Limits, beyond which GMT_ERR_UNSUPPORTED comes back before anything is launched: L <= 2^31 - 2^18; the scan's
- * x_t, dt_t, z_t, dy_t < 2^27 and B_t, C_t < 2^26 (0 will do for L = 1), B C < 2^27, C < 2^24, B G N < 2^26; its single step: C < 2^26. */
+ * x_t, dt_t, z_t, dy_t < 2^27 and B_t, C_t < 2^26 (0 will do for L = 1), B C < 2^27, C < 2^24, B G N < 2^26; its single step: C < 2^26;
+ * the convolution's B C < 2^31, C <= 2^30 - 64 (its single step: neither). */
 
 /* Short causal convolution, one filter of K = 2 .. 4 taps per channel:  past = [state; x],
  * pre[t] = bias + sum_k w[k] past[t + k],  y[t] = silu(pre[t]) (silu = 0: pre[t]).

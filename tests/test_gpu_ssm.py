@@ -739,3 +739,16 @@ def test_single_steps_of_millions_of_rows(B, C, N, dtype):
     for s, h0 in zip((slice(0, 5), slice(B - 77, B)), ends):
         want = ops_ssm.selective_scan_step(x[s], d[s], A, Bm[s], Cm[s], h0, D=D, z=z[s], dt_bias=bias)
         assert torch.equal(y[s], want) and torch.equal(h[s], h0)
+
+
+def test_convolution_step_of_more_than_2_31_elements():
+    from generative_mouse_trajectories_amd import ops_ssm
+    B, C, K = 2 ** 21 + 5, 1024, 2
+    gen = torch.Generator(DEV).manual_seed(1)
+    x, state = (torch.randn(*s, device=DEV, generator=gen, dtype=torch.bfloat16) for s in ((B, C), (K - 1, B, C)))
+    w, b = torch.randn(C, K, device=DEV, generator=gen), torch.randn(C, device=DEV, generator=gen)
+    ends = (slice(0, 5), slice(B - 77, B))
+    kept = [state[:, s].clone() for s in ends]
+    y = ops_ssm.causal_conv_step(x, state, w, b)
+    for s, c0 in zip(ends, kept):
+        assert torch.equal(y[s], ops_ssm.causal_conv_step(x[s], c0, w, b)) and torch.equal(state[:, s], c0) and torch.equal(c0[-1], x[s])

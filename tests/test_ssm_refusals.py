@@ -297,3 +297,22 @@ def test_the_limits_of_a_single_scan_step_are_its_own():
         a.update(over)
         s = _lib.ScanArgs(**a)
         assert _lib.lib().gmt_selective_scan_step(ctypes.addressof(s), None, None) == want, over
+
+
+def test_the_limits_of_the_convolution():
+    """Whole sequences: B C < 2^31, C <= 2^30 - 64; a single step: neither.  (-1: past the limits, the output is missing.)"""
+    import ctypes
+    lib, n = _lib.lib(), ctypes.c_longlong(0)
+    for want, over in ((0, dict(B=2 ** 21, C=1023)), (-2, dict(B=2 ** 21, C=1024)), (0, dict(B=2 ** 30 - 1, C=2)), (-2, dict(B=2 ** 30, C=2)),
+                       (0, dict(B=1, C=2 ** 30 - 64)), (-2, dict(B=1, C=2 ** 30 - 63))):
+        a = dict(x=16, w=16, L=1, K=4, dy=16, dx=16, dparam=16, bf16=1)
+        a.update(over)
+        a = _lib.ConvArgs(**a)
+        assert lib.gmt_causal_conv_bwd_workspace_floats(ctypes.addressof(a), ctypes.addressof(n)) == want, over
+        assert lib.gmt_causal_conv_fwd(ctypes.addressof(a), None) == (want or -1), over
+        assert lib.gmt_causal_conv_bwd(ctypes.addressof(a), None) == (want or -1), over
+    for want, over in ((-1, dict(B=2 ** 22, C=1024)), (-1, dict(B=2 ** 31 - 2 ** 18, C=4)), (-2, dict(B=1, C=4, K=5))):
+        a = dict(x=16, w=16, state=16, state_out=16, L=1, K=4, bf16=1)
+        a.update(over)
+        a = _lib.ConvArgs(**a)
+        assert lib.gmt_causal_conv_step(ctypes.addressof(a), None, None) == want, over
