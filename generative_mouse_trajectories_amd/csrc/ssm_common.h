@@ -101,31 +101,34 @@ __global__ __launch_bounds__(1024) void slab_reduce_kernel(const float* __restri
 {
     __shared__ float part[16][64];
     const int col = threadIdx.x & 63, grp = threadIdx.x >> 6;
-    const long long i = (long long)blockIdx.x * 64 + col;
-    float s = 0.f;
-    if (i < n) {
-        int p = grp;
-        for (; p + 7 * 16 < P; p += 8 * 16) {
-            float v[8];
+    for (long long i0 = (long long)blockIdx.x * 64; i0 < n; i0 += (long long)gridDim.x * 64) {
+        const long long i = i0 + col;
+        float s = 0.f;
+        if (i < n) {
+            int p = grp;
+            for (; p + 7 * 16 < P; p += 8 * 16) {
+                float v[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = slab[(p + 16 * j) * pitch + i];
+                for (int j = 0; j < 8; ++j) v[j] = slab[(p + 16 * j) * pitch + i];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) s += v[j];
+                for (int j = 0; j < 8; ++j) s += v[j];
+            }
+            for (; p < P; p += 16) s += slab[p * pitch + i];
         }
-        for (; p < P; p += 16) s += slab[p * pitch + i];
-    }
-    part[grp][col] = s;
-    __syncthreads();
-    if (grp == 0 && i < n) {
+        part[grp][col] = s;
+        __syncthreads();
+        if (grp == 0 && i < n) {
 #pragma unroll
-        for (int g = 1; g < 16; ++g) s += part[g][col];
-        out[i] = s;
+            for (int g = 1; g < 16; ++g) s += part[g][col];
+            out[i] = s;
+        }
+        __syncthreads();                                // before `part` is written again
     }
 }
 static inline int launch_slab_reduce(const float* slab, float* out, long long n, long long pitch, int P, hipStream_t stream)
 {
-    if (n >= (1LL << 27)) return GMT_ERR_UNSUPPORTED;   // (16 threads a column: 2^31 threads)
-    hipLaunchKernelGGL(slab_reduce_kernel<0>, dim3((unsigned)((n + 63) / 64)), dim3(1024), 0, stream, slab, out, n, pitch, P);
+    const int grid = gmt_grid_1d(n, 64, 1 << 20);       // (below 2^32 threads)
+    hipLaunchKernelGGL(slab_reduce_kernel<0>, dim3(grid), dim3(1024), 0, stream, slab, out, n, pitch, P);
     GMT_LAUNCH_CHECK();
     return GMT_OK;
 }

@@ -752,3 +752,47 @@ def test_convolution_step_of_more_than_2_31_elements():
     y = ops_ssm.causal_conv_step(x, state, w, b)
     for s, c0 in zip(ends, kept):
         assert torch.equal(y[s], ops_ssm.causal_conv_step(x[s], c0, w, b)) and torch.equal(state[:, s], c0) and torch.equal(c0[-1], x[s])
+
+
+def test_parameter_gradients_of_more_than_2_27_elements():
+    """4 M channels x 32 states, and a convolution of 33 M channels: a step each, against the formulas in float64."""
+    from generative_mouse_trajectories_amd import ops_ssm
+    gen = torch.Generator(DEV).manual_seed(1)
+    r = lambda *s: torch.randn(*s, device=DEV, generator=gen)  # noqa: E731
+
+    def close(got, want, what):
+        err = float((got.double() - want).abs().max()) / float(want.abs().max())
+        assert got.shape == want.shape and err <= 200 * R.U32, (what, err)
+    C, N = 2 ** 22, 32
+    x, dt, A, D, h0 = r(1, 1, C), r(1, 1, C), -torch.exp(r(C, N)), r(C), r(1, C, N)
+    Bm, Cm, ay, al = r(1, 1, N), r(1, 1, N), r(1, 1, C), r(1, C, N)
+    leaves = [t.requires_grad_(True) for t in (x, dt, A, D, h0)]
+    y, h = ops_ssm.selective_scan(x, dt, A, Bm, Cm, D=D, state=h0)
+    dx, ddt, dA, dD, dh = torch.autograd.grad([y, h], leaves, [ay, al])
+    with torch.no_grad():
+        step = torch.log1p(torch.exp(dt.double())).view(C, 1)
+        e = torch.exp(step * A.double())
+        g = Cm.double().view(1, N) * ay.double().view(C, 1) + al.double()[0]
+        close(dh[0], g * e, 'dstate')
+        q = g * e * h0.double()[0]
+        close(dA, q * step, 'dA')
+        gB = (g * Bm.double().view(1, N)).sum(1)
+        close(ddt.view(C), ((q * A.double()).sum(1) + x.double().view(C) * gB) * torch.sigmoid(dt.double()).view(C), 'ddt')
+        close(dx.view(C), step.view(C) * gB + D.double() * ay.double().view(C), 'dx')
+        close(dD, (ay.double() * x.double()).view(C), 'dD')
+    del x, dt, A, D, h0, leaves, y, h, dx, ddt, dA, dD, dh, e, g, q, al
+    C, K = 2 ** 25 + 65, 3
+    x, w, b, s, ay = r(1, 1, C), r(C, K), r(C), r(K - 1, 1, C), r(1, 1, C)
+    assert (K + 1) * C > 2 ** 27
+    leaves = [t.requires_grad_(True) for t in (x, w, b, s)]
+    y, _ = ops_ssm.causal_conv(x, w, b, state=s)
+    dx, dw, db, ds = torch.autograd.grad(y, leaves, ay)
+    with torch.no_grad():
+        past = torch.cat([s, x]).double().view(K, C)
+        pre = (past * w.double().t()).sum(0) + b.double()
+        sig = torch.sigmoid(pre)
+        g = ay.double().view(C) * sig * (1 + pre * (1 - sig))
+        close(db, g, 'db')
+        close(dw, (g * past).t(), 'dw')
+        close(dx.view(C), g * w.double()[:, K - 1], 'dx')
+        close(ds.view(K - 1, C), g * w.double().t()[:K - 1], 'dstate')
