@@ -317,7 +317,6 @@ template <class T> int launch_wgrad8(const void* dY, long long ldy, const signed
                                      int N, int I, int ks, int want_db, hipStream_t stream)
 {
     const long long tiles = (long long)((N + WG_T - 1) / WG_T) * ((I + WG_T - 1) / WG_T), grid = tiles * ks;
-    if (grid >= (1LL << 24) || ldy >= (1LL << 24) || I >= (1 << 24)) return GMT_ERR_UNSUPPORTED;
     hipLaunchKernelGGL(wgrad8_kernel<T>, dim3((unsigned)grid), dim3(256), 0, stream, (const typename T::raw*)dY, ldy, codes, scale, slab, R, N, I,
                        ks, want_db);
     GMT_LAUNCH_CHECK();
@@ -363,6 +362,9 @@ extern "C" int gmt_ckpt8_wgrad(const void* dY, long long ldy, const signed char*
 {
     GMT_CHECK_ARG(dY && codes && scale && dW_db && R > 0 && N > 0 && I > 0 && ldy >= N);
     const int ks = wgrad8_slabs(R, N, I);
+    // 32-bit offsets within a stage of rows; fewer than 2^32 threads; 32-bit numbers of stages
+    const long long tiles = (long long)((N + WG_T - 1) / WG_T) * ((I + WG_T - 1) / WG_T);
+    if (ldy >= (1LL << 24) || I >= (1 << 24) || tiles * ks >= (1LL << 24) || R >= (1LL << 35)) return GMT_ERR_UNSUPPORTED;
     const long long n = (long long)N * I + (want_db ? N : 0), pitch = (long long)N * I + N;
     if (ks > 1 && (!workspace || workspace_floats < ks * pitch)) return GMT_ERR_WORKSPACE;
     float* slab = ks > 1 ? workspace : dW_db;

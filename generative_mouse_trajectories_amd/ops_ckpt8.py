@@ -21,6 +21,8 @@ BLOCK = 32
 DTYPES = (torch.float32, torch.bfloat16)
 MAX_SIZE = (1 << 31) - (1 << 18)             # the kernels' sizes are 32-bit, and so are their sums with a tile's or a segment's
 
+FAR = 1 << 24                                # elements from row to row that the weight gradient's 32-bit offsets do not reach
+
 
 def fits(shape, name: str) -> None:
     """GmtError if one of these sizes would not arrive at the kernels as it is."""
@@ -167,14 +169,14 @@ def wgrad(dY: torch.Tensor, p: Ckpt8, want_db: bool = False) -> Tuple[torch.Tens
     dY = time_major(dY.detach()) if dY.requires_grad else time_major(dY)
     if dY.dim() != 2:
         dY = dY.reshape(R, N)
-    if R > 1 and dY.stride(0) < N:                       # (an expanded gradient: its rows share memory)
+    if R > 1 and not N <= dY.stride(0) < FAR:            # (an expanded gradient, whose rows share memory, or rows out of reach)
         dY = dY.contiguous()
     with on(dev):
         need = ctypes.c_longlong(0)
         L_.call('gmt_ckpt8_wgrad_workspace_floats', R, N, I, ctypes.addressof(need), label='skip')
         ws = dY.new_empty(need.value, dtype=torch.float32)
         out = dY.new_empty(N * I + N, dtype=torch.float32)
-        L_.call('gmt_ckpt8_wgrad', dY.data_ptr(), max(dY.stride(0), N), p.codes.data_ptr(), p.exponents.data_ptr(), out.data_ptr(), R,
+        L_.call('gmt_ckpt8_wgrad', dY.data_ptr(), dY.stride(0) if R > 1 else N, p.codes.data_ptr(), p.exponents.data_ptr(), out.data_ptr(), R,
                 N, I, int(dY.dtype == torch.bfloat16), int(want_db), L_.ptr(ws), need.value, L_.stream_of(dev),
                 label=f'wgrad8_N{N}_I{I}', flops=2.0 * R * N * I)
     return out[:N * I].view(N, I), (out[N * I:] if want_db else None)

@@ -681,7 +681,8 @@ int gmt_selective_scan_step(const gmt_scan_args* args, const unsigned char* acti
  * (s = 255, q = 0).  x [T][B][C] with free pitches (fp32, or bf16) -> codes [T][B][C], scale [T][B][ceil(C / 32)].
  * _unpack: rows of C channels -> out [rows][C].
  * _wgrad: dW[n][i] = sum_r dY[r][n] Xhat[r][i] (fp32 [N][I]) and, if wanted, db[n] = sum_r dY[r][n] behind it (dW_db holds
- * N * I + N floats either way); dY [R][ldy] fp32 or bf16, Xhat [R][I] the checkpoint.  Products exact, sums fp32. */
+ * N * I + N floats either way); dY [R][ldy] fp32 or bf16, Xhat [R][I] the checkpoint.  Products exact, sums fp32.  ldy < 2^24,
+ * I < 2^24, R < 2^35, fewer than 2^24 tiles of 128 x 128. */
 int gmt_ckpt8_pack(const void* x, long long x_t, long long x_b, signed char* codes, unsigned char* scale, long long T, int B,
                    int C, int bf16, hipStream_t stream);
 int gmt_ckpt8_unpack(const signed char* codes, const unsigned char* scale, void* out, long long rows, int C, int bf16,

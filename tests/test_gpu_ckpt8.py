@@ -152,3 +152,16 @@ def test_weight_gradient_of_infinite_and_tiny_dy(dtype):
         mag = R.d(small).abs().t() @ x.double().abs()
         lost = 3 * 2.0 ** -126 * (x.double().abs().sum(0) + Rows) if scale < 2.0 ** -102 else 0.0
         assert bool(((R.d(dW) - R.d(small).t() @ x.double()).abs() <= (Rows / 16 + 64) * R.U32 * mag + lost).all()), scale
+
+
+def test_weight_gradient_of_rows_far_apart():
+    from generative_mouse_trajectories_amd import ops_ckpt8
+    p = ops_ckpt8.pack(spread(7, 40, torch.float32, 2).to(DEV))
+    dy = torch.randn(7, 9, device=DEV)
+    far = torch.zeros(8 * 2 ** 24, device=DEV)
+    for pitch in (2 ** 24 - 1, 2 ** 24 + 3):
+        v = far.as_strided((7, 9), (pitch, 1)).copy_(dy)
+        assert torch.equal(ops_ckpt8.wgrad(v, p)[0], ops_ckpt8.wgrad(dy, p)[0])
+    one = far.as_strided((1, 9), (2 ** 24, 1)).copy_(dy[:1])
+    q = ops_ckpt8.pack(spread(1, 40, torch.float32, 2).to(DEV))
+    assert torch.equal(ops_ckpt8.wgrad(one, q)[0], ops_ckpt8.wgrad(dy[:1], q)[0])

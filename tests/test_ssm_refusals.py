@@ -316,3 +316,25 @@ def test_the_limits_of_the_convolution():
         a.update(over)
         a = _lib.ConvArgs(**a)
         assert lib.gmt_causal_conv_step(ctypes.addressof(a), None, None) == want, over
+
+
+def test_weight_gradient_of_rows_far_apart(no_launch, monkeypatch):
+    """A row pitch that the kernel's 32-bit offsets do not reach is copied, and the pitch of a single row does not count."""
+    seen = []
+    monkeypatch.setattr(_lib, 'call', lambda name, *a, **k: seen.append(a[1]) if name == 'gmt_ckpt8_wgrad' else None)
+    monkeypatch.setattr(_lib, 'stream_of', lambda dev: 0)
+    monkeypatch.setattr(ops_ckpt8, 'on', lambda dev: ops_ckpt8._HERE)
+    far = torch.empty(2 ** 24 + 64)
+    for R, pitch, want in ((2, 2 ** 24 - 1, 2 ** 24 - 1), (2, 2 ** 24, 8), (1, 2 ** 24, 8), (1, 3, 8)):
+        p = ops_ckpt8.Ckpt8(torch.zeros(R, 40, dtype=torch.int8), torch.zeros(R, 2, dtype=torch.uint8), torch.float32)
+        ops_ckpt8.wgrad(far.as_strided((R, 8), (pitch, 1)), p)
+        assert seen.pop() == want and not seen, (R, pitch)
+
+
+def test_the_limits_of_the_weight_gradient():
+    """-4: past the limits, the workspace is missing."""
+    lib = _lib.lib()
+    for want, over in ((-4, dict(ldy=2 ** 24 - 1)), (-2, dict(ldy=2 ** 24)), (-2, dict(N=1, I=2 ** 24))):
+        a = dict(ldy=128, R=1 << 20, N=128, I=128)
+        a.update(over)
+        assert lib.gmt_ckpt8_wgrad(16, max(a['ldy'], a['N']), 16, 16, 16, a['R'], a['N'], a['I'], 0, 0, None, 0, None) == want, over
