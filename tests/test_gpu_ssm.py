@@ -796,3 +796,114 @@ def test_parameter_gradients_of_more_than_2_27_elements():
         close(dw, (g * past).t(), 'dw')
         close(dx.view(C), g * w.double()[:, K - 1], 'dx')
         close(ds.view(K - 1, C), g * w.double().t()[:K - 1], 'dstate')
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('B,C,N,G,aligned', [(8203, 130, 16, 1, True), (8203, 130, 16, 2, False), (8195, 64, 5, 1, True), (2051, 520, 32, 4, True),
+                                             (16389, 33, 8, 3, True), (9000, 260, 4, 1, True)])
+def test_single_steps_of_many_rows(B, C, N, G, aligned, dtype):
+    """Four rows at a time, several groups of them a workgroup, the last of one to three rows; states aligned to 4 bytes; inactive rows."""
+    from generative_mouse_trajectories_amd import ops_ssm
+    t, _, _ = scan_inputs(1, B, C, N, G, dtype, True, True, True, B + C)
+    gen = torch.Generator().manual_seed(2)
+    w, b, cs = torch.randn(C, 4, generator=gen), torch.randn(C, generator=gen), torch.randn(3, B, C, generator=gen).to(dtype)
+    act = torch.rand(B, generator=gen) < 0.8
+    act[-3:] = torch.tensor([True, False, True])
+    ref = {k: R.d(t[k]) for k in NAMES}
+    wu, wc = R.conv(ref['x'], R.d(w), R.d(b), None, R.d(cs))
+    wy, wh = R.scan(*(ref[k] for k in NAMES[:8]), None, ref['state'])
+    v = {k: a.to(DEV) for k, a in t.items()}
+    one = [v[k][0] if k in ('x', 'dt', 'B', 'C') else v[k] for k in NAMES[:5]]
+    for active, aside in ((None, False), (act, True), (act, False)):
+        h = v['state'].clone() if aligned else torch.empty(B * C * N + 1, device=DEV)[1:].view(B, C, N).copy_(v['state'])
+        c = cs.to(DEV)
+        h2 = torch.full_like(h, 7.0) if aside else None
+        c2 = torch.full_like(c, 7.0) if aside else None
+        a = None if active is None else active.to(DEV)
+        y = ops_ssm.selective_scan_step(*one, h, D=v['D'], z=v['z'][0], dt_bias=v['dt_bias'], active=a, state_out=h2)
+        u = ops_ssm.causal_conv_step(one[0], c, w.to(DEV), b.to(DEV), active=a, state_out=c2)
+        h, c = (h2, c2) if aside else (h, c)
+        on = torch.ones(B, dtype=torch.bool) if active is None else act
+        R.close(h[on.to(DEV)], wh[on], N + 48, 'state')
+        R.close(y[on.to(DEV)], wy[0][on], N + 48, 'y')
+        R.close(u[on.to(DEV)], wu[0][on], 49, 'u')
+        assert torch.equal(R.d(c)[:, on], wc[:, on])
+        if active is not None:
+            off = ~act
+            assert torch.equal(R.d(h)[off], ref['state'][off]) and torch.equal(R.d(c)[:, off], R.d(cs)[:, off])
+            assert float(y[off.to(DEV)].abs().max()) == 0 and float(u[off.to(DEV)].abs().max()) == 0
+
+
+@pytest.mark.parametrize('B,C,N,G,dtype,gate,ckpt8', [(300, 256, 16, 1, 'bf16', True, False), (300, 128, 32, 1, 'fp32', False, False),
+                                                      (600, 256, 16, 2, 'fp32', False, True), (300, 128, 20, 1, 'bf16', True, True)])
+def test_many_rows_of_unequal_length_and_many_states(B, C, N, G, dtype, gate, ckpt8):
+    """Rows taken by length with two and four lanes a channel, in both types."""
+    from generative_mouse_trajectories_amd import ops_ssm
+    L, dt = 20, {'fp32': torch.float32, 'bf16': torch.bfloat16}[dtype]
+    t, ay, al = scan_inputs(L, B, C, N, G, dt, gate, True, True, B + N)
+    if ckpt8:                                                # values that 8-bit checkpoints hold exactly
+        t.update({k: (t[k].float() * 32).round().clamp(-100, 100).div(32).to(dt) for k in ('x', 'dt', 'z') if t[k] is not None})
+    lengths = torch.randint(0, L + 1, (B,), generator=torch.Generator().manual_seed(B), dtype=torch.int32)
+    names = [k for k in NAMES if t[k] is not None]
+    leaves = {k: t[k].to(DEV).requires_grad_(True) for k in names}
+    y, last = ops_ssm.selective_scan(*(leaves[k] for k in NAMES[:5]), D=leaves['D'], z=leaves.get('z'), dt_bias=leaves['dt_bias'],
+                                     state=leaves['state'], ckpt8=ckpt8, lengths=lengths.to(DEV))
+    got = dict(zip(names, grads([y, last], [leaves[k] for k in names], [ay.to(DEV), al.to(DEV)])))
+    rl = {k: R.d(t[k]).requires_grad_(True) for k in names}
+    outs = R.scan(*(rl.get(k) for k in NAMES[:8]), lengths, rl['state'])
+    chain = 3 * L + N + 45
+    R.close(y, outs[0], chain, 'y')
+    R.close(last, outs[1], chain, 'final state')
+    want = dict(zip(names, grads(outs, [rl[k] for k in names], [R.d(ay), R.d(al)])))
+    for k in names:
+        extra = {'A': 3 * L + 80, 'D': 3 * L + 80, 'dt_bias': 3 * L + 80, 'B': C // G, 'C': C // G}.get(k, 0)
+        R.close(got[k], want[k], 2 * chain + 45 + extra, 'd' + k)
+
+
+def test_backward_offsets_beyond_32_bits():
+    """2.2e9 elements a sequence, backward: the gradients of the last steps agree with those of calls on the last steps alone (whose adjoint
+    is all there is), from kept states and from 8-bit checkpoints, which hold these inputs exactly; unpacking and the weight gradient."""
+    from generative_mouse_trajectories_amd import ops_ckpt8, ops_ssm
+    L, B, C, N, T = 70000, 32, 1000, 4, 640
+    x = (torch.randint(-100, 101, (L, B, C), device=DEV, dtype=torch.int8, generator=torch.Generator(DEV).manual_seed(1)).to(torch.bfloat16) / 32)
+    assert x.numel() > 2 ** 31
+    x.requires_grad_(True)
+    dy = torch.zeros(L, B, C, device=DEV, dtype=torch.bfloat16)
+    dy[-T:] = torch.randn(T, B, C, generator=torch.Generator(DEV).manual_seed(2), device=DEV).to(torch.bfloat16)
+    w = torch.randn(C, 4, generator=torch.Generator().manual_seed(2)).to(DEV).requires_grad_(True)
+    tail = x.detach()[-T:].clone().requires_grad_(True)
+    for ckpt8 in (False, True):
+        y, _ = ops_ssm.causal_conv(x, w, ckpt8=ckpt8)
+        dx, dw = torch.autograd.grad(y, [x, w], dy)
+        y2, _ = ops_ssm.causal_conv(tail, w, state=x.detach()[-T - 3:-T])
+        dx2, dw2 = torch.autograd.grad(y2, [tail, w], dy[-T:])
+        assert torch.equal(dx[-T:], dx2) and float(dx[:-T - 3].abs().max()) == 0
+        R.close(dw, R.d(dw2), T * B * 2, 'dw')               # the same terms in another order
+        del y, dx, y2, dx2
+    A = -torch.rand(C, N, generator=torch.Generator().manual_seed(3)).to(DEV) * 4
+    Bm = torch.randn(L, B, N, generator=torch.Generator(DEV).manual_seed(4), device=DEV).to(torch.bfloat16)
+    Bt = Bm[-T:].clone()
+    with torch.no_grad():
+        _, h1 = ops_ssm.selective_scan(x[:-T], x[:-T], A, Bm[:-T], Bm[:-T], z=x[:-T])
+    for ckpt8 in (False, True):
+        both = []
+        for seq, m, adj, state in ((x, Bm, dy, None), (tail, Bt, dy[-T:], h1)):
+            v = [t.detach().requires_grad_(True) for t in (seq, seq, m, m, seq)]
+            y, _ = ops_ssm.selective_scan(v[0], v[1], A, v[2], v[3], z=v[4], state=state, ckpt8=ckpt8)
+            both.append([g[-T:].clone() for g in torch.autograd.grad(y, v, adj)])
+            del y, v
+        for name, g, want in zip(('x', 'dt', 'B', 'C', 'z'), *both):
+            # two partitions of one recurrence (a memory of a few hundred steps of 3 roundings), each rounded to bf16: at most a whole step apart
+            R.close(g.float(), R.d(want), 2000 + 2 * 2 ** 16, 'd' + name)
+    p = ops_ckpt8.pack(x)
+    out = ops_ckpt8.unpack(p)
+    assert torch.equal(out[-T:], x[-T:]) and torch.equal(out[:T], x[:T])
+    del out
+    rows = L * B
+    dz = torch.zeros(rows, 8, device=DEV)
+    dz[-100:] = torch.randn(100, 8, generator=torch.Generator(DEV).manual_seed(5), device=DEV)
+    dW, db = ops_ckpt8.wgrad(dz, p, want_db=True)
+    last = x.detach().reshape(rows, C)[-100:]
+    dW2, db2 = dz[-100:].double().t() @ last.double(), dz.double().sum(0)
+    R.close(dW, dW2, 200, 'dW')
+    R.close(db, db2, 200, 'db')
