@@ -304,6 +304,20 @@ def extra_configs(args, dev):
     return res
 
 
+def short_line(out):
+    """The line without its per-kernel tables (some 30 KB with them: whoever keeps only the end of the output loses the headline)."""
+    def without(d):
+        d = {k: v for k, v in d.items() if k != 'kernels'}
+        if d.get('roofline'):
+            d['roofline'] = {k: v for k, v in d['roofline'].items() if k not in ('all_kernels_ms_per_step', 'note')}
+        return d
+    out = without(out)
+    if 'extra_configs' in out:
+        keep = ('metric', 'value', 'unit', 'steps', 'ms_per_step', 'dtype', 'roofline', 'error')
+        out['extra_configs'] = {n: {k: v for k, v in without(e).items() if k in keep} for n, e in out['extra_configs'].items()}
+    return out
+
+
 def main():
     if os.environ.get('GMT_DEBUG_HANG'):              # diagnosis aid: dump every thread's stack if the run stalls
         import faulthandler
@@ -329,7 +343,9 @@ def main():
                     help='do not launch the next D step\'s real-sample critic forward beside the G step\'s BPTT kernel')
     ap.add_argument('--sync-metrics', action='store_true',
                     help='block on the metrics read-back inside every step function (the reference\'s .item() behaviour)')
+    ap.add_argument('--full', action='store_true', help='one line with the tables of all kernels (some 30 KB)')
     args = ap.parse_args()
+    shown = (lambda out: out) if args.full else short_line
     args.steps_given, args.warmup_given = args.steps is not None, args.warmup is not None
     if args.steps is None:
         args.steps = 8
@@ -360,9 +376,9 @@ def main():
     torch.cuda.set_device(local_rank)
     dev = torch.device('cuda', local_rank)
     if args.config == 5:
-        return print(json.dumps(bench_config5(args, dev)), flush=True)
+        return print(json.dumps(shown(bench_config5(args, dev))), flush=True)
     if args.config == 3:
-        return print(json.dumps(bench_config3(args, dev)), flush=True)
+        return print(json.dumps(shown(bench_config3(args, dev))), flush=True)
     pg = None
     force_dist = bool(os.environ.get('GMT_FORCE_DIST'))      # exercise the RCCL path with one rank
     if world > 1 or force_dist:
@@ -492,7 +508,7 @@ def main():
             del metrics[:]
             tr.__dict__.clear()
             out['extra_configs'] = extra_configs(args, dev)
-        print(json.dumps(out), flush=True)
+        print(json.dumps(shown(out)), flush=True)
     if world > 1 or force_dist:
         import torch.distributed as dist
         dist.destroy_process_group()

@@ -5,7 +5,7 @@ tag=$1; shift
 out=gpurun_out
 i=0
 for flags in "$@"; do
-  timeout -k 10 300 python3 bench.py --config 3 $flags > $out/${tag}_v$i.log 2> $out/${tag}_v$i.err
+  timeout -k 10 300 python3 bench.py --full --config 3 $flags > $out/${tag}_v$i.log 2> $out/${tag}_v$i.err
   echo "variant $i [$flags]"; python3 - $out/${tag}_v$i.log <<'PY'
 import json, sys
 for l in open(sys.argv[1]):
