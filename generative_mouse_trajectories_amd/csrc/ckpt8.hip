@@ -3,8 +3,10 @@
 // A row is cut into blocks of 32 channels.  A block is stored as int8 codes q and one exponent byte s = e + 127 and stands for
 // q 2^e:  e = the smallest exponent in -118 .. 121 with max|x| <= 127 * 2^e, q = x 2^-e rounded to nearest even (|q| <= 127).  The
 // scale is a power of two, so that packing rounds once, a code's value is exact in fp32 and in bf16 (7 bits), and its error
-// is at most 2^(e-1), that is max|x| / 127.  The exponent's range keeps 2^-e, and every value that a block of normal numbers stands
-// for, a normal number.  A block that holds an infinity or a NaN stands for NaN throughout: s = 255, q = 0.
+// is at most 2^(e-1), that is max|x| / 127 - but at the ends of the range: a block whose maximum is below 127 2^-119 (1.9e-34) is off by
+// up to 2^-119 (numbers below that become 0), one above 127.5 2^121, where 127 is the largest code, by up to 2^121.  The exponent's range
+// keeps 2^-e, and every value that a block of normal numbers stands for, a normal number.  A block that holds an infinity or a NaN
+// stands for NaN throughout: s = 255, q = 0.
 //
 // Weight gradient: dW[n][i] = sum_r dY[r][n] Xhat[r][i], db[n] = sum_r dY[r][n].  Xhat is exact in bf16; an fp32 dY is exactly
 // the sum of three bf16 numbers (its 24 mantissa bits cut into 8 + 8 + 8; all of them normal numbers from |dY| = 2^-102 on, below

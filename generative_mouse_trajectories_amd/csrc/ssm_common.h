@@ -96,8 +96,7 @@ __device__ __forceinline__ int row_of_rank(const int* lengths, int rank, int B, 
 
 // ---- sum of P slabs, `pitch` floats apart, in a fixed order: out[i] = sum_p slab[p][i], i < n.  64 columns x 16 slab groups a workgroup,
 // eight loads in flight a thread.
-template <int UNUSED = 0>
-__global__ __launch_bounds__(1024) void slab_reduce_kernel(const float* __restrict__ slab, float* __restrict__ out, long long n, long long pitch, int P)
+static __global__ __launch_bounds__(1024) void slab_reduce_kernel(const float* __restrict__ slab, float* __restrict__ out, long long n, long long pitch, int P)
 {
     __shared__ float part[16][64];
     const int col = threadIdx.x & 63, grp = threadIdx.x >> 6;
@@ -128,7 +127,7 @@ __global__ __launch_bounds__(1024) void slab_reduce_kernel(const float* __restri
 static inline int launch_slab_reduce(const float* slab, float* out, long long n, long long pitch, int P, hipStream_t stream)
 {
     const int grid = gmt_grid_1d(n, 64, 1 << 20);       // (below 2^32 threads)
-    hipLaunchKernelGGL(slab_reduce_kernel<0>, dim3(grid), dim3(1024), 0, stream, slab, out, n, pitch, P);
+    hipLaunchKernelGGL(slab_reduce_kernel, dim3(grid), dim3(1024), 0, stream, slab, out, n, pitch, P);
     GMT_LAUNCH_CHECK();
     return GMT_OK;
 }

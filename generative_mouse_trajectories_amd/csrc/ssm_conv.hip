@@ -6,7 +6,7 @@
 // Bound by HBM (2 K + 6 operations per 4 - 8 bytes).  A thread owns V neighbouring channels (16 bytes) of one row and walks
 // along time with the last K - 1 inputs in registers: every element is read once.  A workgroup is 2^k channel vectors x rows,
 // so that narrow rows share a wave.  When rows x channels do not fill the machine, time is cut into segments of 16 steps or
-// more; a segment reads the K - 1 inputs before it again (and the backward pass K - 1 steps behind it).
+// a little fewer (conv_map); a segment reads the K - 1 inputs before it again (and the backward pass K - 1 steps behind it).
 #include "ssm_common.h"
 
 namespace {
@@ -334,8 +334,9 @@ int conv_vec(const gmt_conv_args* a, bool backward)
 }
 
 // Threads are 2^k channel vectors (at most 64) x rows.  Time is cut so that about 2^17 threads run (2 waves on each SIMD, all that
-// the backward pass's registers admit), never below 16 steps: the K - 1 inputs read twice stay under a fifth.  L=128 B=1024
-// C=512 bf16, forward / backward: 2^16 threads 80 / 130 us, 2^17 59 / 111 us, 2^18 60 / 129 us.
+// the backward pass's registers admit), into ceil(L / 16) segments at most: of 16 steps for long sequences, where the K - 1 inputs read twice
+// are under a fifth, of 9 at the least (L = 17: a third at K = 4).  L=128 B=1024 C=512 bf16, forward / backward, when the number was chosen:
+// 2^16 threads 80 / 130 us, 2^17 59 / 111 us, 2^18 60 / 129 us.
 Map conv_map(int L, int B, int C, int V)
 {
     Map m;

@@ -15,8 +15,7 @@
 // Few rows (long prompts) do not fill 1024 SIMDs: time is then cut into segments.  A segment maps its incoming state
 // linearly, h_out = exp(A S) h_in + h_loc, S = the sum of its steps - one float per channel holds the whole decay.  Pass 1 finds
 // (h_loc, S) of every segment, pass 2 chains them, pass 3 runs the segments from their incoming states; the backward pass
-// does the same with the adjoint.  It costs the recurrence twice, so segments are cut only where half of the machine or more
-// would stand idle (scan_plan).
+// does the same with the adjoint.  It costs the recurrence twice, so segments are cut only where few waves run (scan_plan).
 #pragma once
 #include <cfloat>
 #include "ssm_common.h"
@@ -28,7 +27,9 @@ constexpr int CH = 8;                    // steps per chunk; the state before ev
 
 struct ScanPlan { int np, parts, waves, width, chans, cblk, nseg, seglen, nck; };   // chans: channels a workgroup; cblk: workgroups a group
 
-// Padded state count, lanes per channel, workgroup width (at most max_waves waves) and time segments
+// Padded state count, lanes per channel, workgroup width (at most max_waves waves) and time segments: up to 512 waves (the idle ones of a
+// workgroup with fewer channels counted) and four segments of 32 steps or more.  From 513 waves on time is not cut, although up to 1023 waves of the
+// forward pass leave SIMDs idle, and 65 .. 255 workgroups of 8 waves of the backward pass leave CUs idle.
 static inline ScanPlan scan_plan(int L, int B, int C, int N, int G, int parts, int max_waves)
 {
     ScanPlan p;
@@ -143,7 +144,7 @@ __device__ __forceinline__ void lds_barrier() {
 template <int CTRL> __device__ __forceinline__ float dpp(float v) {
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
 }
-constexpr int DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E, DPP_XOR7 = 0x141, DPP_XOR8 = 0x128;     // quad_perm, row_half_mirror, row_ror:8
+constexpr int DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E;             // quad_perm
 
 // (a, b) -> lanes 0 - 31: a summed over bit 5 of the lane, lanes 32 - 63: b
 __device__ __forceinline__ float half32(float a, float b) {

@@ -241,7 +241,7 @@ void scan_bwd_kernel(ScanArgs<T, M> a)
         if (k >= 0) request(t0 + k * CH);
         for (; k >= 0; --k) {
             const int tc = t0 + k * CH;
-            float h[CH + 1][NS], ex[KE ? KE : 1][NS];
+            float h[CH + 1][NS], ex[KE][NS];
             float xv[OWN], st[OWN], sig[OWN], d[OWN], dzf[OWN], out[OWN], gBk[OWN], qAk[OWN];        // dzf: dy silu'(z)
 #pragma unroll
             for (int j = 0; j < OWN; ++j) {
@@ -452,7 +452,6 @@ extern "C" int gmt_selective_scan_bwd(const gmt_scan_args* a, hipStream_t stream
     if (int rc = scan_check(a)) return rc;
     GMT_CHECK_ARG(a->dy && a->dx && a->ddt && a->dB && a->dC && a->dparam && a->workspace && (!a->z || a->dz));
     GMT_CHECK_ARG(a->ck);
-    GMT_CHECK_ARG((long long)a->B * bwd_plan(a->L, a->B, a->C, a->N, a->G).nseg < (1LL << 31));
     if (a->x_scale) {
         if (int rc = scan_states_q8(a, stream)) return rc;
         return a->bf16 ? run<Q8, B16>(a, stream) : run<Q8, F32>(a, stream);

@@ -2,7 +2,8 @@
 32 channels, a quarter of its fp32 bytes, and the weight gradient that reads it.
 
 A block of 32 neighbouring channels of one row stands for q 2^e with |q| <= 127 and the smallest e in -118 .. 121 that reaches
-its largest magnitude: an element is off by at most 2^(e-1).  A block that holds an infinity or a NaN stands for NaN.  `ops.linear`,
+its largest magnitude: an element is off by at most 2^(e-1) (2^e next to fp32's largest number, where 127 2^121 is the last value).  A block
+that holds an infinity or a NaN stands for NaN.  `ops.linear`,
 `ops_ssm.causal_conv` and `ops_ssm.selective_scan` take `ckpt8=True`: their gradients are then those at the values that the
 checkpoints stand for (the outputs are computed from the inputs themselves).
 """
@@ -154,8 +155,8 @@ def unpack(p: Ckpt8, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
 
 def wgrad(dY: torch.Tensor, p: Ckpt8, want_db: bool = False) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """dW = dY^T X over the rows, X [..., I] given as its checkpoint and dY [..., N] (fp32 or bf16) with as many rows: fp32 [N, I];
-    with want_db also db = dY.sum over the rows.  The products are exact, the sums fp32 (csrc/ckpt8.hip); `ops.wgrad` is the same
-    for an fp32 X."""
+    with want_db also db = dY.sum over the rows.  The products are exact (for an fp32 dY from 2^-102 on, below to 2^-126 in dY), the sums fp32
+    (csrc/ckpt8.hip); `ops.wgrad` is the same for an fp32 X."""
     dev = check(p)
     if on_device(dY) != dev:
         raise L_.GmtError('wgrad: dY and the checkpoint are on different devices')
