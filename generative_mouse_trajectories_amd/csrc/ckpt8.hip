@@ -26,7 +26,7 @@ template <class V, class E> __device__ __forceinline__ V load_any(const E* p) { 
 template <class V, class E> __device__ __forceinline__ void store_any(E* p, const V& v) { __builtin_memcpy(p, &v, sizeof(V)); }
 
 // A lane takes 16 bytes of elements, 32 / V lanes share a block; a row's last lanes take what is left of it one by one.
-// Bound by HBM: 210 MB of bf16 in, 105 MB of codes out, and back (200 x 512 rows of 512 channels): 33 and 26 us.
+// Bound by HBM: 105 MB of bf16 in, 54 MB of codes and exponents out, and back (200 x 512 rows of 512 channels): 35 and 26 us.
 template <class T>
 __global__ __launch_bounds__(256)
 void pack_kernel(const typename T::raw* __restrict__ x, long long x_t, long long x_b, signed char* __restrict__ codes,
@@ -304,8 +304,8 @@ void wgrad8_kernel(const typename T::raw* __restrict__ dY, long long ldy, const 
     }
 }
 
-// Slabs of four stages or more, three workgroups a CU in all (R=524288 N=512 I=128 fp32, one box: three with one LDS image each
-// 314 us, two 359 us, two with two images, which need one barrier a stage, 362 us).
+// Slabs of four stages or more, three workgroups a CU in all (R=524288 N=512 I=128 fp32, in one build when it was chosen: three with one LDS
+// image each 314 us, two 359 us, two with two images, which need one barrier a stage, 362 us; now 267 us).
 int wgrad8_slabs(long long R, int N, int I)
 {
     const long long tiles = (long long)((N + WG_T - 1) / WG_T) * ((I + WG_T - 1) / WG_T);

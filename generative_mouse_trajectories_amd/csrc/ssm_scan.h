@@ -9,8 +9,9 @@
 // Time runs in chunks of CH steps, requested one chunk ahead, in three phases: what depends on (t, channel) alone - softplus,
 // gate - for all steps at once, divided between a channel's lanes; the recurrence, step by step; the outputs, divided again.
 // The recurrence is 5 instructions a state and step, one of them an exponential at half rate, and VALU issue is what bounds these
-// kernels: N = 16 forward 150 issue slots for a step of 64 channels, 88 % of them filled (L=256 B=256 C=512 bf16 160 us = 210e9
-// elements a second, 2.7 TB/s); backward 440, 82 % filled (465 us).
+// kernels: N = 16 forward with kept states 165 issue slots for a step of 64 channels, 88 % of them filled (L=256 B=256 C=512 bf16 155 us =
+// 216e9 elements a second); backward 434, 80 % filled (455 us).  Pairs of times beside a choice below compare both sides in one build on one
+// card when it was made; later steps moved both.
 //
 // Few rows (long prompts) do not fill 1024 SIMDs: time is then cut into segments.  A segment maps its incoming state
 // linearly, h_out = exp(A S) h_in + h_loc, S = the sum of its steps - one float per channel holds the whole decay.  Pass 1 finds
